@@ -403,6 +403,81 @@ int32_t wocr_pp_lines(wocr_ctx *ctx, const uint8_t *d_rgb, int32_t w, int32_t h,
  * compacted to the source rows the grey/resize reads.  No reference counterpart (measurement). */
 int32_t wocr_last_transfer_bytes(void *handle, int32_t kind, int64_t *h2d, int64_t *d2h);
 
+/* ---- Operators on device tensors -----------------------------------------------------------
+ * No counterpart in the reference: what a recogniser with attention or a search over its classes
+ * needs beside the graphs above.  Tensors are the caller's device memory; nothing is copied, and
+ * nothing waits.  Work is queued on `stream` (a cudaStream_t of the context's device; NULL: the
+ * context's stream; cudaStreamLegacy for the legacy default stream) and may be captured into a
+ * graph.  The calling thread's current device is left as it was.  Element types are ONNX
+ * TensorProto codes; sums, weights and masses are held in 32 bits or more whatever the type, and
+ * results are rounded once. */
+enum { WOCR_F32 = 1, WOCR_F16 = 10, WOCR_BF16 = 16 };
+
+/* Softmax attention over [batch, heads, tokens, head_dim] tensors of one type.  Strides in
+ * elements for batch, head and token, none negative; the head dimension (1 to 256) is contiguous.
+ * `heads` is a multiple of `kv_heads`: query head h reads key head h / (heads / kv_heads).
+ *   score(i, j) = cap tanh(scale q_i . k_j / cap)   (cap 0: scale q_i . k_j)
+ *                 - slopes[h] |pos_i - j|           (slopes NULL: without)
+ *   pos_i = kv_lens[b] - q_lens[b] + i              (lengths NULL: kv_len, q_len)
+ * Query i sees key j when j < kv_lens[b], and (causal) j <= pos_i or j < prefix[b], and (documents)
+ * q_docs[b][i] == kv_docs[b][j] >= 0.  Keys and values that a query does not see do not reach its
+ * result, NaN and infinities among them.  A query that sees nothing gets zeros; rows of `out` from
+ * q_lens[b] on are left as they were.  Lengths outside the tensors are held to them.  slopes
+ * [heads], prefix, q_lens, kv_lens [batch] and the document ids (a row per batch element, their
+ * strides between rows) are device memory, each nullable (documents: both or neither; a prefix
+ * needs `causal`).  `out` must not overlap the inputs. */
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    const float *slopes;
+    const int32_t *prefix, *q_lens, *kv_lens, *q_docs, *kv_docs;
+    int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+    int64_t q_docs_stride, kv_docs_stride;
+    int32_t type, batch, heads, kv_heads, q_len, kv_len, head_dim, causal;
+    float scale, cap;
+} wocr_attention_args;
+int32_t wocr_attention(wocr_ctx *ctx, const wocr_attention_args *args, void *stream);
+
+/* One step of beam search: of all beams x vocab candidates of a batch element, candidate (j, v)
+ * worth scores[j] + logits[j][v] - log sum_u exp(logits[j][u]), the best out_beams in descending
+ * order, ties to the lowest j * vocab + v.  logits [batch][beams][vocab] with element strides,
+ * tokens contiguous; scores and out_* are [batch][beams] and [batch][out_beams], at most 32 beams
+ * each.  A beam with finished[j] != 0 has one candidate of its own: token `end` at its score.
+ * out_finished: the parent was finished or the token is `end` (end < 0: none ends).  finished and
+ * out_finished are nullable.  Logits that are no number are never chosen before others, infinite
+ * ones count as the largest 32-bit number.  With as many beams out as in, scores and flags may be
+ * updated in place.  Candidates are compared in 64 bits. */
+int32_t wocr_beam_select(wocr_ctx *ctx, const void *logits, int32_t type, int32_t batch, int32_t beams, int32_t vocab,
+                         int64_t batch_stride, int64_t beam_stride, const float *scores, const uint8_t *finished,
+                         int32_t end, int32_t out_beams, float *out_scores, int32_t *out_parents, int32_t *out_tokens,
+                         uint8_t *out_finished, void *stream);
+
+/* The beams' states in their new order: row b * out_beams + j of dst becomes row
+ * b * beams + parents[b][j] of src.  A row is `pieces` pieces of piece_bytes bytes, piece_stride
+ * bytes apart (the live part of a cache, head by head); rows are row_stride bytes apart in src and
+ * dst.  What lies between the pieces is left as it was, and so is a row whose parent is not a beam.
+ * src and dst must not overlap. */
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t pieces, piece_bytes, piece_stride, row_stride;
+} wocr_beam_state;
+int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, int32_t beams, int32_t out_beams,
+                          const wocr_beam_state *states, int32_t n_states, void *stream);
+
+/* CTC prefix beam search over logits [lines][steps][classes] (element strides, classes
+ * contiguous); line i has lens[i] steps (NULL: steps).  A text's mass is the sum over its
+ * alignments of the product of the steps' softmax probabilities; `width` (1 to 31) texts are kept
+ * per step, compared in multiples of 2^-30 of the log mass (32-bit logits below 2^-6 are rounded
+ * to such multiples), ties to texts kept before texts grown, in the order of their beams, then of
+ * classes.  Outputs, the best `paths` texts of each line: tokens [lines][paths][steps], -1 past
+ * a text's end, lengths and scores (log mass) [lines][paths]; a path that does not exist has
+ * length 0 and score -inf.  Logits are cleaned as in wocr_beam_select.  The call's workspace comes
+ * from the device's stream-ordered pool, on `stream`. */
+int32_t wocr_ctc_beam(wocr_ctx *ctx, const void *logits, int32_t type, int32_t lines, int32_t steps, int32_t classes,
+                      int64_t line_stride, int64_t step_stride, const int32_t *lens, int32_t width, int32_t blank,
+                      int32_t paths, int32_t *tokens, int32_t *lengths, float *scores, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

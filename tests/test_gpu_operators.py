@@ -1,0 +1,571 @@
+"""The operators on device tensors against their definitions in 64 bits (tests/_operators.py).
+
+Tolerances, derived before the first run.  u = finfo(type).eps / 2 is the rounding of a type, U = 2^-24 that of 32 bits.
+  attention: a score is off by at most (dim + 8) U times the sum of its products' magnitudes (an fp32 dot product, its scale
+    and cap), plus 4 U of the bias and 8 U of the cap's range; a weight's relative error is twice that (its own and the
+    maximum's) plus 2^-20 for the exponential, and keys U for the sums; in 16 bits the weights are rounded once to the
+    values' type (u, or 2^-25 absolute in fp16's subnormals) and the capped score's fast tanh is off by 2^-18 of the cap.
+    The output is off by that times sum w |v|, and by its own rounding u |out| (2^-25 absolute in fp16).
+  scores of beams: rounded once from 64 bits, log-sum-exps from 32-bit exponentials: 2^-24 |score| + 2^-20.
+  tokens, parents, lengths: equal.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import _operators as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24
+
+
+def randn(shape, type, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(TYPES[type])
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def attention_check(gpu, q, k, v, out=None, stream="torch", scale=None, **kw):
+    """Runs the kernel and holds it to the definition; rows that are not written must keep what they held."""
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    if out is None:
+        out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    before = out.clone()
+    st = torch.cuda.current_stream().cuda_stream if stream == "torch" else stream
+    gpu.attention(q, k, v, out, scale=scale, stream=st, **kw)
+    torch.cuda.synchronize()
+    attention_compare(out, before, q, k, v, scale, **kw)
+    return out
+
+
+def attention_compare(out, before, q, k, v, scale, **kw):
+    want, size, rows = ref.attention(q, k, v, scale, **kw)
+    got = out.cpu().double()
+    assert torch.equal(out.cpu()[~rows], before.cpu()[~rows])
+    # unseen keys may hold anything: magnitudes over the finite ones bound those that count
+    fin = lambda t: torch.nan_to_num(t.cpu().double(), 0, 0, 0)  # noqa: E731
+    G = q.shape[1] // k.shape[1]
+    mag = scale * float(torch.einsum("bhqd,bhkd->bhqk", fin(q).abs(), fin(k).abs().repeat_interleave(G, 1)).max()) if k.shape[2] else 0
+    far = k.shape[2] + q.shape[2]
+    slopes = kw.get("slopes")
+    bias = float(slopes.abs().max()) * far if slopes is not None else 0.0
+    cap = kw.get("cap", 0.0)
+    es = (q.shape[3] + 8) * U * abs(mag) + 4 * U * bias + 8 * U * cap
+    half = q.dtype != torch.float32
+    u = torch.finfo(q.dtype).eps / 2
+    if half:
+        es += cap * 2.0 ** -18
+    ew = 2 * es + 2.0 ** -20 + k.shape[2] * U + (u if half else 0)
+    tol = size * ew + want.abs() * u
+    if q.dtype == torch.float16:
+        tol = tol + 2.0 ** -25 * (1 + k.shape[2] * fin(v).abs().max())
+    tol = tol + 1e-30
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got[rows]), nan[rows])
+    ok = rows[..., None].expand_as(got) & ~nan
+    bad = (got - want).abs() > tol
+    assert not (bad & ok).any(), f"{int((bad & ok).sum())} of {int(ok.sum())} off, worst {float(((got - want).abs() / tol)[ok].max()):.2f} of the tolerance"
+
+
+def qkv(B, H, HK, TQ, TK, D, type, seed=0):
+    return randn((B, H, TQ, D), type, seed, 1.5), randn((B, HK, TK, D), type, seed + 1), randn((B, HK, TK, D), type, seed + 2)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("B, H, HK, TQ, TK, D", [
+    (1, 1, 1, 1, 1, 1), (2, 3, 3, 5, 5, 15), (3, 8, 8, 40, 40, 15), (2, 4, 2, 33, 65, 64), (1, 2, 1, 130, 257, 128),
+    (1, 6, 2, 100, 64, 72), (1, 2, 2, 129, 300, 40), (1, 1, 1, 70, 90, 256), (1, 7, 1, 257, 257, 96), (2, 2, 2, 1, 33, 31),
+    (1, 2, 2, 300, 20, 16), (1, 5, 1, 260, 520, 64),
+])
+def test_attention(gpu, type, B, H, HK, TQ, TK, D):
+    attention_check(gpu, *qkv(B, H, HK, TQ, TK, D, type))
+
+
+MASKS = ["causal", "prefix", "docs", "causal docs", "lens", "causal lens", "cap", "slopes", "cap slopes causal lens", "padding docs",
+         "all"]
+
+
+def masks(kind, B, H, TQ, TK, seed=5):
+    rng = np.random.default_rng(seed)
+    kw = {}
+    if "causal" in kind or kind in ("prefix", "all"):
+        kw["causal"] = True
+    if kind in ("prefix", "all"):
+        kw["prefix"] = i32(rng.integers(-2, TK + 3, B))
+    if "docs" in kind or kind == "all":
+        ids = np.sort(rng.integers(0, 4, (B, TK)), 1).astype(np.int32)
+        if "padding" in kind or kind == "all":
+            ids[:, rng.integers(0, TK, max(1, TK // 5))] = -1
+        kw["kv_docs"] = torch.tensor(ids, device="cuda")
+        qd = np.stack([np.resize(ids[b][max(0, TK - TQ):], TQ) for b in range(B)])
+        if "padding" in kind or kind == "all":
+            qd[:, ::3] = -1
+            qd[:, 1::7] = 9  # an id that no key has
+        kw["q_docs"] = torch.tensor(qd.astype(np.int32), device="cuda")
+    if "lens" in kind or kind == "all":
+        kw["kv_lens"] = i32(np.concatenate([[0], rng.integers(1, TK + 2, B)])[:B] if B > 1 else rng.integers(1, TK + 1, B))
+        kw["q_lens"] = i32(rng.integers(0, TQ + 2, B))
+    if "cap" in kind or kind == "all":
+        kw["cap"] = 4.0
+    if "slopes" in kind or kind == "all":
+        kw["slopes"] = torch.tensor(rng.uniform(-0.02, 0.5, H).astype(np.float32), device="cuda")
+    return kw
+
+
+@pytest.mark.parametrize("kind", MASKS)
+@pytest.mark.parametrize("type, D, TQ, TK", [("f32", 15, 50, 70), ("bf16", 64, 150, 300), ("f16", 128, 280, 280), ("f16", 20, 3, 90),
+                                             ("bf16", 128, 1, 700), ("f32", 64, 2, 400), ("bf16", 32, 300, 130)])
+def test_attention_masks(gpu, kind, type, D, TQ, TK):
+    B, H, HK = 3, 4, 2
+    attention_check(gpu, *qkv(B, H, HK, TQ, TK, D, type, 11), **masks(kind, B, H, TQ, TK))
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("TQ, TK, D", [(1, 200, 64), (64, 200, 15), (200, 300, 64), (260, 400, 128)])
+def test_attention_leaves_what_is_masked_alone(gpu, type, TQ, TK, D):
+    """NaN and infinities behind every kind of mask: behind the keys' end, a causal mask and other documents."""
+    B, H = 2, 2
+    q, k, v = qkv(B, H, H, TQ, TK, D, type, 21)
+    kv_lens = i32([TK - 37, TK - 5])
+    for b, n in enumerate(kv_lens.tolist()):
+        k[b, :, n:] = float("nan")
+        v[b, :, n:] = float("inf")
+    attention_check(gpu, q, k, v, kv_lens=kv_lens)
+    attention_check(gpu, q, k, v, kv_lens=kv_lens, causal=True)
+    # a key that the later queries see and the earlier ones do not
+    if TQ > 1:
+        at = int(kv_lens[0]) - TQ // 2
+        v[0, 0, at, D // 2] = float("nan")
+        v[1, 1, at, 0] = -float("inf")
+        k[1, 0, at] = float("inf")
+        q[1, 0] = q[1, 0].abs()  # scores of +inf: NaN weights, in both
+        attention_check(gpu, q, k, v, kv_lens=kv_lens, causal=True)
+    docs = torch.zeros((B, TK), dtype=torch.int32, device="cuda")
+    docs[:, 10:13] = 5
+    k[:, :, 11], v[:, :, 12], v[:, :, 10, 0] = float("nan"), float("nan"), float("inf")
+    attention_check(gpu, q, k, v, kv_lens=kv_lens, q_docs=torch.zeros((B, TQ), dtype=torch.int32, device="cuda"), kv_docs=docs,
+                    causal=False) if TQ == 1 else attention_check(gpu, q[:, :, :3], k, v, kv_lens=kv_lens, kv_docs=docs,
+                                                                  q_docs=torch.zeros((B, 3), dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [30.0, -30.0, 1000.0, -1000.0])
+def test_attention_of_large_scores(gpu, type, value):
+    """Scores far from zero and far apart: the running maximum decides, nothing overflows."""
+    q, k, v = qkv(1, 2, 1, 150, 200, 64, type, 31)
+    q.fill_(1.0)
+    k.zero_()
+    k[..., 0] = torch.linspace(value, value / 2, 200, device="cuda").to(k.dtype)
+    attention_check(gpu, q, k, v, scale=1.0)
+    attention_check(gpu, q[:, :, :1], k, v, scale=1.0)
+    attention_check(gpu, q, k.flip(2), v, scale=1.0, causal=True)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [15, 64])
+def test_attention_layouts(gpu, type, D):
+    """Packed projections, broadcast keys, padded rows, odd offsets, an output between other values."""
+    B, T, H = 2, 140, 4
+    x = randn((B, T, 3, H, D), type, 41)
+    q, k, v = (x[:, :, i].transpose(1, 2) for i in range(3))
+    out = torch.full((B, T, H + 1, D + 3), 5.0, dtype=x.dtype, device="cuda")
+    view = out[:, :, 1:, 1:D + 1].transpose(1, 2)
+    attention_check(gpu, q, k, v, out=view)
+    assert (out[:, :, 0] == 5).all() and (out[..., 0] == 5).all() and (out[..., D + 1:] == 5).all()
+    pad = randn((B, H, T, D + 1), type, 42)
+    attention_check(gpu, pad[..., 1:], k, pad[..., :D])
+    one = randn((1, 1, T, D), type, 43).expand(B, H, T, D)
+    attention_check(gpu, q, one, one)
+    attention_check(gpu, q[:, :, :1], one, one)
+
+
+def test_attention_of_nothing(gpu):
+    q, k, v = qkv(2, 2, 2, 3, 0, 16, "f32")
+    out = torch.full(q.shape, 7.0, device="cuda")
+    gpu.attention(q, k, v, out, stream=0)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+    gpu.attention(q[:0], k[:0], v[:0], out[:0])
+    gpu.attention(q[:, :, :0], k, v, out[:, :, :0])
+
+
+@pytest.mark.parametrize("type, TQ, TK, D", [("bf16", 1, 3000, 128), ("f16", 4, 5000, 64), ("f32", 1, 4097, 32), ("bf16", 300, 2000, 64)])
+def test_attention_over_long_caches(gpu, type, TQ, TK, D):
+    B, H, HK = 2, 8, 2
+    q, k, v = qkv(B, H, HK, TQ, TK, D, type, 51)
+    attention_check(gpu, q, k, v, causal=True, kv_lens=i32([TK, TK // 2 + 1]))
+    attention_check(gpu, q, k, v, causal=True, cap=20.0, slopes=torch.full((H,), 0.01, device="cuda"), kv_lens=i32([TQ, TK - 3]))
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+def test_attention_offsets_beyond_32_bits(gpu, type):
+    """A head that starts more than 2^32 elements (f16) or bytes (f32) into the cache."""
+    D, TK = 64, 256
+    rows = (1 << 32) // D + TK if type == "f16" else (1 << 30) // D + TK
+    cache = torch.zeros((rows, D), dtype=TYPES[type], device="cuda")
+    far = cache[-TK:]
+    far.copy_(randn((TK, D), type, 61))
+    q = randn((1, 1, 200, D), type, 62)
+    stride = (rows - TK) * D
+    k = torch.as_strided(cache, (2, 1, TK, D), (stride, 0, D, 1))
+    attention_check(gpu, q.expand(2, 1, 200, D), k, k)
+    attention_check(gpu, q[:, :, :1].expand(2, 1, 1, D), k, k)
+
+
+def test_attention_streams_and_graphs(gpu):
+    """On a side stream and the context's own, captured twice and replayed in turn on new values."""
+    import wocr
+    a, b = (qkv(2, 4, 2, 140, 300, 64, "bf16", s) for s in (71, 72))
+    t1, t2 = (qkv(2, 4, 2, 1, 300, 64, "bf16", s) for s in (73, 74))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attention_check(gpu, *a)
+    torch.cuda.synchronize()
+    attention_check(gpu, *a, stream=None)
+    graphs, outs = [], []
+    for args in (a, t1):
+        out = torch.zeros_like(args[0])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            gpu.attention(*args, out, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+        outs.append(out)
+    for args, new in ((a, b), (t1, t2)):
+        for x, y in zip(args, new):
+            x.copy_(y)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for args, out in ((a, outs[0]), (t1, outs[1])):
+        attention_compare(out, out, *args, 64 ** -0.5)
+    assert torch.cuda.current_device() == gpu.device
+    # an allocation that is no torch tensor
+    q, k, v = a
+    wrap = lambda t: wocr.DeviceArray(t.data_ptr(), "bfloat16", t.shape, t.stride())  # noqa: E731
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    gpu.attention(wrap(q), wrap(k), wrap(v), wrap(out))
+    gpu.submit_wait()
+    attention_compare(out, out, q, k, v, 64 ** -0.5)
+
+
+def test_attention_gives_the_same_twice(gpu):
+    for TQ in (1, 200):
+        q, k, v = qkv(2, 8, 2, TQ, 1500, 64, "bf16", 81)
+        outs = [torch.zeros_like(q) for _ in range(3)]
+        for o in outs:
+            gpu.attention(q, k, v, o, stream=0, causal=True)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ---- beam search ---------------------------------------------------------------------------
+def select(gpu, logits, scores, kout, end=-1, finished=None, stream=0):
+    B = logits.shape[0]
+    o = [torch.zeros((B, kout), dtype=t, device="cuda") for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+    gpu.beam_select(logits, scores, o[0], o[1], o[2], end=end, finished=finished, out_finished=o[3], stream=stream)
+    torch.cuda.synchronize()
+    return [t.cpu().numpy() for t in o]
+
+
+def select_check(gpu, logits, scores, kout, end=-1, finished=None):
+    got = select(gpu, logits, scores, kout, end, finished)
+    want = ref.beam_select(logits, scores, kout, end, finished.cpu().numpy() if finished is not None else None)
+    assert (got[1] == want[1]).all() and (got[2] == want[2]).all() and (got[3] == want[3]).all()
+    fin = np.isfinite(want[0])
+    assert (np.isneginf(got[0]) == ~fin).all()
+    assert (np.abs(got[0][fin] - want[0][fin]) <= 2.0 ** -24 * np.abs(want[0][fin]) + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("B, K, V, M", [(1, 1, 1, 1), (1, 1, 40, 32), (3, 4, 97, 4), (2, 32, 97, 32), (2, 8, 18709, 8), (1, 3, 151, 7),
+                                        (5, 2, 5001, 3), (1, 32, 4099, 32), (300, 2, 65, 2), (1, 2, 200003, 4), (1, 32, 70001, 5)])
+def test_beam_select(gpu, type, B, K, V, M):
+    logits = randn((B, K, V), type, 100 + V, 2.0)
+    scores = -torch.rand((B, K), generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") * 6
+    select_check(gpu, logits, scores, M)
+    fin = torch.tensor(np.random.default_rng(V).random((B, K)) < 0.4, device="cuda").to(torch.uint8)
+    select_check(gpu, logits, scores, M, end=V // 2, finished=fin)
+
+
+@pytest.mark.parametrize("B, K, V, M", [(2, 4, 97, 4), (1, 4, 9000, 8), (1, 8, 40000, 32)])
+def test_beam_select_ties_and_masks(gpu, B, K, V, M):
+    """Equal logits everywhere, sorted rows (all of the best in one block's slice), masked classes, first steps of a search."""
+    scores = torch.zeros((B, K), device="cuda")
+    flat = torch.zeros((B, K, V), device="cuda")
+    select_check(gpu, flat, scores, M)
+    select_check(gpu, flat.half(), scores - 3, M, end=0)
+    rise = torch.arange(V, device="cuda", dtype=torch.float32).expand(B, K, V).contiguous() * 2.0 ** -10
+    select_check(gpu, rise, scores, M)
+    select_check(gpu, rise.flip(2).contiguous(), scores, M)
+    select_check(gpu, (rise * 2.0 ** -8).bfloat16(), scores, M)
+    first = scores.clone()
+    first[:, 1:] = -math.inf  # one beam alive
+    x = randn((B, K, V), "f32", 7)
+    select_check(gpu, x, first, M)
+    x[:, :, 3:] = -math.inf   # three classes left
+    select_check(gpu, x, first, M)
+    x[:, 0] = -math.inf       # and none of the first beam's
+    select_check(gpu, x, scores, M)
+    select_check(gpu, torch.full_like(x, -math.inf), scores, M)
+    y = randn((B, K, V), "f32", 8)
+    y[:, :, ::5] = float("nan")
+    y[:, 1, 2] = torch.finfo(torch.float32).min
+    select_check(gpu, y, scores, M)
+    s = scores.clone()
+    s[:, 0] = float("nan")
+    select_check(gpu, y, s, M)
+    every = torch.ones((B, K), dtype=torch.uint8, device="cuda")
+    if M <= K:
+        select_check(gpu, y, torch.linspace(-3, -1, K, device="cuda").expand(B, K).contiguous(), M, end=5, finished=every)
+
+
+def test_beam_select_one_thread_holds_the_best(gpu):
+    """Every good candidate 256 tokens from the next: one thread's, far more than its share."""
+    x = torch.zeros((1, 16, 60000), device="cuda")
+    x[:, :, 5::256] = torch.arange(235, device="cuda") * 2.0 ** -6 + 1
+    select_check(gpu, x, torch.zeros((1, 16), device="cuda"), 32)
+    x[:, :, 5::256] = 1.0
+    select_check(gpu, x, torch.zeros((1, 16), device="cuda"), 32)
+    # scores that drown the logits in 32 bits, not in 64
+    select_check(gpu, randn((2, 4, 3000), "f32", 3, 1e-3), torch.full((2, 4), -4000.0, device="cuda"), 8)
+
+
+def test_beam_select_strides_in_place_and_graph(gpu):
+    B, K, V = 3, 4, 500
+    wide = randn((B, K + 1, 2 * V + 3), "bf16", 9)
+    logits = wide[:, 1:, 3:V + 3]
+    scores = torch.linspace(-2, 0, B * K, device="cuda").reshape(B, K).contiguous()
+    fin = torch.zeros((B, K), dtype=torch.uint8, device="cuda")
+    fin[0, 1] = 1
+    select_check(gpu, logits, scores, K, end=4, finished=fin)
+    want = ref.beam_select(logits, scores, K, 4, fin.cpu().numpy())
+    s, f = scores.clone(), fin.clone()
+    par, tok = (torch.zeros((B, K), dtype=torch.int32, device="cuda") for _ in range(2))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        gpu.beam_select(logits, s, s, par, tok, end=4, finished=f, out_finished=f, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(2):
+        s.copy_(scores)
+        f.copy_(fin)
+        g.replay()
+        torch.cuda.synchronize()
+        assert (par.cpu().numpy() == want[1]).all() and (tok.cpu().numpy() == want[2]).all() and (f.cpu().numpy() == want[3]).all()
+        assert np.allclose(s.cpu().numpy(), want[0], rtol=2.0 ** -22, atol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.uint8])
+@pytest.mark.parametrize("shape, axis, live", [((4, 9, 16), 2, 5), ((4, 9, 16), 0, None), ((3, 7, 5), 2, 7), ((3, 7, 5), 1, 2), ((33,), 0, None),
+                                               ((2, 8, 3), 2, 0), ((1, 300, 64), 2, 299)])
+def test_beam_reorder(gpu, dtype, shape, axis, live):
+    B, N, M = 3, 4, 5
+    rng = np.random.default_rng(1)
+    par = rng.integers(0, N, (B, M)).astype(np.int32)
+    par[1, 2], par[2, 0] = -1, N  # no such beams
+    states = []
+    for i in range(3):
+        src = torch.randint(0, 200, (B * N,) + shape, device="cuda").to(dtype)
+        dst = torch.full((B * M,) + shape, 77, device="cuda").to(dtype)
+        states.append((src, dst))
+    # one that starts at an odd place of a larger allocation
+    raw = torch.randint(0, 200, (B * N * int(np.prod(shape)) + 1,), device="cuda").to(dtype)
+    states.append((raw[1:].reshape((B * N,) + shape), torch.full((B * M,) + shape, 77, device="cuda").to(dtype)))
+    want = []
+    for src, dst in states:
+        w = dst.clone()
+        for b in range(B):
+            for j in range(M):
+                if 0 <= par[b, j] < N:
+                    cut = (slice(None),) * (axis - 1) + (slice(0, live),) if axis and live is not None else ()
+                    w[b * M + j][cut] = src[b * N + int(par[b, j])][cut]
+        want.append(w)
+    gpu.beam_reorder(torch.tensor(par, device="cuda"), states, axis=axis, live=live, stream=0)
+    torch.cuda.synchronize()
+    for (_, dst), w in zip(states, want):
+        assert torch.equal(dst, w)
+
+
+def test_beam_reorder_of_many(gpu):
+    """More states than a launch takes, more rows than a grid's second dimension."""
+    par = i32(np.random.default_rng(2).integers(0, 3, (2, 3)))
+    states = [(torch.randn((6, 10 + i), device="cuda"), torch.zeros((6, 10 + i), device="cuda")) for i in range(130)]
+    gpu.beam_reorder(par, states, stream=0)
+    rows = (torch.arange(2, device="cuda")[:, None] * 3 + par).reshape(-1)
+    for src, dst in states:
+        assert torch.equal(dst, src[rows])
+    B, N = 3000, 31
+    par = torch.randint(0, N, (B, N), device="cuda", dtype=torch.int32)
+    src = torch.randn((B * N, 3), device="cuda")
+    dst = torch.zeros_like(src)
+    gpu.beam_reorder(par, [(src, dst)], stream=0)
+    assert torch.equal(dst, src[(torch.arange(B, device="cuda")[:, None] * N + par).reshape(-1)])
+
+
+# ---- CTC -----------------------------------------------------------------------------------
+def search(gpu, logits, lens, width, blank, paths, stream=0):
+    n, t, _ = logits.shape
+    o = (torch.full((n, paths, t), 99, dtype=torch.int32, device="cuda"), torch.full((n, paths), 99, dtype=torch.int32, device="cuda"),
+         torch.zeros((n, paths), device="cuda"))
+    gpu.ctc_beam(logits, *o, lens=lens, width=width, blank=blank, stream=stream)
+    torch.cuda.synchronize()
+    return [x.cpu().numpy() for x in o]
+
+
+def search_check(gpu, logits, width, lens=None, blank=0, paths=None):
+    paths = paths or width
+    got = search(gpu, logits, lens, width, blank, paths)
+    search_compare(got, logits, lens, width, blank, paths)
+
+
+def search_compare(got, logits, lens, width, blank, paths):
+    want = ref.ctc_beam(logits, lens.cpu().numpy() if lens is not None else None, width, blank, paths)
+    assert (got[1] == want[1]).all() and (got[0] == want[0]).all()
+    fin = np.isfinite(want[2])
+    assert (np.isneginf(got[2]) == ~fin).all()
+    # a log-sum-exp per step from 32-bit exponentials, each off by less than 2^-20
+    assert (np.abs(got[2][fin] - want[2][fin]) <= 2.0 ** -24 * np.abs(want[2][fin]) + logits.shape[1] * 2.0 ** -20).all()
+
+
+def peaky(n, t, v, type, seed):
+    """Steps near certain of a class, the blank more often than not."""
+    rng = np.random.default_rng(seed)
+    x = rng.normal(size=(n, t, v)) * 1.5
+    hit = np.where(rng.random((n, t)) < 0.5, 0, rng.integers(0, v, (n, t)))
+    np.put_along_axis(x, hit[..., None], np.take_along_axis(x, hit[..., None], 2) + rng.uniform(1, 10, (n, t, 1)), 2)
+    return torch.tensor(x.astype(np.float32), device="cuda").to(TYPES[type])
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n, t, v, width", [(1, 1, 1, 1), (1, 1, 2, 4), (2, 12, 3, 31), (3, 30, 12, 8), (2, 70, 40, 5), (1, 9, 300, 16),
+                                            (2, 5, 2000, 31), (1, 130, 5, 3)])
+def test_ctc_beam(gpu, type, n, t, v, width):
+    search_check(gpu, peaky(n, t, v, type, n + t + v), width)
+    lens = i32(np.random.default_rng(t).integers(0, t + 2, n))
+    search_check(gpu, peaky(n, t, v, type, 5), width, lens=lens, blank=v - 1, paths=max(1, width // 2))
+
+
+def test_ctc_beam_repeats_and_merges(gpu):
+    """Two classes and wide beams: texts with repeated classes, reached from several others at once."""
+    x = randn((4, 25, 3), "f32", 1, 0.7)
+    search_check(gpu, x, 20)
+    search_check(gpu, x.bfloat16(), 20)
+    search_check(gpu, torch.zeros_like(x), 20)  # every alignment alike: ties all the way
+    search_check(gpu, torch.zeros((2, 6, 700), device="cuda"), 12)
+    search_check(gpu, randn((2, 20, 4), "bf16", 3, 4.0).round(), 15)
+
+
+def test_ctc_beam_of_masked_and_odd_logits(gpu):
+    x = peaky(3, 14, 50, "f32", 8)
+    x[:, :, 20:] = -math.inf
+    search_check(gpu, x, 8)
+    x[:, :, 7] = float("nan")
+    search_check(gpu, x, 8)
+    x[:, :, 5] = -1e9
+    x[1, 3] = 2.0 ** -9 * torch.arange(50, device="cuda")
+    x[1, 4] = 2.0 ** -33 * torch.arange(50, device="cuda")
+    search_check(gpu, x, 8)
+    x[1, 5] = -math.inf  # a step that allows nothing
+    search_check(gpu, x, 8)
+    search_check(gpu, peaky(2, 14, 50, "f32", 9) * 1e4, 8)
+    lens = i32([0, -3])
+    search_check(gpu, peaky(2, 6, 20, "f32", 9), 3, lens=lens)
+    empty = search(gpu, torch.zeros((2, 0, 5), device="cuda"), None, 3, 0, 2)
+    assert (empty[1] == 0).all() and (empty[2][:, 0] == 0).all() and np.isneginf(empty[2][:, 1]).all()
+
+
+@pytest.mark.parametrize("type, v", [("f32", 18709), ("bf16", 18709), ("f32", 70001), ("f16", 6000)])
+def test_ctc_beam_over_dictionaries(gpu, type, v):
+    x = peaky(2, 4, v, type, v)
+    search_check(gpu, x, 4)
+    rise = (torch.arange(v, device="cuda") * 2.0 ** -10).expand(1, 2, v).to(TYPES[type]).contiguous()
+    search_check(gpu, rise, 4)
+    one = torch.zeros((1, 2, v), device="cuda")
+    one[:, :, 9::256] = torch.arange(len(range(9, v, 256)), device="cuda") * 2.0 ** -6 + 1  # all in one thread's hands
+    search_check(gpu, one.to(TYPES[type]), 5)
+
+
+def test_ctc_beam_strides_streams_and_graphs(gpu):
+    """Two captured calls share nothing: replayed in turn on new logits, beside a call on another stream."""
+    wide = peaky(3, 20, 45, "f32", 4)
+    search_check(gpu, wide[:, ::2, 3:40], 6)
+    xs = [peaky(3, 20, 30, "f32", s) for s in (1, 2)]
+    outs, graphs = [], []
+    for x in xs:
+        o = (torch.zeros((3, 4, 20), dtype=torch.int32, device="cuda"), torch.zeros((3, 4), dtype=torch.int32, device="cuda"),
+             torch.zeros((3, 4), device="cuda"))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            gpu.ctc_beam(x, *o, width=6, stream=torch.cuda.current_stream().cuda_stream)
+        outs.append(o)
+        graphs.append(g)
+    for s, x in zip((5, 6), xs):
+        x.copy_(peaky(3, 20, 30, "f32", s))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    third = peaky(3, 20, 30, "f32", 7)
+    o3 = [torch.zeros_like(t) for t in outs[0]]
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        with torch.cuda.stream(side):
+            gpu.ctc_beam(third, *o3, width=6, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    for x, o in zip(xs + [third], outs + [o3]):
+        search_compare([t.cpu().numpy() for t in o], x, None, 6, 0, 4)
+
+
+# ---- together ------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_a_decoder_with_beams(gpu, type):
+    """A decoder over a line's features: every step attends over the cache, selects and puts the cache in the beams' order;
+    the same texts come out when each step attends over the whole of each beam's own text again."""
+    B, K, H, D, V, F, STEPS = 2, 3, 4, 16, 30, 11, 6
+    t = TYPES[type]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    emb, wq, wk, wv, wo = rnd(V, H * D), rnd(H * D, H * D) / 8, rnd(H * D, H * D) / 8, rnd(H * D, H * D) / 8, rnd(H * D, V) / 2
+    feats = rnd(B, F, H * D)
+    S = F + STEPS
+    heads = lambda x: x.reshape(x.shape[0], -1, H, D).transpose(1, 2)  # noqa: E731
+    cache = [torch.full((B * K, H, S, D), float("nan"), device="cuda", dtype=t) for _ in range(4)]
+    for c, w in zip(cache[:2], (wk, wv)):
+        c[:, :, :F] = heads(feats @ w).to(t).repeat_interleave(K, 0)
+    scores = torch.full((B, K), -math.inf, device="cuda")
+    scores[:, 0] = 0
+    done = torch.zeros((B, K), dtype=torch.uint8, device="cuda")
+    par, tok = (torch.zeros((B, K), dtype=torch.int32, device="cuda") for _ in range(2))
+    texts = [[[0]] * K for _ in range(B)]
+    st = torch.cuda.current_stream().cuda_stream
+    for i in range(STEPS):
+        x = emb[tok.reshape(-1).long()]
+        cache[0][:, :, F + i] = (x @ wk).reshape(B * K, H, D).to(t)
+        cache[1][:, :, F + i] = (x @ wv).reshape(B * K, H, D).to(t)
+        q = heads((x @ wq)[:, None]).to(t)
+        out = torch.empty((B * K, H, 1, D), device="cuda", dtype=t)
+        gpu.attention(q, cache[0], cache[1], out, causal=True, kv_lens=torch.full((B * K,), F + i + 1, dtype=torch.int32, device="cuda"), stream=st)
+        logits = (out.float().reshape(B, K, H * D) @ wo).contiguous()
+        # the same from the texts alone, in one causal pass over features and text
+        for b in range(B):
+            for j in range(K):
+                if scores[b, j] == -math.inf:
+                    continue
+                xs = torch.cat([feats[b], emb[torch.tensor(texts[b][j], device="cuda")]])
+                whole, _, _ = ref.attention(*[heads((xs @ w)[None]).to(t) for w in (wq, wk, wv)], D ** -0.5, causal=True)
+                got = out[b * K + j, :, 0].cpu().double()
+                assert (got - whole[0, :, -1]).abs().max() < (0.03 if type == "bf16" else 1e-5)
+        want = ref.beam_select(logits, scores, K, 1, done.cpu().numpy())
+        gpu.beam_select(logits, scores, scores, par, tok, end=1, finished=done, out_finished=done, stream=st)
+        gpu.beam_reorder(par, [(cache[0], cache[2]), (cache[1], cache[3])], axis=2, live=F + i + 1, stream=st)
+        cache = [cache[2], cache[3], cache[0], cache[1]]
+        p, k = par.cpu().numpy(), tok.cpu().numpy()
+        assert (p == want[1]).all() and (k == want[2]).all()
+        texts = [[texts[b][p[b, j]] + [int(k[b, j])] for j in range(K)] for b in range(B)]

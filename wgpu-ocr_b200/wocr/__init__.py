@@ -9,6 +9,7 @@ from .api import (Batch, Detector, Gpu, NdGraph, OcrsPipeline, Pending, PPPipeli
                   ocrs_decode, pad_line, pp_decode, text_lines)
 from .model import Model, Node
 from .onnx import load_onnx, parse_onnx
+from .ops import DeviceArray
 
 __all__ = ["Gpu", "Batch", "Pending", "Detector", "Recognizer", "NdGraph", "PPPipeline", "OcrsPipeline", "text_lines", "pad_line", "WocrError", "Model", "Node", "ocrs_decode",
-           "pp_decode", "load_pp_dictionary", "lib", "LIB_PATH", "EXPORTS", "load_onnx", "parse_onnx"]
+           "pp_decode", "load_pp_dictionary", "lib", "LIB_PATH", "EXPORTS", "load_onnx", "parse_onnx", "DeviceArray"]

@@ -133,6 +133,12 @@ _SIGS = [
                                 c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
     ("wocr_pp_lines", c_i32, [c_void_p, c_void_p, c_i32, c_i32, c_void_p, c_i32, c_i32, c_void_p, c_i64, c_void_p,
                               c_void_p, c_void_p, P(c_i32), P(c_i64)]),
+    ("wocr_attention", c_i32, [c_void_p, c_char_p, c_void_p]),
+    ("wocr_beam_select", c_i32, [c_void_p, c_void_p, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_void_p, c_void_p, c_i32,
+                                 c_i32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("wocr_beam_reorder", c_i32, [c_void_p, c_void_p, c_i32, c_i32, c_i32, c_char_p, c_i32, c_void_p]),
+    ("wocr_ctc_beam", c_i32, [c_void_p, c_void_p, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_void_p, c_i32, c_i32, c_i32,
+                              c_void_p, c_void_p, c_void_p, c_void_p]),
 ]
 
 EXPORTS = [s[0] for s in _SIGS]

@@ -18,9 +18,10 @@ import numpy as np
 
 from . import _lib as L
 from .model import Model
+from .ops import DeviceOps
 
 
-class Gpu:
+class Gpu(DeviceOps):
     """`Gpu::new(lines)` (src/gpu.rs:850): one CUDA device, one stream, a pooled allocator."""
 
     def __init__(self, lines: int = 8, device: int = 0):

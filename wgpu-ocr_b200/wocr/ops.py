@@ -1,0 +1,199 @@
+"""Operators on device tensors: attention, beam search's selection and reordering, CTC prefix beam search.
+
+They take CUDA tensors of the context's device: torch tensors, or `DeviceArray`s around any other allocation.  Nothing is
+copied and nothing waits: work is queued on `stream`, a cudaStream_t as an int (0: the legacy default stream, as torch's
+`current_stream().cuda_stream` names it; None: the context's own stream).  Outputs are the caller's tensors.  A tensor must
+stay allocated until the stream has passed the call.
+"""
+from __future__ import annotations
+
+import struct
+from typing import Optional, Sequence, Tuple
+
+from . import _lib as L
+
+F32, F16, BF16, I32, U8 = 1, 10, 16, 6, 2  # ONNX TensorProto codes
+_NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int32": I32, "uint8": U8, "bool": U8}
+_SIZES = {F32: 4, F16: 2, BF16: 2, I32: 4, U8: 1}
+_codes = {}  # dtype object -> code
+_ARGS = struct.Struct("10Q14q8i2f")
+_STATE = struct.Struct("2Q4q")
+_LEGACY = 1  # cudaStreamLegacy
+
+
+class DeviceArray:
+    """A device allocation of the caller's as a tensor: `dtype` by name, `strides` in elements (None: dense)."""
+
+    def __init__(self, ptr: int, dtype: str, shape: Sequence[int], strides: Optional[Sequence[int]] = None, device: int = 0):
+        self.ptr, self.dtype, self.shape, self.device = int(ptr), dtype, tuple(shape), device
+        if strides is None:
+            dense, n = [], 1
+            for d in reversed(self.shape):
+                dense.append(n)
+                n *= d
+            strides = dense[::-1]
+        self._strides = tuple(strides)
+
+    def data_ptr(self) -> int:
+        return self.ptr
+
+    def stride(self) -> Tuple[int, ...]:
+        return self._strides
+
+    def get_device(self) -> int:
+        return self.device
+
+
+def _code(x) -> int:
+    try:
+        return _codes[x.dtype]
+    except KeyError:
+        name = str(x.dtype).rsplit(".", 1)[-1]
+        if name not in _NAMES:
+            raise ValueError(f"element type {x.dtype} is not supported")
+        _codes[x.dtype] = _NAMES[name]
+        return _codes[x.dtype]
+
+
+def _ptr(gpu, x, name: str) -> int:
+    if x.get_device() != gpu.device:
+        raise ValueError(f"{name} is not on device {gpu.device}")
+    return x.data_ptr()
+
+
+def _dense(gpu, x, name: str, code: int, shape) -> int:
+    """The address of a dense tensor of one type and shape (0 for None)."""
+    if x is None:
+        return 0
+    if _code(x) != code or tuple(x.shape) != shape:
+        raise ValueError(f"{name}: expected type {code} of shape {shape}, got {x.dtype} {tuple(x.shape)}")
+    n = 1
+    for d, s in zip(reversed(shape), reversed(x.stride())):
+        if d != 1 and s != n and 0 not in shape:
+            raise ValueError(f"{name} is not contiguous")
+        n *= d
+    return _ptr(gpu, x, name)
+
+
+def _rows(gpu, x, name: str, code: int, shape) -> Tuple[int, int]:
+    """The address and row stride of a [rows, n] tensor whose rows are contiguous."""
+    if x is None:
+        return 0, 0
+    if _code(x) != code or tuple(x.shape) != shape:
+        raise ValueError(f"{name}: expected type {code} of shape {shape}, got {x.dtype} {tuple(x.shape)}")
+    s = x.stride()
+    if shape[1] > 1 and s[1] != 1:
+        raise ValueError(f"{name}: rows are not contiguous")
+    return _ptr(gpu, x, name), s[0]
+
+
+def _inner(x, name: str):
+    """The strides of a tensor whose last dimension is contiguous."""
+    s = x.stride()
+    if x.shape[-1] > 1 and s[-1] != 1:
+        raise ValueError(f"{name}: the last dimension is not contiguous")
+    return s
+
+
+def _stream(stream) -> Optional[int]:
+    return None if stream is None else (stream or _LEGACY)
+
+
+class DeviceOps:
+    """The operators as methods of `Gpu`."""
+
+    def attention(self, q, k, v, out, scale: Optional[float] = None, cap: float = 0.0, slopes=None, causal: bool = False,
+                  prefix=None, q_lens=None, kv_lens=None, q_docs=None, kv_docs=None, stream: Optional[int] = None):
+        """Softmax attention (`wocr_attention`): q, out [batch, heads, queries, dim], k, v [batch, kv_heads, keys, dim]
+        of one type (float32, float16, bfloat16) and any strides but for a contiguous last dimension of 1 to 256.
+
+        score = cap tanh(scale q.k / cap) - slopes[h] |distance|; query i of batch element b stands at position
+        kv_lens[b] - q_lens[b] + i among its keys and sees those below kv_lens[b]; with `causal` up to its own position
+        or below prefix[b]; with documents those whose id is its own, negative ids none.  scale None: dim ** -0.5.
+        slopes float32 [heads]; prefix, q_lens, kv_lens int32 [batch]; q_docs [batch, queries], kv_docs [batch, keys]
+        int32.  A query that sees nothing gets zeros; rows from q_lens[b] on are left as they were."""
+        code = _code(q)
+        if _code(k) != code or _code(v) != code or _code(out) != code:
+            raise ValueError("q, k, v and out have different types")
+        qs, ks = q.shape, k.shape
+        if len(qs) != 4 or len(ks) != 4 or v.shape != ks or out.shape != qs or qs[0] != ks[0] or qs[3] != ks[3]:
+            raise ValueError(f"attention shapes: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)}, out {tuple(out.shape)}")
+        b, h, tq, d = qs
+        hk, tk = ks[1], ks[2]
+        a, c, e, f = _inner(q, "q"), _inner(k, "k"), _inner(v, "v"), _inner(out, "out")
+        qd, qds = (0, 0) if q_docs is None else _rows(self, q_docs, "q_docs", I32, (b, tq))
+        kd, kds = (0, 0) if kv_docs is None else _rows(self, kv_docs, "kv_docs", I32, (b, tk))
+        args = _ARGS.pack(_ptr(self, q, "q"), _ptr(self, k, "k"), _ptr(self, v, "v"), _ptr(self, out, "out"),
+                          0 if slopes is None else _dense(self, slopes, "slopes", F32, (h,)),
+                          0 if prefix is None else _dense(self, prefix, "prefix", I32, (b,)),
+                          0 if q_lens is None else _dense(self, q_lens, "q_lens", I32, (b,)),
+                          0 if kv_lens is None else _dense(self, kv_lens, "kv_lens", I32, (b,)), qd, kd,
+                          a[0], a[1], a[2], c[0], c[1], c[2], e[0], e[1], e[2], f[0], f[1], f[2], qds, kds,
+                          code, b, h, hk, tq, tk, d, causal, d ** -0.5 if scale is None else scale, cap)
+        L.check(L.lib().wocr_attention(self.h, args, _stream(stream)))
+
+    def beam_select(self, logits, scores, out_scores, out_parents, out_tokens, end: int = -1, finished=None,
+                    out_finished=None, stream: Optional[int] = None):
+        """One selection of beam search (`wocr_beam_select`): logits [batch, beams, vocab] (float32, float16, bfloat16,
+        last dimension contiguous), scores float32 [batch, beams]; the best candidates' scores (float32), parent beams and
+        tokens (int32), [batch, out_beams] each, best first, ties to the lowest beam * vocab + token.  `finished` (uint8
+        [batch, beams]) beams keep their score and give `end`; out_finished (uint8) says which of the chosen have ended."""
+        if len(logits.shape) != 3 or len(out_scores.shape) != 2:
+            raise ValueError("logits [batch, beams, vocab] and out_scores [batch, beams] expected")
+        b, n, v = logits.shape
+        m = out_scores.shape[1]
+        s = _inner(logits, "logits")
+        L.check(L.lib().wocr_beam_select(
+            self.h, _ptr(self, logits, "logits"), _code(logits), b, n, v, s[0], s[1],
+            _dense(self, scores, "scores", F32, (b, n)), _dense(self, finished, "finished", U8, (b, n)) or None, end, m,
+            _dense(self, out_scores, "out_scores", F32, (b, m)), _dense(self, out_parents, "out_parents", I32, (b, m)),
+            _dense(self, out_tokens, "out_tokens", I32, (b, m)),
+            _dense(self, out_finished, "out_finished", U8, (b, m)) or None, _stream(stream)))
+
+    def beam_reorder(self, parents, states, axis: int = 0, live: Optional[int] = None, stream: Optional[int] = None):
+        """The states of the chosen beams in their new order (`wocr_beam_reorder`): `parents` int32 [batch, out_beams] as
+        beam_select gives them; `states` pairs of tensors (src [batch * beams, ...], dst [batch * out_beams, ...]), dense
+        and alike but for the first dimension.  With `axis` > 0 only the first `live` entries along it are copied (a
+        cache's tokens); the rest of dst, and rows whose parent is not a beam, are left as they were."""
+        if len(parents.shape) != 2:
+            raise ValueError("parents [batch, beams] expected")
+        b, m = parents.shape
+        n, parts = None, []
+        for src, dst in states:
+            shape = tuple(src.shape)
+            size = _SIZES[_code(src)]
+            if not 0 <= axis < len(shape):
+                raise ValueError(f"axis {axis} of a state of shape {shape}")
+            rows = shape[0] // b if b else 1
+            if shape[0] != rows * b or tuple(dst.shape) != (b * m,) + shape[1:] or (n is not None and rows != n):
+                raise ValueError(f"state shapes {shape} and {tuple(dst.shape)} for {b} x {m} parents")
+            n = rows
+            pieces, inner = 1, 1
+            for x in shape[1:axis]:
+                pieces *= x
+            for x in shape[max(axis, 0) + 1:]:
+                inner *= x
+            full = inner * size if axis == 0 else shape[axis] * inner * size
+            part = full if axis == 0 or live is None else live * inner * size
+            if axis and live is not None and not 0 <= live <= shape[axis]:
+                raise ValueError(f"live {live} of a state of shape {shape}")
+            parts.append(_STATE.pack(_dense(self, src, "state", _code(src), shape),
+                                     _dense(self, dst, "state", _code(src), tuple(dst.shape)), pieces, part, full, pieces * full))
+        L.check(L.lib().wocr_beam_reorder(self.h, _dense(self, parents, "parents", I32, (b, m)), b, n or 1, m, b"".join(parts),
+                                          len(parts), _stream(stream)))
+
+    def ctc_beam(self, logits, tokens, lengths, scores, lens=None, width: int = 8, blank: int = 0,
+                 stream: Optional[int] = None):
+        """CTC prefix beam search (`wocr_ctc_beam`): logits [lines, steps, classes] (float32, float16, bfloat16, last
+        dimension contiguous), lens int32 [lines]; `width` (1 to 31) texts kept per step.  The best `paths` texts of each
+        line: tokens int32 [lines, paths, steps] (-1 past the end), lengths int32 and scores float32 (log mass) [lines,
+        paths]; paths is at most width."""
+        if len(logits.shape) != 3 or len(tokens.shape) != 3:
+            raise ValueError("logits [lines, steps, classes] and tokens [lines, paths, steps] expected")
+        n, t, v = logits.shape
+        p = tokens.shape[1]
+        s = _inner(logits, "logits")
+        L.check(L.lib().wocr_ctc_beam(
+            self.h, _ptr(self, logits, "logits"), _code(logits), n, t, v, s[0], s[1],
+            _dense(self, lens, "lens", I32, (n,)) or None, width, blank, p, _dense(self, tokens, "tokens", I32, (n, p, t)),
+            _dense(self, lengths, "lengths", I32, (n, p)), _dense(self, scores, "scores", F32, (n, p)), _stream(stream)))
