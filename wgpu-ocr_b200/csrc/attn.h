@@ -1,6 +1,9 @@
-// Attention, what its kernels share: the score of a query and a key, which keys a query sees, and
-// one query row by a warp straight from the definition.
+// Attention, what its kernels share: the score of a query and a key, which keys a query sees, warp
+// matrix instructions, the join of partial results, and one query row by a warp straight from the
+// definition.
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "elem.h"
 #include "ops.h"
@@ -8,6 +11,8 @@
 namespace wocr {
 namespace k {
 namespace attn {
+
+namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -36,20 +41,27 @@ __device__ __forceinline__ int key_end(const AttnP &p, const Span &s, int i) {
     return p.causal ? min(s.nk, max(s.prefix, s.off + i + 1)) : s.nk;
 }
 
-// The score in units of log 2 from the dot product: cap tanh(scale dot / cap) (or scale dot),
-// less slope |distance|.  tanhf is within 2 ulp; the 32-bit path needs that (a score error is a
-// relative error of the weight).
+// cap tanh(y / cap) in units of log 2.  A score's error is a relative error of its weight: with
+// 32-bit values tanhf (within 2 ulp), with 16-bit values 1 - 2 / (1 + e^2y) from two approximate
+// instructions (within 2^-21).
+template <typename T>
+__device__ __forceinline__ float capped2(float y, float cap) {
+    y /= cap;
+    if (sizeof(T) == 4) return cap * tanhf(y) * kLog2e;
+    return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + ex2(fminf(y * (2.f * kLog2e), 126.f))));
+}
+// A score in units of log 2 from the dot product: cap tanh(scale dot / cap) (or scale dot) less
+// slope |distance|.
+template <typename T>
 __device__ __forceinline__ float score2(const AttnP &p, float dot, float slope, int dist) {
-    float s = dot * p.scale;
-    if (p.cap > 0.f) s = p.cap * tanhf(s / p.cap);
-    s -= slope * fabsf((float)dist);
-    return s * kLog2e;
+    float s = p.cap > 0.f ? capped2<T>(dot * p.scale, p.cap) : dot * (p.scale * kLog2e);
+    return s - slope * kLog2e * fabsf((float)dist);
 }
 
 // Row i of (b, h) by one warp from global memory, two passes over the keys: the maximum and the sum
 // of the weights, then the weighted values.  Keys behind a mask are never read into a sum, so NaN
-// and infinities there stay where they are.  Slow and right for every shape: the other kernels hand
-// it the rows whose sums came out non-finite.
+// and infinities there stay where they are.  Slow and right for every shape: the kernels hand it
+// the rows whose sums came out non-finite.
 template <typename T>
 __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
     const int lane = threadIdx.x & 31;
@@ -69,7 +81,7 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
         const T *kr = kb + (int64_t)j * p.ks[2];
         float dot = 0.f;
         for (int d = 0; d < p.dim; d++) dot = fmaf(to_f(q[d]), to_f(kr[d]), dot);
-        return score2(p, dot, slope, sp.off + i - j);
+        return score2<T>(p, dot, slope, sp.off + i - j);
     };
     float m = -INFINITY, l = 0.f;
     for (int j0 = 0; j0 < end; j0 += 32) {
@@ -107,6 +119,81 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
     for (int x = 0; x < 8; x++)
         if (lane + 32 * x < p.dim) o[lane + 32 * x] = from_f<T>(acc[x] * inv);
 }
+
+// ---- warp matrix instructions (16 x 8 x 16, fp32 accumulators) -----------------------------
+template <typename E>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<E, __half>::value)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+            "%2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+            "%2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"((uint32_t)__cvta_generic_to_shared(p))
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"((uint32_t)__cvta_generic_to_shared(p))
+                 : "memory");
+}
+// two values rounded to E in one word, the first in the low half
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    uint32_t r;
+    if constexpr (std::is_same<E, __half>::value)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+
+// 32-bit values on 16-bit matrix instructions: x = h0 + h1 + h2 with three bf16 parts hold its 24
+// bits exactly, and the six products of order 2^-16 and more leave 2^-23 of |x y| out.
+// Operand element and number of parts of a tensor type:
+template <typename T>
+struct Parts {
+    using E = T;
+    static constexpr int n = 1;
+};
+template <>
+struct Parts<float> {
+    using E = __nv_bfloat16;
+    static constexpr int n = 3;
+};
+// parts[x] of two values, packed
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&parts)[Parts<T>::n]) {
+    using E = typename Parts<T>::E;
+    parts[0] = pack2<E>(x, y);
+    if constexpr (Parts<T>::n == 3) {
+#pragma unroll
+        for (int i = 1; i < 3; i++) {
+            x -= __uint_as_float(parts[i - 1] << 16);
+            y -= __uint_as_float(parts[i - 1] & 0xffff0000u);
+            parts[i] = pack2<E>(x, y);
+        }
+    }
+}
+
+// ---- partial results ------------------------------------------------------------------------
+// Part x of 16 rows: maximum and sum of the weights seen, and the weighted values.
+template <int DP>
+struct PartSums {
+    float o[16][DP];
+    float m[16], l[16];
+};
 
 }  // namespace attn
 }  // namespace k

@@ -1,6 +1,8 @@
 // Softmax attention with capped scores, a bias by distance and causal, prefix and document masks.
 //   o_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(s_ij - max_j s_ij) over the keys that i sees
+// One pass over the keys: the running maximum and sum of a row rescale what it has summed.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn.h"
 
@@ -10,25 +12,439 @@ namespace k {
 namespace {
 using namespace attn;
 
-template <typename T>
-__global__ void __launch_bounds__(128) k_attn_rows(const AttnP p) {
-    const int64_t rows = (int64_t)p.batch * p.heads * p.q_len;
-    for (int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 5); r < rows; r += gridDim.x * 4ll) {
-        const int i = (int)(r % p.q_len);
-        const int h = (int)(r / p.q_len % p.heads);
-        row_by_warp<T>(p, (int)(r / p.q_len / p.heads), h, i);
+// Keys of a tile.  32-bit heads above 128 take half tiles: three parts of queries, keys and values
+// have to fit in shared memory.
+template <typename T, int DP>
+constexpr int tile_keys() { return Parts<T>::n * DP > 384 ? 32 : 64; }
+
+template <typename T, int DP>
+struct TileSmem {
+    static constexpr int P = Parts<T>::n, BK = tile_keys<T, DP>();
+    static constexpr int LD = DP + 8;  // elements per row: eight rows start in eight different 16-byte banks
+    static constexpr bool q_in_regs = P * DP <= 128;
+    static constexpr int q_rows = q_in_regs ? 0 : 64;
+    static constexpr size_t q = (size_t)P * q_rows * LD * 2, kv = (size_t)P * BK * LD * 2;
+    static constexpr size_t tiles = q + 2 * kv, parts = 4 * sizeof(PartSums<DP>);
+    static constexpr size_t bytes = tiles > parts ? tiles : parts;
+};
+
+// `rows` rows of a [.., dim] tensor from row r0 on, split into parts in shared memory; rows from
+// `end` on and dimensions from dim on become zero.
+template <typename T, int DP>
+__device__ __forceinline__ void load_rows(uint16_t *dst, int rows, const T *src, int64_t stride, int r0, int end, int dim, bool vec) {
+    constexpr int P = Parts<T>::n, LD = DP + 8;
+#pragma unroll 2
+    for (int u = threadIdx.x; u < rows * (DP / 8); u += 128) {
+        const int r = u / (DP / 8), d0 = u % (DP / 8) * 8;
+        const bool in = r0 + r < end;
+        const T *s = src + (int64_t)(r0 + r) * stride + d0;
+        T v[8];
+        if (in && vec && d0 + 8 <= dim) {
+#pragma unroll
+            for (int x = 0; x < (int)sizeof(T) / 2; x++) reinterpret_cast<uint4 *>(v)[x] = reinterpret_cast<const uint4 *>(s)[x];
+        } else {
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] = in && d0 + x < dim ? s[x] : from_f<T>(0.f);
+        }
+        if constexpr (P == 1) {
+            *reinterpret_cast<uint4 *>(dst + r * LD + d0) = *reinterpret_cast<const uint4 *>(v);
+        } else {
+            uint32_t w[4][P];
+#pragma unroll
+            for (int x = 0; x < 4; x++) split2<T>(v[2 * x], v[2 * x + 1], w[x]);
+#pragma unroll
+            for (int y = 0; y < P; y++)
+                *reinterpret_cast<uint4 *>(dst + (y * rows + r) * LD + d0) = make_uint4(w[0][y], w[1][y], w[2][y], w[3][y]);
+        }
     }
+}
+
+// The weights' products: part pairs (x, y) with x + y < the number of parts.
+template <typename T, int N>
+__device__ __forceinline__ void mma_parts(float (&c)[4], const uint32_t (&a)[N][4], const uint32_t (&b0)[N], const uint32_t (&b1)[N]) {
+#pragma unroll
+    for (int y = N - 1; y >= 0; y--)  // the small products first
+#pragma unroll
+        for (int x = N - 1 - y; x >= 0; x--) mma16816<typename Parts<T>::E>(c, a[x], b0[y], b1[y]);
+}
+
+// Four warps.  FEW: all have the same 16 rows, which are the queries of all heads that share a key
+// head (row r: head r / q_len, query r % q_len), and each a quarter of a tile's keys; otherwise 64
+// queries of one head, 16 to a warp.  A cluster's blocks share the keys out tile by tile; partial
+// results are joined in shared memory.
+template <typename T, int DP, bool FEW>
+__global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ AttnP p, int vec) {
+    using S = TileSmem<T, DP>;
+    using E = typename Parts<T>::E;
+    constexpr int P = S::P, BK = S::BK, LD = S::LD, KS = DP / 16;
+    constexpr int WK = FEW ? BK / 4 : BK;  // keys of a warp in a tile
+    constexpr int NT = WK / 8;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ float weight[2][64][8];  // joining: a part's share of a row
+    __shared__ uint8_t odd[64];         // rows whose sums are not finite
+    __shared__ int ends[64], seen;
+    uint16_t *sq = (uint16_t *)dyn, *sk = (uint16_t *)(dyn + S::q), *sv = (uint16_t *)(dyn + S::q + S::kv);
+    cg::cluster_group cl = cg::this_cluster();
+    const int cs = cl.num_blocks(), rank = cl.block_rank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int group = p.heads / p.kv_heads;
+    const int hx = FEW ? p.kv_heads : p.heads;
+    const int tile = blockIdx.y;
+    const int b = blockIdx.x / cs / hx, hq = blockIdx.x / cs % hx;
+    const int hk = FEW ? hq : hq / group;
+    const Span sp = span_of(p, b);
+    const int nrows = FEW ? group * p.q_len : 64;
+    // head and query of a row of the block; -1 for rows past the last
+    auto row_head = [&](int r) { return FEW ? hk * group + r / p.q_len : hq; };
+    auto row_query = [&](int r) {
+        const int i = FEW ? r % p.q_len : tile * 64 + r;
+        return (FEW ? r < nrows : true) && i < sp.nq ? i : -1;
+    };
+    if (threadIdx.x == 0) seen = 0;
+    if (threadIdx.x < 64) odd[threadIdx.x] = 0;
+    __syncthreads();
+    if (threadIdx.x < (FEW ? 16 : 64)) {
+        const int i = row_query(threadIdx.x);
+        const int e = i >= 0 ? key_end(p, sp, i) : 0;
+        ends[threadIdx.x] = e;
+        atomicMax(&seen, e);
+    }
+    const T *kb = (const T *)p.k + b * p.ks[0] + hk * p.ks[1];
+    const T *vb = (const T *)p.v + b * p.vs[0] + hk * p.vs[1];
+    const int wr = FEW ? 0 : warp * 16;  // the warp's first row
+    // this thread's two rows
+    const int r0 = wr + (lane >> 2), r1 = r0 + 8;
+    const int i0 = row_query(r0), i1 = row_query(r1);
+    uint32_t qf[S::q_in_regs ? KS : 1][P][4];
+    const T *q0 = (const T *)p.q + b * p.qs[0] + row_head(r0) * p.qs[1] + (int64_t)i0 * p.qs[2];
+    const T *q1 = (const T *)p.q + b * p.qs[0] + row_head(r1) * p.qs[1] + (int64_t)i1 * p.qs[2];
+    if constexpr (S::q_in_regs) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int d = ks * 16 + (x >> 1) * 8 + (lane & 3) * 2;
+                const T *q = x & 1 ? q1 : q0;
+                const bool in = (x & 1 ? i1 : i0) >= 0;
+                uint32_t w[P];
+                split2<T>(in && d < p.dim ? to_f(q[d]) : 0.f, in && d + 1 < p.dim ? to_f(q[d + 1]) : 0.f, w);
+#pragma unroll
+                for (int y = 0; y < P; y++) qf[ks][y][x] = w[y];
+            }
+    } else if constexpr (FEW) {
+        for (int u = threadIdx.x; u < 16 * DP / 2; u += 128) {
+            const int r = u / (DP / 2), d = u % (DP / 2) * 2, i = row_query(r);
+            const T *q = (const T *)p.q + b * p.qs[0] + row_head(r) * p.qs[1] + (int64_t)i * p.qs[2];
+            uint32_t w[P];
+            split2<T>(i >= 0 && d < p.dim ? to_f(q[d]) : 0.f, i >= 0 && d + 1 < p.dim ? to_f(q[d + 1]) : 0.f, w);
+#pragma unroll
+            for (int y = 0; y < P; y++) *reinterpret_cast<uint32_t *>(sq + (y * 64 + r) * LD + d) = w[y];
+        }
+    } else {
+        load_rows<T, DP>(sq, 64, (const T *)p.q + b * p.qs[0] + hq * p.qs[1], p.qs[2], tile * 64, sp.nq, p.dim, vec);
+    }
+    __syncthreads();
+    const int last = seen;  // keys that any row sees
+    const int e0 = ends[r0], e1 = ends[r1];
+    int all;                // keys below it are seen by both rows of every thread of the warp
+    {
+        int e = min(i0 >= 0 ? e0 : 0x7fffffff, i1 >= 0 ? e1 : 0x7fffffff);
+        all = __reduce_min_sync(0xffffffffu, e);
+    }
+    const float sl0 = p.slopes ? p.slopes[row_head(min(r0, nrows - 1))] * kLog2e : 0.f;
+    const float sl1 = p.slopes ? p.slopes[row_head(min(r1, nrows - 1))] * kLog2e : 0.f;
+    const int d0 = p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
+    const int *kd = p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
+    const int pos0 = sp.off + i0, pos1 = sp.off + i1;
+    const float scale2 = p.scale * kLog2e;
+    float acc[DP / 8][4];
+#pragma unroll
+    for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) acc[n][x] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    for (int j0 = rank * BK; j0 < last; j0 += cs * BK) {
+        __syncthreads();  // the tile before has been read
+        load_rows<T, DP>(sk, BK, kb, p.ks[2], j0, sp.nk, p.dim, vec);
+        load_rows<T, DP>(sv, BK, vb, p.vs[2], j0, sp.nk, p.dim, vec);
+        __syncthreads();
+        const int jw = j0 + (FEW ? warp * WK : 0), kw = FEW ? warp * WK : 0;
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) s[n][x] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            uint32_t a[P][4];
+#pragma unroll
+            for (int y = 0; y < P; y++) {
+                if constexpr (S::q_in_regs) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++) a[y][x] = qf[ks][y][x];
+                } else {
+                    ldsm4(a[y], sq + (y * 64 + wr + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8);
+                }
+            }
+            // two n-tiles of 8 keys per load: keys (lane & 7) + 8 (lane >> 4), dims 8 ((lane >> 3) & 1)
+            if constexpr (NT >= 2) {
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t bb[P][4], b0[P], b1[P];
+#pragma unroll
+                    for (int y = 0; y < P; y++)
+                        ldsm4(bb[y], sk + (y * BK + kw + n * 8 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8);
+#pragma unroll
+                    for (int y = 0; y < P; y++) b0[y] = bb[y][0], b1[y] = bb[y][1];
+                    mma_parts<T, P>(s[n], a, b0, b1);
+#pragma unroll
+                    for (int y = 0; y < P; y++) b0[y] = bb[y][2], b1[y] = bb[y][3];
+                    mma_parts<T, P>(s[n + 1], a, b0, b1);
+                }
+            } else {
+                uint32_t b0[P], b1[P];
+#pragma unroll
+                for (int y = 0; y < P; y++) {
+                    const uint16_t *at = sk + (y * BK + kw + (lane >> 2)) * LD + ks * 16 + (lane & 3) * 2;
+                    b0[y] = *reinterpret_cast<const uint32_t *>(at);
+                    b1[y] = *reinterpret_cast<const uint32_t *>(at + 8);
+                }
+                mma_parts<T, P>(s[0], a, b0, b1);
+            }
+        }
+        // scores in units of log 2, masked
+        const bool whole = jw + WK <= all && !kd;
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int j = jw + n * 8 + (lane & 3) * 2 + x;
+                float u = s[n][x], w = s[n][2 + x];
+                if (p.cap > 0.f) {
+                    u = capped2<T>(u * p.scale, p.cap);
+                    w = capped2<T>(w * p.scale, p.cap);
+                } else {
+                    u *= scale2;
+                    w *= scale2;
+                }
+                if (p.slopes) {
+                    u -= sl0 * fabsf((float)(pos0 - j));
+                    w -= sl1 * fabsf((float)(pos1 - j));
+                }
+                if (!whole) {
+                    bool in0 = j < e0, in1 = j < e1;
+                    if (kd) {
+                        const int doc = j < sp.nk ? kd[j] : -1;
+                        in0 = in0 && doc == d0 && doc >= 0;
+                        in1 = in1 && doc == d1 && doc >= 0;
+                    }
+                    if (!in0) u = -INFINITY;
+                    if (!in1) w = -INFINITY;
+                }
+                s[n][x] = u;
+                s[n][2 + x] = w;
+                t0 = fmaxf(t0, u);
+                t1 = fmaxf(t1, w);
+            }
+#pragma unroll
+        for (int d = 1; d < 4; d *= 2) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+        }
+        const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+        const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+        const float c0 = ex2(m0 - z0), c1 = ex2(m1 - z1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= c0;
+        l1 *= c1;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                s[n][x] = ex2(s[n][x] - z0);
+                s[n][2 + x] = ex2(s[n][2 + x] - z1);
+                l0 += s[n][x];
+                l1 += s[n][2 + x];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++) {
+            acc[n][0] *= c0;
+            acc[n][1] *= c0;
+            acc[n][2] *= c1;
+            acc[n][3] *= c1;
+        }
+        // the weights as the left operand, 16 keys at a time, rounded to the parts (16-bit types:
+        // once, to the values' type, as the matrix instruction asks)
+#pragma unroll
+        for (int n = 0; n < (NT + 1) / 2; n++) {
+            uint32_t a[P][4], w[P];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int nt = 2 * n + (x >> 1);
+                if (nt < NT) split2<T>(s[nt < NT ? nt : 0][(x & 1) * 2], s[nt < NT ? nt : 0][(x & 1) * 2 + 1], w);
+#pragma unroll
+                for (int y = 0; y < P; y++) a[y][x] = nt < NT ? w[y] : 0u;
+            }
+#pragma unroll
+            for (int dn = 0; dn < DP / 16; dn++) {
+                uint32_t bb[P][4], b0[P], b1[P];
+                // keys (lane & 15), dims 8 (lane >> 4); with 8 keys only, the upper half repeats the lower
+                const int key = kw + n * 16 + (NT == 1 ? lane & 7 : lane & 15);
+#pragma unroll
+                for (int y = 0; y < P; y++) ldsm4t(bb[y], sv + (y * BK + key) * LD + dn * 16 + (lane >> 4) * 8);
+#pragma unroll
+                for (int y = 0; y < P; y++) b0[y] = bb[y][0], b1[y] = bb[y][1];
+                mma_parts<T, P>(acc[2 * dn], a, b0, b1);
+#pragma unroll
+                for (int y = 0; y < P; y++) b0[y] = bb[y][2], b1[y] = bb[y][3];
+                mma_parts<T, P>(acc[2 * dn + 1], a, b0, b1);
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    T *ob = (T *)p.o + b * p.os[0];
+    if (!FEW && cs == 1) {
+        const float v0 = l0 == 0.f ? 0.f : 1.f / l0, v1 = l1 == 0.f ? 0.f : 1.f / l1;
+        bool bad0 = false, bad1 = false;
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int d = n * 8 + (lane & 3) * 2 + x;
+                const float u = acc[n][x] * v0, w = acc[n][2 + x] * v1;
+                bad0 |= !(fabsf(u) <= 3.4028234e38f);
+                bad1 |= !(fabsf(w) <= 3.4028234e38f);
+                if (d < p.dim) {
+                    if (i0 >= 0) ob[hq * p.os[1] + (int64_t)i0 * p.os[2] + d] = from_f<T>(u);
+                    if (i1 >= 0) ob[hq * p.os[1] + (int64_t)i1 * p.os[2] + d] = from_f<T>(w);
+                }
+            }
+        if (bad0) odd[r0] = 1;
+        if (bad1) odd[r1] = 1;
+        __syncwarp();
+        for (int r = wr; r < wr + 16; r++)
+            if (odd[r] && row_query(r) >= 0) row_by_warp<T>(p, b, hq, row_query(r));
+        return;
+    }
+    __syncthreads();  // the tiles have been read: their place holds the parts now
+    PartSums<DP> *parts = (PartSums<DP> *)dyn;
+    {
+        PartSums<DP> &pt = parts[warp];
+        const int a = lane >> 2;
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++) {
+            const int d = n * 8 + (lane & 3) * 2;
+            *reinterpret_cast<float2 *>(&pt.o[a][d]) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2 *>(&pt.o[a + 8][d]) = make_float2(acc[n][2], acc[n][3]);
+        }
+        if ((lane & 3) == 0) {
+            pt.m[a] = m0;
+            pt.m[a + 8] = m1;
+            pt.l[a] = l0;
+            pt.l[a + 8] = l1;
+        }
+    }
+    cl.sync();
+    // rows of the block (16 or 64) x parts: cs blocks, and with FEW four warps each (two per slot)
+    const int rows = FEW ? 16 : 64;
+    const int per = FEW ? 4 : 1;
+    if (threadIdx.x < rows) {
+        const int r = threadIdx.x;
+        float m = -INFINITY;
+        for (int c = 0; c < cs; c++)
+            for (int w = 0; w < per; w++)
+                m = fmaxf(m, cl.map_shared_rank(parts, c)[FEW ? w : r / 16].m[r % 16]);
+        const float z = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        for (int c = 0; c < cs; c++)
+            for (int w = 0; w < per; w++) {
+                const PartSums<DP> &pt = cl.map_shared_rank(parts, c)[FEW ? w : r / 16];
+                const float f = ex2(pt.m[r % 16] - z);
+                l += f * pt.l[r % 16];
+                if (FEW) weight[w >> 1][r + 16 * (w & 1)][c] = f;
+                else weight[0][r][c] = f;
+            }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        for (int c = 0; c < cs; c++)
+            for (int w = 0; w < per; w++) {
+                if (FEW) weight[w >> 1][r + 16 * (w & 1)][c] *= inv;
+                else weight[0][r][c] *= inv;
+            }
+    }
+    __syncthreads();
+    // the cluster's blocks share the values out
+    for (int u = rank * 128 + threadIdx.x; u < rows * DP; u += cs * 128) {
+        const int r = u / DP, d = u % DP, i = row_query(r);
+        if (i < 0 || d >= p.dim) continue;
+        float v = 0.f;
+        for (int c = 0; c < cs; c++)
+            for (int w = 0; w < per; w++)
+                v += (FEW ? weight[w >> 1][r + 16 * (w & 1)][c] : weight[0][r][c]) *
+                     cl.map_shared_rank(parts, c)[FEW ? w : r / 16].o[r % 16][d];
+        if (!(fabsf(v) <= 3.4028234e38f)) odd[r] = 1;
+        ob[row_head(r) * p.os[1] + (int64_t)i * p.os[2] + d] = from_f<T>(v);
+    }
+    cl.sync();  // the parts are read until here; non-finite rows are written after the others
+    for (int r = warp; r < rows; r += 4)
+        if (odd[r] && row_query(r) >= 0) row_by_warp<T>(p, b, row_head(r), row_query(r));
+}
+
+template <typename T, int DP, bool FEW>
+void launch_tiles(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
+    using S = TileSmem<T, DP>;
+    const int64_t units = (int64_t)p.batch * (FEW ? p.kv_heads : p.heads);
+    const int tiles = FEW ? 1 : (p.q_len + 63) / 64;
+    // blocks that share a row's keys: while the GPU has room and each keeps two tiles or more
+    int cs = 1;
+    while (cs < 8 && units * tiles * cs < 2 * c->sm_count && p.kv_len > 2 * cs * S::BK) cs *= 2;
+    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tiles<T, DP, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::bytes));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = S::bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (units * cs > 0x7fffffff || tiles > 65535) fail(WOCR_ERR_UNSUPPORTED, "attention: too many heads or queries");
+    cfg.gridDim = dim3((unsigned)(units * cs), tiles);
+    WOCR_CUDA(cudaLaunchKernelEx(&cfg, k_attn_tiles<T, DP, FEW>, p, vec));
+    WOCR_LAUNCHED(c);
+}
+
+template <typename T, int DP>
+void launch_dim(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
+    if ((int64_t)p.heads / p.kv_heads * p.q_len <= 16) launch_tiles<T, DP, true>(c, p, vec, s);
+    else launch_tiles<T, DP, false>(c, p, vec, s);
+}
+
+template <typename T>
+void launch_type(Ctx *c, const AttnP &p, cudaStream_t s) {
+    // 16-byte loads where every row of queries, keys and values allows them
+    const int n = 16 / sizeof(T);
+    bool vec = ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0;
+    for (int i = 0; i < 3; i++) vec = vec && p.qs[i] % n == 0 && p.ks[i] % n == 0 && p.vs[i] % n == 0;
+    if (p.dim <= 16) launch_dim<T, 16>(c, p, vec, s);
+    else if (p.dim <= 32) launch_dim<T, 32>(c, p, vec, s);
+    else if (p.dim <= 64) launch_dim<T, 64>(c, p, vec, s);
+    else if (p.dim <= 128) launch_dim<T, 128>(c, p, vec, s);
+    else launch_dim<T, 256>(c, p, vec, s);
 }
 }  // namespace
 
 void attention(Ctx *c, const AttnP &p, cudaStream_t s) {
-    if (p.batch == 0 || p.q_len == 0) return;
-    const int64_t rows = (int64_t)p.batch * p.heads * p.q_len;
-    const int grid = (int)std::min<int64_t>((rows + 3) / 4, c->sm_count * 64);
-    if (p.type == WOCR_F32) k_attn_rows<float><<<grid, 128, 0, s>>>(p);
-    else if (p.type == WOCR_F16) k_attn_rows<__half><<<grid, 128, 0, s>>>(p);
-    else k_attn_rows<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-    WOCR_LAUNCHED(c);
+    if (p.type == WOCR_F32) launch_type<float>(c, p, s);
+    else if (p.type == WOCR_F16) launch_type<__half>(c, p, s);
+    else launch_type<__nv_bfloat16>(c, p, s);
 }
 
 }  // namespace k
