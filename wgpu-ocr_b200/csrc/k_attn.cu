@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "attn.h"
+#include "attn_tc.h"
 
 namespace wocr {
 namespace k {
@@ -442,6 +443,7 @@ void launch_type(Ctx *c, const AttnP &p, cudaStream_t s) {
 }  // namespace
 
 void attention(Ctx *c, const AttnP &p, cudaStream_t s) {
+    if (p.q_len >= 128 && attention_tc_ok(p)) return attention_tc(c, p, s);
     if (p.type == WOCR_F32) launch_type<float>(c, p, s);
     else if (p.type == WOCR_F16) launch_type<__half>(c, p, s);
     else launch_type<__nv_bfloat16>(c, p, s);

@@ -1,0 +1,545 @@
+// Attention of many queries over 16-bit keys and values on the tensor cores: tcgen05 with scores,
+// weights and sums in tensor memory, tiles fed by TMA.
+//
+// A block takes 256 queries of one head as two tiles of 128 (one tensor-memory lane each) and walks
+// the keys in tiles of 128.  Roles:
+//   warps 0-3, 4-7  softmax of query tile 0 and 1, a thread per row: scores from tensor memory, mask,
+//                   running maximum and sum, weights back into tensor memory as the left operand of
+//                   the second product, in the columns of the scores they came from
+//   warp 8          (one thread) issues S = Q K^T and O += P V.  While one tile's softmax runs, the
+//                   other tile's products do, so the matrix pipe and the exponentials overlap
+//   warp 9          (one thread) TMA loads of queries, keys and values, two stages each
+// A row's sums are rescaled only when its maximum has grown by more than 2^8 since it was last used
+// (the weights stay below 2^8, the quotient is the same), so the accumulator is seldom touched
+// between products.
+// Bound: 4 D flops and one exponential a pair.  An SM's matrix pipe takes 128 x 128 x 128 in 512
+// cycles and its 16 exponentials a cycle take as long for two such products (D = 128).
+#include <algorithm>
+#include <type_traits>
+
+#include "attn.h"
+#include "attn_tc.h"
+#include "tc.h"
+
+namespace wocr {
+namespace k {
+
+namespace {
+using namespace attn;
+using namespace tc;
+
+constexpr int kThreads = 320, kMmaWarp = 8, kTmaWarp = 9;
+constexpr int kMaxTiles = 8192;              // key tiles of a call (2^20 keys): their bits fit in shared memory
+constexpr int kWords = kMaxTiles / 32;
+constexpr float kSlack = 8.f;                // growth of a maximum (log 2) that leaves the sums alone
+constexpr uint32_t kColS = 0, kColO = 256;   // tensor-memory columns: two score tiles, two sums of 128
+
+template <int DP>
+struct Smem {
+    static constexpr int tile = 128 * DP * 2;
+    // values first: a stage ends inside the block's shared memory whatever follows it
+    static constexpr int v = 0, k = v + 2 * tile, q = k + 2 * tile, bits = q + 2 * tile, docs = bits + 4 * kWords * 4,
+                         bars = docs + 8 * 128 * 4, bytes = bars + 256 + 1024;  // 1,024: alignment of the start
+};
+
+struct TcArgs {
+    AttnP a;
+    int *status;
+    long long budget;
+    int tiles, vec_out;  // query tile pairs of a head; rows of out take 16-byte stores
+};
+
+// kind::f16, D fp32, M = 128; B is K-major (scores) or N-major (values: dimensions contiguous)
+__host__ __device__ constexpr uint32_t idesc(bool bf16, int n, bool b_n_major) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_n_major ? 1u : 0u) << 16) |
+           ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+// N-major operand in the 128-byte swizzle: rows (keys) of 64 dimensions, eight rows an atom of
+// 1,024 bytes (the stride between groups of eight keys); the next 64 dimensions a panel further.
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t addr, uint32_t panel) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float *f) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+#pragma unroll
+    for (int i = 0; i < 32; i++) f[i] = __uint_as_float(r[i]);
+}
+// waits for the thread's tensor-memory loads; the values pass through, so that no use moves ahead
+__device__ __forceinline__ void tmem_wait32(float *f) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]),
+                   "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]), "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15]),
+                   "+f"(f[16]), "+f"(f[17]), "+f"(f[18]), "+f"(f[19]), "+f"(f[20]), "+f"(f[21]), "+f"(f[22]), "+f"(f[23]),
+                   "+f"(f[24]), "+f"(f[25]), "+f"(f[26]), "+f"(f[27]), "+f"(f[28]), "+f"(f[29]), "+f"(f[30]), "+f"(f[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attn_tc(const __grid_constant__ TcArgs ta, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+              const __grid_constant__ CUtensorMap mv) {
+    using L = Smem<DP>;
+    constexpr int kPanels = DP / 64, kPanel = 128 * 128;  // 64 dimensions of 128 rows
+    extern __shared__ uint8_t raw[];
+    uint8_t *sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const AttnP &p = ta.a;
+    uint32_t *act = (uint32_t *)(sm + L::bits), *full = act + 2 * kWords;  // per query tile: key tiles to visit, without masks
+    int *docs = (int *)(sm + L::docs);
+    uint64_t *bars = (uint64_t *)(sm + L::bars);
+    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
+             *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13, *tail = bars + 15;
+    uint32_t *slot = (uint32_t *)(bars + 16);
+    volatile int *stop = (volatile int *)(slot + 1);
+    int *lim = (int *)(slot + 2);  // [4] least and greatest document of the two query tiles
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // long rows first: with a causal mask the last queries see the most keys
+    const int heads = p.heads * p.batch;
+    const int tile = ta.tiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
+    const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kv_heads);
+    const Span sp = span_of(p, b);
+    const int i_first = tile * 256;
+    if (i_first >= sp.nq) return;
+    // keys that the first and the last row of each query tile may see
+    int emin[2], emax[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int a = i_first + t * 128, z = min(a + 127, sp.nq - 1);
+        emin[t] = a < sp.nq ? max(key_end(p, sp, a), 0) : 0;
+        emax[t] = a < sp.nq ? max(key_end(p, sp, z), 0) : 0;
+    }
+    const int ntiles = (max(emax[0], emax[1]) + 127) / 128;
+    if (tid == 0) {
+        for (int i = 0; i < 16; i++) mbar_init(bars + i, i == 11 || i == 12 ? 4 : 1);  // p_full: a warp each
+        *stop = 0;
+        for (int i = 0; i < 4; i++) lim[i] = i & 1 ? -1 : 0x7fffffff;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    const int my = warp >> 2;  // softmax: the thread's query tile and row
+    const int i = i_first + my * 128 + (tid & 127);
+    const bool row = warp < 8 && i < sp.nq;
+    int doc = -1;
+    if (p.q_docs) {
+        for (int w = tid; w < 4 * kWords; w += kThreads) act[w] = 0;
+        __syncthreads();
+        if (row) doc = p.q_docs[b * p.qds + i];
+        if (doc >= 0) {
+            atomicMin(&lim[2 * my], doc);
+            atomicMax(&lim[2 * my + 1], doc);
+        }
+        bool neg = row && doc < 0;
+        if (neg) atomicMin(&lim[2 * my], -1);  // a row that sees nothing: no tile goes without its mask
+        __syncthreads();
+        // a key tile's documents against the query tiles': none shared, all the same, or some
+        for (int j = warp; j < ntiles; j += kThreads / 32) {
+            int lo = 0x7fffffff, hi = -1;
+            bool odd = false;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int key = j * 128 + x * 32 + lane;
+                const int d = key < sp.nk ? p.kv_docs[b * p.kds + key] : -1;
+                if (d >= 0) lo = min(lo, d), hi = max(hi, d);
+                else odd = true;
+            }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+            odd = __any_sync(0xffffffffu, odd);
+            if (lane == 0)
+                for (int t = 0; t < 2; t++) {
+                    const int ql = max(lim[2 * t], 0), qh = lim[2 * t + 1];
+                    if (j * 128 < emax[t] && lo <= qh && hi >= ql) atomicOr(&act[t * kWords + j / 32], 1u << (j & 31));
+                    if (!odd && lo == hi && lim[2 * t] == lo && qh == lo && (j + 1) * 128 <= emin[t])
+                        atomicOr(&full[t * kWords + j / 32], 1u << (j & 31));
+                }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    auto visits = [&](int t, int j) -> bool {
+        return p.q_docs ? (act[t * kWords + j / 32] >> (j & 31)) & 1 : j * 128 < emax[t];
+    };
+    auto unmasked = [&](int t, int j) -> bool {
+        return p.q_docs ? (full[t * kWords + j / 32] >> (j & 31)) & 1 : (j + 1) * 128 <= emin[t];
+    };
+
+    if (warp == kTmaWarp) {
+        const uint32_t qbytes = 128 * DP * 2;
+        bool any = false;
+        int it = 0;
+        bool ok = true;
+        for (int j = 0; j < ntiles && ok; j++) {
+            if (!visits(0, j) && !visits(1, j)) continue;
+            const int s = it & 1;
+            const uint32_t par = (it >> 1) & 1;
+            uint8_t *sk = sm + L::k + s * L::tile, *sv = sm + L::v + s * L::tile;
+            // values behind the last key must be finite: they are multiplied by weights of zero
+            const bool edge = sp.nk < (j + 1) * 128 && sp.nk < p.kv_len;
+            if (lane == 0) {
+                if (!any) {
+                    mbar_expect_tx(q_full, 2 * qbytes);
+                    for (int t = 0; t < 2; t++)
+                        for (int x = 0; x < kPanels; x++)
+                            tma_load_4d(sm + L::q + t * L::tile + x * kPanel, &mq, q_full, x * 64, i_first + t * 128, h, b);
+                    any = true;
+                }
+                ok = mbar_wait_spin(&k_empty[s], par ^ 1, ta.status, stop, 41, ta.budget);
+                if (ok) {
+                    mbar_expect_tx(&k_full[s], qbytes);
+                    for (int x = 0; x < kPanels; x++) tma_load_4d(sk + x * kPanel, &mk, &k_full[s], x * 64, j * 128, hk, b);
+                    ok = mbar_wait_spin(&v_empty[s], par ^ 1, ta.status, stop, 42, ta.budget);
+                }
+                if (ok) {
+                    uint64_t *bar = edge ? tail : &v_full[s];
+                    mbar_expect_tx(bar, qbytes);
+                    for (int x = 0; x < kPanels; x++) tma_load_4d(sv + x * kPanel, &mv, bar, x * 64, j * 128, hk, b);
+                    if (edge) ok = mbar_wait_spin(tail, 0, ta.status, stop, 43, ta.budget);  // the last tile: once
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            __syncwarp();
+            if (edge && ok) {
+                const int from = sp.nk - j * 128;  // a row is 128 bytes of each panel, wherever the swizzle puts its pieces
+                for (int u = lane; u < (128 - from) * 8 * kPanels; u += 32) {
+                    const int x = u / ((128 - from) * 8), v = u % ((128 - from) * 8);
+                    *(uint4 *)(sv + x * kPanel + (from + v / 8) * 128 + (v % 8) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[s]);
+            }
+            it++;
+        }
+        if (lane == 0) {
+            // copies land before the block may exit, however it ends (bounded)
+            const long long t0 = clock64();
+            if (it > 0)
+                while (!mbar_try(q_full, 0) && clock64() - t0 < ta.budget) {
+                }
+            for (int j = it > 2 ? it - 2 : 0; j < it; j++)
+                for (uint64_t *bar : {&k_full[j & 1], &v_full[j & 1]})
+                    while (!mbar_try(bar, (j >> 1) & 1) && clock64() - t0 < ta.budget && !*stop) {
+                    }
+            if (*stop) {  // given up: some loads may never have been asked for, others are on their way
+                const long long t1 = clock64();
+                while (clock64() - t1 < 2000000) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        if (lane == 0) {
+            constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+            const int ksteps = (p.dim + 15) / 16;
+            const uint32_t id_s = idesc(bf, 128, false), id_o = idesc(bf, ksteps * 16, true);
+            bool ok = true, first = true;
+            bool begun[2] = {false, false};
+            int pend[2] = {-1, -1};      // stage (and phase) of the values that a tile's weights wait for
+            int np[2] = {0, 0};          // weights consumed
+            int it = 0, prev = -1;
+            auto product = [&](int t) {  // O_t += P_t V
+                if (pend[t] < 0) return;
+                const int s = pend[t] & 1;
+                ok = ok && mbar_wait_spin(&p_full[t], np[t] & 1, ta.status, stop, 44, ta.budget) &&
+                     mbar_wait_spin(&v_full[s], (pend[t] >> 1) & 1, ta.status, stop, 45, ta.budget);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t v = smem_u32(sm + L::v + s * L::tile);
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    umma_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + x * 8, desc_n_major(v + x * 2048, kPanel), id_o,
+                            begun[t] || x > 0);
+                begun[t] = true;
+                pend[t] = -1;
+                np[t]++;
+            };
+            for (int j = 0; j < ntiles && ok; j++) {
+                const bool v0 = visits(0, j), v1 = visits(1, j);
+                if (!v0 && !v1) continue;
+                const int s = it & 1;
+                if (first) ok = mbar_wait_spin(q_full, 0, ta.status, stop, 46, ta.budget);
+                first = false;
+                ok = ok && mbar_wait_spin(&k_full[s], (it >> 1) & 1, ta.status, stop, 47, ta.budget);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    product(t);
+                    if (!ok) break;
+                    if (!(t ? v1 : v0)) continue;
+                    const uint32_t q = smem_u32(sm + L::q + t * L::tile), k = smem_u32(sm + L::k + s * L::tile);
+                    for (int x = 0; x < ksteps; x++) {
+                        const uint32_t off = (x >> 2) * kPanel + (x & 3) * 32;
+                        umma(tmem + kColS + t * 128, smem_desc(q + off), smem_desc(k + off), id_s, x > 0);
+                    }
+                    umma_commit(&s_full[t]);
+                    pend[t] = it & 3;
+                }
+                if (!ok) break;
+                umma_commit(&k_empty[s]);
+                if (prev >= 0) umma_commit(&v_empty[prev]);
+                prev = s;
+                it++;
+            }
+            for (int t = 0; t < 2; t++) {
+                product(t);
+                umma_commit(&o_full[t]);
+            }
+            const long long t0 = clock64();
+            for (int t = 0; t < 2; t++)
+                while (!mbar_try(&o_full[t], 0) && clock64() - t0 < ta.budget) {
+                }
+        }
+        __syncwarp();
+    } else {
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 tensor-memory lanes
+        const uint32_t ts = tmem + lanes + kColS + my * 128, to = tmem + lanes + kColO + my * 128;
+        const bool live = row && (!p.q_docs || doc >= 0);
+        const int end = live ? key_end(p, sp, i) : 0, pos = sp.off + i;
+        const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.f, scale2 = p.scale * kLog2e;
+        int *dk = docs + warp * 128;
+        float m = -INFINITY, l = 0.f;
+        int n = 0;
+        bool ok = true;
+        for (int j = 0; j < ntiles && ok; j++) {
+            if (!visits(my, j)) continue;
+            const int j0 = j * 128;
+            const bool plain = unmasked(my, j);
+            if (p.q_docs && !plain) {
+                __syncwarp();  // the ids of the tile before have been read
+#pragma unroll
+                for (int x = lane; x < 128; x += 32) dk[x] = j0 + x < sp.nk ? p.kv_docs[b * p.kds + j0 + x] : -1;
+                __syncwarp();
+            }
+            ok = warp_wait(&s_full[my], n & 1, ta.status, stop, 48, ta.budget);
+            if (!ok) break;
+            tc_fence_after();
+            float f[128];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(ts + c * 32, f + c * 32);
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_wait32(f + c * 32);
+            float mul = scale2;
+            if (p.cap > 0.f) {
+                mul = 1.f;
+#pragma unroll
+                for (int x = 0; x < 128; x++) f[x] = capped2<T>(f[x] * p.scale, p.cap);
+            } else if (p.slopes || !(scale2 > 0.f)) {
+                mul = 1.f;
+#pragma unroll
+                for (int x = 0; x < 128; x++) f[x] *= scale2;
+            }
+            if (p.slopes) {
+                const float far = (float)(pos - j0);
+#pragma unroll
+                for (int x = 0; x < 128; x++) f[x] = fmaf(-slope, fabsf(far - (float)x), f[x]);
+            }
+            if (!plain) {
+#pragma unroll
+                for (int x = 0; x < 128; x++)
+                    if (j0 + x >= end) f[x] = -INFINITY;
+                if (p.q_docs)
+#pragma unroll
+                    for (int x = 0; x < 128; x += 4) {
+                        const int4 d = *(const int4 *)(dk + x);
+                        if (d.x != doc) f[x] = -INFINITY;
+                        if (d.y != doc) f[x + 1] = -INFINITY;
+                        if (d.z != doc) f[x + 2] = -INFINITY;
+                        if (d.w != doc) f[x + 3] = -INFINITY;
+                    }
+            }
+            float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int x = 0; x < 128; x++) a[x & 3] = fmaxf(a[x & 3], f[x]);
+            const float top = fmaxf(m, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * mul);
+            if (m == -INFINITY) m = top;  // nothing seen so far: nothing to rescale
+            const bool grown = m > -INFINITY && top - m > kSlack;
+            if (__any_sync(0xffffffffu, grown) && n > 0) {
+                // the second product of the tile before is complete: s_full follows it
+                const float c = grown ? ex2(m - top) : 1.f;
+                if (grown) m = top;
+                l *= c;
+#pragma unroll
+                for (int c0 = 0; c0 < DP; c0 += 32) {
+                    if (c0 >= p.dim) break;
+                    float o[32];
+                    uint32_t w[16];
+                    tmem_ld32(to + c0, o);
+                    tmem_wait32(o);
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+#pragma unroll
+                        for (int x = 0; x < 16; x++) w[x] = __float_as_uint(o[y * 16 + x] * c);
+                        tmem_st16(to + c0 + y * 16, w);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const float u = ex2(fmaf(f[c * 32 + 2 * x], mul, -base)), v = ex2(fmaf(f[c * 32 + 2 * x + 1], mul, -base));
+                    sum[(2 * x) & 3] += u;
+                    sum[(2 * x + 1) & 3] += v;
+                    w[x] = pack2<T>(u, v);  // the one rounding of a weight: the matrix instruction takes 16 bits
+                }
+                tmem_st16(ts + c * 16, w);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[my]);
+            n++;
+        }
+        if (ok) ok = warp_wait(&o_full[my], 0, ta.status, stop, 49, ta.budget);
+        if (ok) {
+            tc_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            bool bad = !(fabsf(l) <= 3.4028234e38f);
+            T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
+#pragma unroll
+            for (int c0 = 0; c0 < DP; c0 += 32) {
+                if (c0 >= p.dim) break;
+                float f[32];
+                if (n > 0) {
+                    tmem_ld32(to + c0, f);
+                    tmem_wait32(f);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) f[x] = 0.f;
+                }
+#pragma unroll
+                for (int x = 0; x < 32; x++) {
+                    bad |= c0 + x < p.dim && !(fabsf(f[x]) <= 3.4028234e38f);
+                    f[x] *= inv;
+                }
+                if (row) {
+                    if (ta.vec_out) {
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8)
+                            if (c0 + x < p.dim)
+                                *(uint4 *)(o + c0 + x) = make_uint4(pack2<T>(f[x], f[x + 1]), pack2<T>(f[x + 2], f[x + 3]),
+                                                                    pack2<T>(f[x + 4], f[x + 5]), pack2<T>(f[x + 6], f[x + 7]));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            if (c0 + x < p.dim) o[c0 + x] = from_f<T>(f[x]);
+                    }
+                }
+            }
+            uint32_t rows = __ballot_sync(0xffffffffu, bad && row);
+            while (rows) {
+                const int r = __ffs(rows) - 1;
+                rows &= rows - 1;
+                __syncwarp();
+                row_by_warp<T>(p, b, h, i - lane + r);
+            }
+        }
+        tc_fence_before();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// [batch][heads][tokens][dim] with element strides, boxes of 128 tokens x 64 dimensions; what lies
+// outside reads as zero
+void make_map(CUtensorMap &m, bool bf16, const void *p, const int64_t *st, int batch, int heads, int tokens, int dim) {
+    auto fn = encode_fn();
+    if (!fn) fail(WOCR_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
+    // the stride of a dimension of one is not used, but has to be valid
+    auto stride = [&](int64_t s, int n) { return (cuuint64_t)((n > 1 ? s : dim) * 2); };
+    const cuuint64_t strides[3] = {stride(st[2], tokens), stride(st[1], heads), stride(st[0], batch)};
+    const cuuint32_t box[4] = {64, 128, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = fn(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p),
+                          dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) fail(WOCR_ERR_CUDA, "cuTensorMapEncodeTiled (attention) failed: " + std::to_string((int)r));
+}
+
+template <typename T, int DP>
+void launch(Ctx *c, const TcArgs &ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
+    const int bytes = Smem<DP>::bytes;
+    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tc<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    k_attn_tc<T, DP><<<(unsigned)(ta.tiles * ta.a.batch * ta.a.heads), kThreads, bytes, s>>>(ta, mq, mk, mv);
+    WOCR_LAUNCHED(c);
+}
+}  // namespace
+
+bool attention_tc_ok(const AttnP &p) {
+    if (p.type == WOCR_F32 || p.dim % 8 || p.dim > 128 || p.kv_len < 1) return false;
+    if (p.kv_len > kMaxTiles * 128 || (int64_t)p.batch * p.heads * ((p.q_len + 255) / 256) > 0x7fffffff) return false;
+    // TMA: 16-byte rows, at most 2^40 bytes apart, and no broadcast dimension
+    auto fits = [](const void *x, const int64_t *st, int batch, int heads, int tokens) {
+        const int n[3] = {batch, heads, tokens};
+        if ((uintptr_t)x % 16) return false;
+        for (int d = 0; d < 3; d++)
+            if (n[d] > 1 && (st[d] % 8 || st[d] <= 0 || st[d] >= 1ll << 38)) return false;
+        return true;
+    };
+    return fits(p.q, p.qs, p.batch, p.heads, p.q_len) && fits(p.k, p.ks, p.batch, p.kv_heads, p.kv_len) &&
+           fits(p.v, p.vs, p.batch, p.kv_heads, p.kv_len);
+}
+
+void attention_tc(Ctx *c, const AttnP &p, cudaStream_t s) {
+    const bool bf = p.type == WOCR_BF16;
+    TcArgs ta;
+    ta.a = p;
+    ta.status = c->status;
+    ta.budget = kWaitBudget;
+    ta.tiles = (p.q_len + 255) / 256;
+    ta.vec_out = (uintptr_t)p.o % 16 == 0 && p.os[0] % 8 == 0 && p.os[1] % 8 == 0 && p.os[2] % 8 == 0;
+    CUtensorMap mq, mk, mv;
+    make_map(mq, bf, p.q, p.qs, p.batch, p.heads, p.q_len, p.dim);
+    make_map(mk, bf, p.k, p.ks, p.batch, p.kv_heads, p.kv_len, p.dim);
+    make_map(mv, bf, p.v, p.vs, p.batch, p.kv_heads, p.kv_len, p.dim);
+    if (p.dim <= 64) {
+        if (bf) launch<__nv_bfloat16, 64>(c, ta, mq, mk, mv, s);
+        else launch<__half, 64>(c, ta, mq, mk, mv, s);
+    } else {
+        if (bf) launch<__nv_bfloat16, 128>(c, ta, mq, mk, mv, s);
+        else launch<__half, 128>(c, ta, mq, mk, mv, s);
+    }
+}
+
+}  // namespace k
+}  // namespace wocr
