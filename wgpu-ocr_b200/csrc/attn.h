@@ -188,12 +188,85 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&parts)[Parts
 }
 
 // ---- partial results ------------------------------------------------------------------------
-// Part x of 16 rows: maximum and sum of the weights seen, and the weighted values.
+// Sums over some of the keys for 16 rows: maximum and sum of the weights, and the weighted values.
 template <int DP>
 struct PartSums {
     float o[16][DP];
     float m[16], l[16];
 };
+struct JoinSmem {
+    float weight[64 * 32];  // a part's share of a row
+    uint8_t odd[64];        // rows whose sums are not finite
+};
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
+
+// The parts of a cluster's blocks, joined and stored.  Four warps of a block wrote parts[warp]:
+// with PER = 4 the same 16 rows each, with PER = 1 rows 16 warp ..; row r is query query(r) of head
+// head(r), query < 0: none.  The blocks share the values out.
+template <typename T, int DP, int PER, typename Head, typename Query>
+__device__ __forceinline__ void join_parts(const AttnP &p, int b, PartSums<DP> *parts, JoinSmem &js, Head &&head, Query &&query) {
+    constexpr int ROWS = PER == 4 ? 16 : 64;
+    cg::cluster_group cl = cg::this_cluster();
+    const int cs = cl.num_blocks(), rank = cl.block_rank();
+    cl.sync();
+    if (threadIdx.x < ROWS) {
+        const int r = threadIdx.x;
+        float m = -INFINITY, l = 0.f;
+        js.odd[r] = 0;
+        auto part = [&](int c, int w) -> const PartSums<DP> & { return cl.map_shared_rank(parts, c)[PER == 4 ? w : r / 16]; };
+        for (int c = 0; c < cs; c++)
+            for (int w = 0; w < PER; w++) m = fmaxf(m, part(c, w).m[r % 16]);
+        const float z = m == -INFINITY ? 0.f : m;
+        for (int c = 0; c < cs; c++)
+            for (int w = 0; w < PER; w++) {
+                const float f = ex2(part(c, w).m[r % 16] - z);
+                l += f * part(c, w).l[r % 16];
+                js.weight[(c * PER + w) * ROWS + r] = f;
+            }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        for (int x = 0; x < cs * PER; x++) js.weight[x * ROWS + r] *= inv;
+    }
+    __syncthreads();
+    for (int u = rank * 128 + threadIdx.x; u < ROWS * DP; u += cs * 128) {
+        const int r = u / DP, d = u % DP, i = query(r);
+        if (i < 0 || d >= p.dim) continue;
+        float v = 0.f;
+        for (int c = 0; c < cs; c++) {
+            const PartSums<DP> *pc = cl.map_shared_rank(parts, c);
+#pragma unroll
+            for (int w = 0; w < PER; w++) v += js.weight[(c * PER + w) * ROWS + r] * pc[PER == 4 ? w : r / 16].o[r % 16][d];
+        }
+        if (!finite(v)) js.odd[r] = 1;
+        ((T *)p.o)[b * p.os[0] + head(r) * p.os[1] + (int64_t)i * p.os[2] + d] = from_f<T>(v);
+    }
+    cl.sync();  // the parts are read until here; non-finite rows are written after the others
+    for (int r = threadIdx.x >> 5; r < ROWS; r += 4)
+        if (js.odd[r] && query(r) >= 0) row_by_warp<T>(p, b, head(r), query(r));
+}
+
+// Blocks of a cluster that share the keys of one unit of work: while the GPU has room and each
+// keeps `least` keys or more.
+inline int key_split(const Ctx *c, int64_t units, int per_sm, int kv_len, int least) {
+    int cs = 1;
+    while (cs < 8 && units * cs < (int64_t)per_sm * c->sm_count && kv_len >= 2 * cs * least) cs *= 2;
+    return cs;
+}
+template <typename... A>
+inline void launch_cluster(void (*kernel)(A...), dim3 grid, int threads, int cs, size_t smem, cudaStream_t s, A... args) {
+    if (smem > 48 * 1024) WOCR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    WOCR_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
 
 }  // namespace attn
 }  // namespace k

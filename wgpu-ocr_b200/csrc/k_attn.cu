@@ -69,9 +69,9 @@ __device__ __forceinline__ void mma_parts(float (&c)[4], const uint32_t (&a)[N][
         for (int x = N - 1 - y; x >= 0; x--) mma16816<typename Parts<T>::E>(c, a[x], b0[y], b1[y]);
 }
 
-// Four warps.  FEW: all have the same 16 rows, which are the queries of all heads that share a key
-// head (row r: head r / q_len, query r % q_len), and each a quarter of a tile's keys; otherwise 64
-// queries of one head, 16 to a warp.  A cluster's blocks share the keys out tile by tile; partial
+// Four warps.  FEW: all have the same 16 rows of the queries of all heads that share a key head (row
+// r: head r / q_len, query r % q_len), and each a quarter of a tile's keys; otherwise 64 queries of
+// one head, 16 to a warp.  A cluster's blocks share the keys out tile by tile; partial
 // results are joined in shared memory.
 template <typename T, int DP, bool FEW>
 __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ AttnP p, int vec) {
@@ -81,8 +81,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
     constexpr int WK = FEW ? BK / 4 : BK;  // keys of a warp in a tile
     constexpr int NT = WK / 8;
     extern __shared__ __align__(16) uint8_t dyn[];
-    __shared__ float weight[2][64][8];  // joining: a part's share of a row
-    __shared__ uint8_t odd[64];         // rows whose sums are not finite
+    __shared__ JoinSmem js;
     __shared__ int ends[64], seen;
     uint16_t *sq = (uint16_t *)dyn, *sk = (uint16_t *)(dyn + S::q), *sv = (uint16_t *)(dyn + S::q + S::kv);
     cg::cluster_group cl = cg::this_cluster();
@@ -94,15 +93,15 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
     const int b = blockIdx.x / cs / hx, hq = blockIdx.x / cs % hx;
     const int hk = FEW ? hq : hq / group;
     const Span sp = span_of(p, b);
-    const int nrows = FEW ? group * p.q_len : 64;
+    const int nrows = group * p.q_len;
     // head and query of a row of the block; -1 for rows past the last
-    auto row_head = [&](int r) { return FEW ? hk * group + r / p.q_len : hq; };
+    auto row_head = [&](int r) { return FEW ? hk * group + min(tile * 16 + r, nrows - 1) / p.q_len : hq; };
     auto row_query = [&](int r) {
-        const int i = FEW ? r % p.q_len : tile * 64 + r;
-        return (FEW ? r < nrows : true) && i < sp.nq ? i : -1;
+        const int i = FEW ? (tile * 16 + r) % p.q_len : tile * 64 + r;
+        return (!FEW || tile * 16 + r < nrows) && i < sp.nq ? i : -1;
     };
     if (threadIdx.x == 0) seen = 0;
-    if (threadIdx.x < 64) odd[threadIdx.x] = 0;
+    if (threadIdx.x < 64) js.odd[threadIdx.x] = 0;
     __syncthreads();
     if (threadIdx.x < (FEW ? 16 : 64)) {
         const int i = row_query(threadIdx.x);
@@ -152,8 +151,8 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
         int e = min(i0 >= 0 ? e0 : 0x7fffffff, i1 >= 0 ? e1 : 0x7fffffff);
         all = __reduce_min_sync(0xffffffffu, e);
     }
-    const float sl0 = p.slopes ? p.slopes[row_head(min(r0, nrows - 1))] * kLog2e : 0.f;
-    const float sl1 = p.slopes ? p.slopes[row_head(min(r1, nrows - 1))] * kLog2e : 0.f;
+    const float sl0 = p.slopes ? p.slopes[row_head(r0)] * kLog2e : 0.f;
+    const float sl1 = p.slopes ? p.slopes[row_head(r1)] * kLog2e : 0.f;
     const int d0 = p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
     const int *kd = p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
     const int pos0 = sp.off + i0, pos1 = sp.off + i1;
@@ -320,18 +319,18 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
             for (int x = 0; x < 2; x++) {
                 const int d = n * 8 + (lane & 3) * 2 + x;
                 const float u = acc[n][x] * v0, w = acc[n][2 + x] * v1;
-                bad0 |= !(fabsf(u) <= 3.4028234e38f);
-                bad1 |= !(fabsf(w) <= 3.4028234e38f);
+                bad0 |= !finite(u);
+                bad1 |= !finite(w);
                 if (d < p.dim) {
                     if (i0 >= 0) ob[hq * p.os[1] + (int64_t)i0 * p.os[2] + d] = from_f<T>(u);
                     if (i1 >= 0) ob[hq * p.os[1] + (int64_t)i1 * p.os[2] + d] = from_f<T>(w);
                 }
             }
-        if (bad0) odd[r0] = 1;
-        if (bad1) odd[r1] = 1;
+        if (bad0) js.odd[r0] = 1;
+        if (bad1) js.odd[r1] = 1;
         __syncwarp();
         for (int r = wr; r < wr + 16; r++)
-            if (odd[r] && row_query(r) >= 0) row_by_warp<T>(p, b, hq, row_query(r));
+            if (js.odd[r] && row_query(r) >= 0) row_by_warp<T>(p, b, hq, row_query(r));
         return;
     }
     __syncthreads();  // the tiles have been read: their place holds the parts now
@@ -352,79 +351,227 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
             pt.l[a + 8] = l1;
         }
     }
-    cl.sync();
-    // rows of the block (16 or 64) x parts: cs blocks, and with FEW four warps each (two per slot)
-    const int rows = FEW ? 16 : 64;
-    const int per = FEW ? 4 : 1;
-    if (threadIdx.x < rows) {
-        const int r = threadIdx.x;
-        float m = -INFINITY;
-        for (int c = 0; c < cs; c++)
-            for (int w = 0; w < per; w++)
-                m = fmaxf(m, cl.map_shared_rank(parts, c)[FEW ? w : r / 16].m[r % 16]);
-        const float z = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        for (int c = 0; c < cs; c++)
-            for (int w = 0; w < per; w++) {
-                const PartSums<DP> &pt = cl.map_shared_rank(parts, c)[FEW ? w : r / 16];
-                const float f = ex2(pt.m[r % 16] - z);
-                l += f * pt.l[r % 16];
-                if (FEW) weight[w >> 1][r + 16 * (w & 1)][c] = f;
-                else weight[0][r][c] = f;
-            }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        for (int c = 0; c < cs; c++)
-            for (int w = 0; w < per; w++) {
-                if (FEW) weight[w >> 1][r + 16 * (w & 1)][c] *= inv;
-                else weight[0][r][c] *= inv;
-            }
+    join_parts<T, DP, FEW ? 4 : 1>(p, b, parts, js, row_head, row_query);
+}
+
+// A few queries over 16-bit keys and values, straight from global memory into the matrix
+// instructions' operands: a dot product may take the dimensions, and a weighted sum the keys, in any
+// order that both sides share.  A thread's 16-byte load of key (lane / 4) holds its words of two
+// left-hand steps (dimensions 8 (lane % 4) .. of a 32), and its loads of values at its own four
+// weights' keys hold dimensions DP / 8 (lane / 4) .., paired by byte permutes.  No shared memory or
+// barrier until the parts are joined; keys of the next 16 are loaded while the softmax of these runs.
+// Bound: the keys' and values' bytes.  16 rows of the queries of all heads that share a key head.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) k_attn_token(const __grid_constant__ AttnP p) {
+    constexpr int C = DP / 32, VW = DP / 64;  // 32-dimension chunks; 16-byte words of a value row per thread
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ JoinSmem js;
+    PartSums<DP> *parts = (PartSums<DP> *)dyn;
+    cg::cluster_group cl = cg::this_cluster();
+    const int cs = cl.num_blocks(), rank = cl.block_rank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q4 = lane & 3;
+    const int group = p.heads / p.kv_heads, nrows = group * p.q_len, tile = blockIdx.y;
+    const int b = blockIdx.x / cs / p.kv_heads, hk = blockIdx.x / cs % p.kv_heads;
+    const Span sp = span_of(p, b);
+    auto row_head = [&](int r) { return hk * group + min(tile * 16 + r, nrows - 1) / p.q_len; };
+    auto row_query = [&](int r) {
+        const int i = (tile * 16 + r) % p.q_len;
+        return tile * 16 + r < nrows && i < sp.nq ? i : -1;
+    };
+    const int i0 = row_query(g), i1 = row_query(g + 8);
+    const int e0 = i0 >= 0 ? key_end(p, sp, i0) : 0, e1 = i1 >= 0 ? key_end(p, sp, i1) : 0;
+    const int last = __reduce_max_sync(0xffffffffu, max(e0, e1));
+    const int all = __reduce_min_sync(0xffffffffu, min(i0 >= 0 ? e0 : 0x7fffffff, i1 >= 0 ? e1 : 0x7fffffff));
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    uint4 q0[C], q1[C];
+    const T *qb = (const T *)p.q + b * p.qs[0];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int d = c * 32 + q4 * 8;
+        q0[c] = i0 >= 0 && d < p.dim ? *(const uint4 *)(qb + row_head(g) * p.qs[1] + (int64_t)i0 * p.qs[2] + d) : none;
+        q1[c] = i1 >= 0 && d < p.dim ? *(const uint4 *)(qb + row_head(g + 8) * p.qs[1] + (int64_t)i1 * p.qs[2] + d) : none;
     }
-    __syncthreads();
-    // the cluster's blocks share the values out
-    for (int u = rank * 128 + threadIdx.x; u < rows * DP; u += cs * 128) {
-        const int r = u / DP, d = u % DP, i = row_query(r);
-        if (i < 0 || d >= p.dim) continue;
-        float v = 0.f;
-        for (int c = 0; c < cs; c++)
-            for (int w = 0; w < per; w++)
-                v += (FEW ? weight[w >> 1][r + 16 * (w & 1)][c] : weight[0][r][c]) *
-                     cl.map_shared_rank(parts, c)[FEW ? w : r / 16].o[r % 16][d];
-        if (!(fabsf(v) <= 3.4028234e38f)) odd[r] = 1;
-        ob[row_head(r) * p.os[1] + (int64_t)i * p.os[2] + d] = from_f<T>(v);
+    const float sl0 = p.slopes ? p.slopes[row_head(g)] * kLog2e : 0.f, sl1 = p.slopes ? p.slopes[row_head(g + 8)] * kLog2e : 0.f;
+    const int d0 = p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
+    const int *kd = p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
+    const int pos0 = sp.off + i0, pos1 = sp.off + i1;
+    const float scale2 = p.scale * kLog2e;
+    const T *kb = (const T *)p.k + b * p.ks[0] + hk * p.ks[1] + q4 * 8;
+    const T *vb = (const T *)p.v + b * p.vs[0] + hk * p.vs[1] + g * (DP / 8);
+    uint4 kw[2][C], vw[4][VW];
+    auto load_k = [&](int j0) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int j = j0 + t * 8 + g;
+            const T *at = kb + (int64_t)j * p.ks[2];
+#pragma unroll
+            for (int c = 0; c < C; c++) kw[t][c] = j < last && c * 32 + q4 * 8 < p.dim ? __ldg((const uint4 *)(at + c * 32)) : none;
+        }
+    };
+    auto load_v = [&](int j0) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int j = j0 + (t >> 1) * 8 + q4 * 2 + (t & 1);
+            const T *at = vb + (int64_t)j * p.vs[2];
+#pragma unroll
+            for (int c = 0; c < VW; c++) vw[t][c] = j < last && g * (DP / 8) + c * 8 < p.dim ? __ldg((const uint4 *)(at + c * 8)) : none;
+        }
+    };
+    float acc[DP / 8][4];
+#pragma unroll
+    for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) acc[n][x] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    const int step = cs * 64;
+    int j0 = (rank * 4 + warp) * 16;
+    load_k(j0);
+    load_v(j0);
+    for (; j0 < last; j0 += step) {
+        float s[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int x = 0; x < 4; x++) s[t][x] = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                const uint32_t a0[4] = {q0[c].x, q1[c].x, q0[c].y, q1[c].y}, a1[4] = {q0[c].z, q1[c].z, q0[c].w, q1[c].w};
+                mma16816<T>(s[t], a0, kw[t][c].x, kw[t][c].y);
+                mma16816<T>(s[t], a1, kw[t][c].z, kw[t][c].w);
+            }
+        }
+        load_k(j0 + step);
+        const bool whole = j0 + 16 <= all && !kd;
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int j = j0 + t * 8 + q4 * 2 + x;
+                float u = s[t][x], w = s[t][2 + x];
+                if (p.cap > 0.f) {
+                    u = capped2<T>(u * p.scale, p.cap);
+                    w = capped2<T>(w * p.scale, p.cap);
+                } else {
+                    u *= scale2;
+                    w *= scale2;
+                }
+                if (p.slopes) {
+                    u -= sl0 * fabsf((float)(pos0 - j));
+                    w -= sl1 * fabsf((float)(pos1 - j));
+                }
+                if (!whole) {
+                    bool in0 = j < e0, in1 = j < e1;
+                    if (kd) {
+                        const int doc = j < sp.nk ? kd[j] : -1;
+                        in0 = in0 && doc == d0 && doc >= 0;
+                        in1 = in1 && doc == d1 && doc >= 0;
+                    }
+                    if (!in0) u = -INFINITY;
+                    if (!in1) w = -INFINITY;
+                }
+                s[t][x] = u;
+                s[t][2 + x] = w;
+                t0 = fmaxf(t0, u);
+                t1 = fmaxf(t1, w);
+            }
+#pragma unroll
+        for (int d = 1; d < 4; d *= 2) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+        }
+        const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+        const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+        const float c0 = ex2(m0 - z0), c1 = ex2(m1 - z1);
+        const bool grown = __any_sync(0xffffffffu, n0 > m0 || n1 > m1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= c0;
+        l1 *= c1;
+        uint32_t a[4];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const float x0 = ex2(s[t][0] - z0), x1 = ex2(s[t][1] - z0), y0 = ex2(s[t][2] - z1), y1 = ex2(s[t][3] - z1);
+            l0 += x0 + x1;
+            l1 += y0 + y1;
+            a[2 * t] = pack2<T>(x0, x1);  // rounded once, to the values' type
+            a[2 * t + 1] = pack2<T>(y0, y1);
+        }
+        if (grown) {
+#pragma unroll
+            for (int n = 0; n < DP / 8; n++) {
+                acc[n][0] *= c0;
+                acc[n][1] *= c0;
+                acc[n][2] *= c1;
+                acc[n][3] *= c1;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; n += 2) {
+            uint32_t w[4];  // dimensions n, n + 1 of the thread's four keys
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const uint4 &v = vw[t][n / 8];
+                w[t] = (n & 7) == 0 ? v.x : (n & 7) == 2 ? v.y : (n & 7) == 4 ? v.z : v.w;
+            }
+            mma16816<T>(acc[n], a, __byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+            mma16816<T>(acc[n + 1], a, __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+        }
+        load_v(j0 + step);
     }
-    cl.sync();  // the parts are read until here; non-finite rows are written after the others
-    for (int r = warp; r < rows; r += 4)
-        if (odd[r] && row_query(r) >= 0) row_by_warp<T>(p, b, row_head(r), row_query(r));
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    PartSums<DP> &pt = parts[warp];
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int n = 0; n < DP / 8; n += 2) {
+            const int d = (2 * q4 + x) * (DP / 8) + n;
+            *reinterpret_cast<float2 *>(&pt.o[g][d]) = make_float2(acc[n][x], acc[n + 1][x]);
+            *reinterpret_cast<float2 *>(&pt.o[g + 8][d]) = make_float2(acc[n][2 + x], acc[n + 1][2 + x]);
+        }
+    if (q4 == 0) {
+        pt.m[g] = m0;
+        pt.m[g + 8] = m1;
+        pt.l[g] = l0;
+        pt.l[g + 8] = l1;
+    }
+    join_parts<T, DP, 4>(p, b, parts, js, row_head, row_query);
+}
+
+dim3 grid_of(int64_t units, int cs, int64_t tiles) {
+    if (units * cs > 0x7fffffff || tiles > 65535) fail(WOCR_ERR_UNSUPPORTED, "attention: too many heads or queries");
+    return dim3((unsigned)(units * cs), (unsigned)tiles);
 }
 
 template <typename T, int DP, bool FEW>
 void launch_tiles(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
     using S = TileSmem<T, DP>;
     const int64_t units = (int64_t)p.batch * (FEW ? p.kv_heads : p.heads);
-    const int tiles = FEW ? 1 : (p.q_len + 63) / 64;
-    // blocks that share a row's keys: while the GPU has room and each keeps two tiles or more
-    int cs = 1;
-    while (cs < 8 && units * tiles * cs < 2 * c->sm_count && p.kv_len > 2 * cs * S::BK) cs *= 2;
-    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tiles<T, DP, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::bytes));
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = S::bytes;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cs;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    if (units * cs > 0x7fffffff || tiles > 65535) fail(WOCR_ERR_UNSUPPORTED, "attention: too many heads or queries");
-    cfg.gridDim = dim3((unsigned)(units * cs), tiles);
-    WOCR_CUDA(cudaLaunchKernelEx(&cfg, k_attn_tiles<T, DP, FEW>, p, vec));
+    const int tiles = FEW ? (p.heads / p.kv_heads * p.q_len + 15) / 16 : (p.q_len + 63) / 64;
+    const int cs = key_split(c, units * tiles, 2, p.kv_len, 2 * S::BK);
+    launch_cluster<const AttnP, int>(k_attn_tiles<T, DP, FEW>, grid_of(units, cs, tiles), 128, cs, S::bytes, s, p, vec);
     WOCR_LAUNCHED(c);
 }
 
 template <typename T, int DP>
+void launch_token(Ctx *c, const AttnP &p, cudaStream_t s) {
+    const int64_t units = (int64_t)p.batch * p.kv_heads;
+    const int tiles = (p.heads / p.kv_heads * p.q_len + 15) / 16;
+    const int cs = key_split(c, units * tiles, 4, p.kv_len, 128);  // two blocks of 16 keys a warp
+    launch_cluster<const AttnP>(k_attn_token<T, DP>, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
+    WOCR_LAUNCHED(c);
+}
+
+// The queries of the heads that share a key head are taken together: a few tokens of a decoder.
+bool few_rows(const AttnP &p) { return p.q_len <= 16 && (int64_t)p.heads / p.kv_heads * p.q_len <= 64; }
+
+template <typename T, int DP>
 void launch_dim(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
-    if ((int64_t)p.heads / p.kv_heads * p.q_len <= 16) launch_tiles<T, DP, true>(c, p, vec, s);
+    if (few_rows(p)) launch_tiles<T, DP, true>(c, p, vec, s);
     else launch_tiles<T, DP, false>(c, p, vec, s);
 }
 
@@ -434,6 +581,9 @@ void launch_type(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int n = 16 / sizeof(T);
     bool vec = ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0;
     for (int i = 0; i < 3; i++) vec = vec && p.qs[i] % n == 0 && p.ks[i] % n == 0 && p.vs[i] % n == 0;
+    if constexpr (Parts<T>::n == 1)
+        if (few_rows(p) && vec && p.dim % 8 == 0 && p.dim <= 128)
+            return p.dim <= 64 ? launch_token<T, 64>(c, p, s) : launch_token<T, 128>(c, p, s);
     if (p.dim <= 16) launch_dim<T, 16>(c, p, vec, s);
     else if (p.dim <= 32) launch_dim<T, 32>(c, p, vec, s);
     else if (p.dim <= 64) launch_dim<T, 64>(c, p, vec, s);
