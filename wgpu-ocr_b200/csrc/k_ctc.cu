@@ -25,6 +25,13 @@ __device__ __forceinline__ float on_step(float x) {
     return fabsf(x) < 0.015625f ? rintf(x * kStep) * (1.f / kStep) : x;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // What a step's logits leave for the search: its best classes apart from the blank (value, class;
 // class -1 behind the last), the blank's logit and the log-sum-exp.
 struct Step {
@@ -91,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) k_ctc_rows(const CtcP p, const Step 
 #pragma unroll 8
     for (int e = tid; e < n; e += kThreads) {
         const float x = on_step(to_f(cached ? store[e] : row[e]));
-        if (m > -INFINITY) s += exp2f((x - m) * 1.4426950408889634f);
+        if (m > -INFINITY) s += exp2_of((x - m) * kLog2e);
         const Key key = make_key(x, e);
         if (key >= cut && e != p.blank) {
             const int g = atomicAdd(&sm.count, 1);
@@ -139,10 +146,38 @@ __global__ void __launch_bounds__(kThreads) k_ctc_rows(const CtcP p, const Step 
     }
 }
 
-__device__ __forceinline__ double log_add(double a, double b) {
-    const double hi = fmax(a, b), lo = fmin(a, b);
-    return lo == -INFINITY ? hi : hi + log1p(exp(lo - hi));
-}
+// log(1 + e^-d) for d >= 0, on 608 intervals of 1/16 up to 38 (beyond, it is below 2^-54): the Taylor
+// polynomial of degree 7 about an interval's middle leaves (1/32)^8 / 8! max |f^(8)| < 2^-55.  With
+// s = 1 / (1 + e^d) and u = s (1 - s): f' = -s, f'' = u and f^(n+1) = -u df^(n)/ds.
+constexpr int kLogs = 608;
+struct LogTable {
+    double c[kLogs][8];
+    __device__ void fill(int tid, int n) {
+        for (int i = tid; i < kLogs; i += n) {
+            const double d = (i + 0.5) / 16, e = exp(-d), s = e / (1 + e), u = s * (1 - s), w = 1 - 2 * s;
+            c[i][0] = log1p(e);
+            c[i][1] = -s;
+            c[i][2] = u / 2;
+            c[i][3] = -u * w / 6;
+            c[i][4] = u * (1 - 6 * u) / 24;
+            c[i][5] = -u * w * (1 - 12 * u) / 120;
+            c[i][6] = u * (1 - 30 * u + 120 * u * u) / 720;
+            c[i][7] = -u * w * (1 - 60 * u + 360 * u * u) / 5040;
+        }
+    }
+    __device__ __forceinline__ double add(double a, double b) const {
+        const double hi = fmax(a, b), d = hi - fmin(a, b);
+        if (!(d < 38.0)) return hi;  // -inf and both -inf among them
+        const int i = (int)(d * 16);
+        const double x = d - (i + 0.5) / 16;
+        const double2 *q = reinterpret_cast<const double2 *>(c[i]);
+        const double2 q0 = q[0], q1 = q[1], q2 = q[2], q3 = q[3];
+        // by halves: a shorter chain than Horner's
+        const double x2 = x * x, x4 = x2 * x2;
+        const double lo = fma(fma(q1.y, x, q1.x), x2, fma(q0.y, x, q0.x)), up = fma(fma(q3.y, x, q3.x), x2, fma(q2.y, x, q2.x));
+        return hi + fma(up, x4, lo);
+    }
+};
 
 // A text's identity: 64 bits mixed class by class (the multiply-xorshift finaliser of splitmix64,
 // Steele, Lea and Flood, 2014).
@@ -153,102 +188,149 @@ __device__ __forceinline__ uint64_t grow(uint64_t h, int c) {
     return h ^ (h >> 31);
 }
 
-constexpr int kSearch = 128;                     // threads of a search block
-constexpr int kMaxPairs = 160;                   // sum of floor(W / i) + 1 over i <= 31: 142
-constexpr int kMaxCand = 2 * 32 + kMaxPairs;
+// Pairs of a beam i (from 0, in descending order) and a class k (from 0, best first) with
+// k (i + 1) <= width.
+constexpr int pairs(int width) {
+    int n = 0;
+    for (int i = 1; i <= width; i++) n += width / i + 1;
+    return n;
+}
+constexpr int candidates(int width) { return 2 * width + pairs(width); }
+constexpr int kMaxCand = candidates(kMaxWidth);
+constexpr int kMaxSearch = (4 * kMaxCand + 31) / 32 * 32;
 constexpr int kTrace = 64;                       // steps traced back per load
 
+struct Beams {
+    double pb[32], pn[32], tot[32];
+    uint64_t hash[32], before[32];               // of the text, and of the text without its last class
+    int last[32], len[32];
+    float xl[32];                                // the step's logit of the last class
+    int live;
+};
+// What orders a candidate: the log mass in steps, its bits made monotone, and its place.
+struct __align__(16) Order {
+    int64_t key;
+    uint32_t place, unused;
+};
+constexpr int64_t kNever = INT64_MIN;
+
 struct SearchSmem {
-    double pb[2][32], pn[2][32], tot[2][32];
-    uint64_t hash[2][32];
-    int last[2][32], len[2][32];
-    double key[kMaxCand], cb[kMaxCand], cn[kMaxCand];
-    uint32_t place[kMaxCand];
-    uint8_t pi[kMaxPairs], pk[kMaxPairs];
-    float xl[32];                                // the logit of each beam's last class
-    float val[32];
-    int cls[32];
+    LogTable log;
+    Beams beams[2];
+    Order order[(kMaxCand + 7) / 8 * 8];
+    double cb[kMaxCand], cn[kMaxCand], ct[32];
+    uint8_t pi[kMaxCand], pk[kMaxCand];
+    uint32_t kids[2][32];                        // beams that are a beam's text and a class more
+    int parent[32];                              // and the beam that a text is one class more than, or -1
+    float val[2][32];
+    int cls[2][32];
+    float next[2][32];                           // the next step's logits of the beams' last classes, of the best classes
+    double blank[2], norm;
     uint32_t back[kTrace * 32];
-    int live[2];
-    int pairs;
 };
 
-// A block per line, step after step.  Beams lie in descending order, so of beam i (from 0) only the
-// classes k with k (i + 1) <= width can be among the best: each pair before (i, k) in both orders is
-// as good, but for one class a beam repeats, and a pair that grows into a held text leaves that
-// text's own candidate as good.  Candidates in the order of their places: texts kept, then (beam,
-// class); each one's rank is the number of better ones.
+// A block per line, step after step.  Of beam i only the classes k with k (i + 1) <= width can be
+// among the best: each pair before (i, k) in both orders is as good, but for one class that a beam
+// repeats, and where a pair grows into a held text, that text's own candidate is as good.  Candidates
+// in the order of their places: texts kept, then (beam, class); each one's rank is the number of
+// better ones, counted by four threads.
+// Bound: latency.  What a step reads is loaded a step ahead: its best classes, and its logits of every
+// class that a beam may then end in (the beams' last classes and the best classes of the step before),
+// which a prefetch into L2 has asked for a step earlier still.
 template <typename T>
-__global__ void __launch_bounds__(kSearch) k_ctc_search(const CtcP p, const Step st, uint32_t *back) {
-    __shared__ SearchSmem sm;
-    const int line = blockIdx.x, tid = threadIdx.x, W = p.width, K = W + 1;
+__global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const Step st, uint32_t *back) {
+    extern __shared__ __align__(16) uint8_t dyn[];
+    SearchSmem &sm = *reinterpret_cast<SearchSmem *>(dyn);
+    const int line = blockIdx.x, tid = threadIdx.x, N = blockDim.x, lane = tid & 31, warp = tid >> 5, W = p.width, K = W + 1;
     const int len = p.lens ? min(max(p.lens[line], 0), p.steps) : p.steps;
+    const int cand = candidates(W), slots = (cand + 7) / 8 * 8;
     const T *x0 = (const T *)p.logits + line * p.ln;
-    uint32_t *bk = back + (int64_t)line * p.steps * W;
+    const int64_t r0 = (int64_t)line * p.steps;
+    uint32_t *bk = back + r0 * W;
+    sm.log.fill(tid, N);
+    if (tid < 64) sm.kids[tid >> 5][lane] = 0;
+    for (int u = tid; u < slots; u += N) sm.order[u] = {kNever, 0xffffffffu, 0};
     if (tid == 0) {
-        int n = 0;
-        for (int i = 0; i < W; i++)
-            for (int k = 0; k * (i + 1) <= W && k < K; k++) {
+        int n = 2 * W;
+        for (int i = 0; i < W; i++) {
+            sm.pi[i] = sm.pi[W + i] = i;
+            for (int k = 0; k * (i + 1) <= W; k++) {
                 sm.pi[n] = i;
                 sm.pk[n++] = k;
             }
-        sm.pairs = n;
-        sm.live[0] = 1;
-        sm.pb[0][0] = 0.0;
-        sm.pn[0][0] = -INFINITY;
-        sm.tot[0][0] = 0.0;
-        sm.hash[0][0] = 0;
-        sm.last[0][0] = -1;
-        sm.len[0][0] = 0;
+        }
+        Beams &b = sm.beams[0];
+        b.live = 1;
+        b.pb[0] = b.tot[0] = 0.0;
+        b.pn[0] = -INFINITY;
+        b.hash[0] = 0;
+        b.before[0] = ~0ull;
+        b.last[0] = -1;
+        b.len[0] = 0;
+        b.xl[0] = -INFINITY;
+        if (len > 0) sm.blank[0] = st.blank[r0];
+    }
+    if (tid < K && len > 0) {
+        sm.val[0][tid] = st.val[r0 * K + tid];
+        sm.cls[0][tid] = st.cls[r0 * K + tid];
     }
     __syncthreads();
-    const int cand = 2 * W + sm.pairs;
-    double norm = 0;
     int cur = 0;
     for (int t = 0; t < len; t++, cur ^= 1) {
-        const int64_t r = (int64_t)line * p.steps + t;
-        const int n = sm.live[cur];
-        if (tid < K) {
-            sm.val[tid] = st.val[r * K + tid];
-            sm.cls[tid] = st.cls[r * K + tid];
+        const int64_t r = r0 + t;
+        Beams &now = sm.beams[cur], &then = sm.beams[cur ^ 1];
+        const int n = now.live;
+        // loads for the next step, stored at the end of this one's first half
+        T nx = from_f<T>(0.f);
+        float nv = 0.f, nb = 0.f;
+        int nc = -1;
+        const bool more = t + 1 < len;
+        if (more && warp < 2) {
+            const int c = warp == 0 ? (lane < n ? now.last[lane] : -1) : (lane < K ? sm.cls[cur][lane] : -1);
+            const T *row = x0 + (t + 1) * p.lt;
+            if (c >= 0) nx = row[c];
+            if (warp == 1 && lane < K) {
+                nv = st.val[(r + 1) * K + lane];
+                nc = st.cls[(r + 1) * K + lane];
+            }
+            if (tid == 0) nb = st.blank[r + 1];
+            if (t + 2 < len && c >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + p.lt + c));
         }
-        if (tid < n) {
-            const int c = sm.last[cur][tid];
-            sm.xl[tid] = c >= 0 ? on_step(to_f(x0[t * p.lt + c])) : -INFINITY;
-        }
-        if (tid == 0) {
-            norm += st.lse[r];
-            sm.live[cur ^ 1] = 0;
-        }
-        const double xb = st.blank[r];
-        __syncthreads();
-        for (int u = tid; u < cand; u += kSearch) {
-            double b = -INFINITY, q = -INFINITY;
-            uint32_t place = 0xffffffffu;
-            if (u < W) {
-                const int i = u;
-                if (i < n) {
-                    b = sm.tot[cur][i] + xb;
-                    q = sm.pn[cur][i] + sm.xl[i];
-                    if (sm.len[cur][i] > 0) {
-                        const int c = sm.last[cur][i];
-                        for (int o = 0; o < n; o++)
-                            if (sm.len[cur][o] + 1 == sm.len[cur][i] && grow(sm.hash[cur][o], c) == sm.hash[cur][i])
-                                q = log_add(q, (sm.last[cur][o] == c ? sm.pb[cur][o] : sm.tot[cur][o]) + sm.xl[i]);
-                    }
-                    place = i;
+        // which beams are one class more than another: a warp per longer text, lanes are the shorter
+        {
+            const uint64_t h = lane < n ? now.hash[lane] : 0;
+            const int size = lane < n ? now.len[lane] + 1 : -1;
+            for (int j = warp; j < n; j += N / 32) {
+                const uint32_t m = __ballot_sync(0xffffffffu, h == now.before[j] && size == now.len[j]);
+                if (lane == 0) {
+                    sm.parent[j] = m ? __ffs(m) - 1 : -1;
+                    if (m) atomicOr(&sm.kids[cur][__ffs(m) - 1], 1u << j);
                 }
-            } else {
-                const bool again = u < 2 * W;
-                const int i = again ? u - W : sm.pi[u - 2 * W];
-                if (i < n) {
-                    const int c = again ? sm.last[cur][i] : sm.cls[sm.pk[u - 2 * W]];
-                    if (c >= 0 && (again || c != sm.last[cur][i])) {
-                        const uint64_t h = grow(sm.hash[cur][i], c);
+            }
+        }
+        if (tid == N - 1) then.live = 0;
+        __syncthreads();
+        const double xb = sm.blank[cur];
+        if (tid < cand) {
+            const int u = tid, i = sm.pi[u];
+            double b = -INFINITY, q = -INFINITY, total = -INFINITY;
+            uint32_t place = 0xffffffffu;
+            if (i < n) {
+                if (u < W) {
+                    const int o = sm.parent[i];
+                    b = now.tot[i] + xb;
+                    q = now.pn[i] + now.xl[i];
+                    if (o >= 0) q = sm.log.add(q, (now.last[o] == now.last[i] ? now.pb[o] : now.tot[o]) + now.xl[i]);
+                    sm.ct[i] = total = sm.log.add(b, q);
+                    place = i;
+                } else {
+                    const bool again = u < 2 * W;
+                    const int k = sm.pk[u], c = again ? now.last[i] : sm.cls[cur][k];
+                    if (c >= 0 && (again || c != now.last[i])) {
                         bool held = false;
-                        for (int o = 0; o < n; o++) held |= sm.hash[cur][o] == h && sm.len[cur][o] == sm.len[cur][i] + 1;
+                        for (uint32_t kids = sm.kids[cur][i]; kids; kids &= kids - 1) held |= now.last[__ffs(kids) - 1] == c;
                         if (!held) {
-                            q = again ? sm.pb[cur][i] + sm.xl[i] : sm.tot[cur][i] + sm.val[sm.pk[u - 2 * W]];
+                            total = q = again ? now.pb[i] + now.xl[i] : now.tot[i] + sm.val[cur][k];
                             place = W + (uint32_t)i * p.classes + c;
                         }
                     }
@@ -256,54 +338,71 @@ __global__ void __launch_bounds__(kSearch) k_ctc_search(const CtcP p, const Step
             }
             sm.cb[u] = b;
             sm.cn[u] = q;
-            sm.key[u] = rint(log_add(b, q) * (double)kStep);
-            sm.place[u] = place;
+            const int64_t bits = __double_as_longlong(rint(total * (double)kStep) + 0.0);  // -0 as 0
+            sm.order[u] = {total > -INFINITY ? bits ^ ((bits >> 63) & INT64_MAX) : kNever, place, 0};
         }
-        __syncthreads();
-        for (int u = tid; u < cand; u += kSearch) {
-            const double key = sm.key[u];
-            if (!(key > -INFINITY)) continue;
-            const uint32_t place = sm.place[u];
-            int rank = 0;
-            for (int o = 0; o < cand; o++) {
-                const double ko = sm.key[o];
-                rank += ko > key;
-                if (ko == key) rank += sm.place[o] < place;
+        if (tid < 32) sm.kids[cur ^ 1][tid] = 0;
+        if (more && warp < 2) {
+            sm.next[warp][lane] = on_step(to_f(nx));
+            if (warp == 1 && lane < K) {
+                sm.val[cur ^ 1][lane] = nv;
+                sm.cls[cur ^ 1][lane] = nc;
             }
-            if (rank >= W) continue;
-            const int nx = cur ^ 1;
-            const bool kept = u < W;
-            const int i = kept ? u : (u < 2 * W ? u - W : sm.pi[u - 2 * W]);
-            const int c = kept ? -1 : (u < 2 * W ? sm.last[cur][i] : sm.cls[sm.pk[u - 2 * W]]);
-            sm.pb[nx][rank] = sm.cb[u];
-            sm.pn[nx][rank] = sm.cn[u];
-            sm.tot[nx][rank] = log_add(sm.cb[u], sm.cn[u]);
-            sm.hash[nx][rank] = kept ? sm.hash[cur][i] : grow(sm.hash[cur][i], c);
-            sm.last[nx][rank] = kept ? sm.last[cur][i] : c;
-            sm.len[nx][rank] = sm.len[cur][i] + !kept;
-            bk[(int64_t)t * W + rank] = (uint32_t)i << 27 | (uint32_t)(c + 1);
-            atomicMax(&sm.live[nx], rank + 1);
+            if (tid == 0) sm.blank[cur ^ 1] = nb;
+        }
+        __syncthreads();
+        {
+            const int u = tid >> 2;
+            const Order mine = u < cand ? sm.order[u] : Order{kNever, 0, 0};
+            int rank = 0;
+#pragma unroll 4
+            for (int o = tid & 3; o < slots; o += 4) {
+                const Order other = sm.order[o];
+                rank += other.key > mine.key || (other.key == mine.key && other.place < mine.place);
+            }
+            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+            rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+            if (mine.key != kNever && rank < W && (tid & 3) == 0) {
+                const bool kept = u < W, again = u < 2 * W;
+                const int i = sm.pi[u], k = sm.pk[u];
+                const int c = again ? now.last[i] : sm.cls[cur][k];
+                const double q = sm.cn[u];
+                then.pb[rank] = sm.cb[u];
+                then.pn[rank] = q;
+                then.tot[rank] = kept ? sm.ct[u] : q;
+                then.hash[rank] = kept ? now.hash[i] : grow(now.hash[i], c);
+                then.before[rank] = kept ? now.before[i] : now.hash[i];
+                then.last[rank] = c;
+                then.len[rank] = now.len[i] + !kept;
+                then.xl[rank] = c >= 0 ? sm.next[again ? 0 : 1][again ? i : k] : -INFINITY;
+                bk[(int64_t)t * W + rank] = (uint32_t)i << 27 | (uint32_t)(kept ? 0 : c + 1);
+                atomicMax(&then.live, rank + 1);
+            }
         }
         __syncthreads();
     }
-    const int n = sm.live[cur];
+    Beams &end = sm.beams[cur];
+    const int n = end.live;
+    if (warp == 0) {  // the steps' log-sum-exps
+        double norm = 0;
+        for (int t = lane; t < len; t += 32) norm += st.lse[r0 + t];
+        for (int d = 16; d; d /= 2) norm += __shfl_xor_sync(0xffffffffu, norm, d);
+        if (lane == 0) sm.norm = norm;
+    }
     const int64_t o0 = (int64_t)line * p.paths;
-    for (int64_t u = tid; u < (int64_t)p.paths * p.steps; u += kSearch) {
+    for (int64_t u = tid; u < (int64_t)p.paths * p.steps; u += N) {
         const int j = (int)(u / p.steps);
-        if ((int)(u % p.steps) >= (j < n ? sm.len[cur][j] : 0)) p.tokens[(o0 + j) * p.steps + u % p.steps] = -1;
+        if ((int)(u % p.steps) >= (j < n ? end.len[j] : 0)) p.tokens[(o0 + j) * p.steps + u % p.steps] = -1;
     }
-    if (tid < p.paths) {
-        p.lengths[o0 + tid] = tid < n ? sm.len[cur][tid] : 0;
-        if (tid == 0) sm.pb[cur ^ 1][0] = norm;
-    }
+    if (tid < p.paths) p.lengths[o0 + tid] = tid < n ? end.len[tid] : 0;
     __syncthreads();
-    if (tid < p.paths) p.scores[o0 + tid] = tid < n ? (float)(sm.tot[cur][tid] - sm.pb[cur ^ 1][0]) : -INFINITY;
+    if (tid < p.paths) p.scores[o0 + tid] = tid < n ? (float)(end.tot[tid] - sm.norm) : -INFINITY;
     // each path traced back through the steps' origins, kTrace steps in shared memory at a time
-    int j = tid, pos = tid < n ? sm.len[cur][tid] : 0;
+    int j = tid, pos = tid < n ? end.len[tid] : 0;
     for (int t1 = len; t1 > 0; t1 -= kTrace) {
         const int t0 = max(0, t1 - kTrace);
         __syncthreads();
-        for (int u = tid; u < (t1 - t0) * W; u += kSearch) sm.back[u] = bk[(int64_t)t0 * W + u];
+        for (int u = tid; u < (t1 - t0) * W; u += N) sm.back[u] = bk[(int64_t)t0 * W + u];
         __syncthreads();
         if (tid < p.paths && tid < n)
             for (int t = t1 - 1; t >= t0; t--) {
@@ -314,18 +413,161 @@ __global__ void __launch_bounds__(kSearch) k_ctc_search(const CtcP p, const Step
     }
 }
 
+// The same with a row's logits in the registers of N threads, E each: rows of up to N E classes.
+// With N = 32 a block's eight warps have a row each.  Bound: the logits' bytes (18,709 classes of 32
+// bits: 17 instructions a logit are three quarters of the time that its bytes take).
+template <typename T, int N, int E>
+__global__ void __launch_bounds__(N == 32 ? 256 : N) k_ctc_rows_reg(const CtcP p, const Step out, int K, int64_t rows) {
+    constexpr int WARPS = N / 32, PER = N == 32 ? 8 : 1, GOT = 512;
+    __shared__ struct {
+        Key lists[N];
+        Key got[GOT];
+        Key top[32];
+        Key cut;
+        float wm[WARPS], ws[WARPS];
+        int count;
+    } smem[PER];
+    const int part = N == 32 ? threadIdx.x >> 5 : 0, tid = N == 32 ? threadIdx.x & 31 : threadIdx.x;
+    auto &sm = smem[part];
+    auto sync = [] {
+        if (N == 32) __syncwarp();
+        else __syncthreads();
+    };
+    const int64_t r = (int64_t)blockIdx.x * PER + part;
+    if (r >= rows) return;
+    const int line = (int)(r / p.steps), t = (int)(r % p.steps);
+    if (p.lens && t >= p.lens[line]) return;
+    const int lane = tid & 31, warp = tid >> 5, n = p.classes;
+    const T *row = (const T *)p.logits + line * p.ln + t * p.lt;
+    float x[E];
+#pragma unroll
+    for (int k = 0; k < E; k++) x[k] = k * N + tid < n ? to_f(row[k * N + tid]) : -INFINITY;
+    if (tid == 0) sm.count = 0;
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        x[k] = on_step(x[k]);
+        m = fmaxf(m, x[k]);
+    }
+    // the blank is no candidate: it leaves the row, but for the sum
+    float xb = -INFINITY;
+    const bool mine = tid == p.blank % N;
+    if (mine) {
+#pragma unroll
+        for (int k = 0; k < E; k++)
+            if (k == p.blank / N) {
+                xb = x[k];
+                x[k] = -INFINITY;
+            }
+        out.blank[r] = xb;
+    }
+    float bv = x[0];
+    int bk = 0;
+#pragma unroll
+    for (int k = 1; k < E; k++)
+        if (x[k] > bv) bv = x[k], bk = k;
+    const Key best = bv > -INFINITY ? make_key(bv, bk * N + tid) : 0;
+    for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if (lane == 0) sm.wm[warp] = m;
+    const Key sorted = block_best32<WARPS>(best, sm.lists);
+    if (warp == 0) {
+        const Key cut = shfl(sorted, K - 1);
+        if (lane == 0) sm.cut = cut;
+        sm.top[lane] = 0;
+    }
+    sync();
+    const Key cut = sm.cut;
+    const float least = cut ? key_value(cut) : -INFINITY;
+    m = sm.wm[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) m = fmaxf(m, sm.wm[w]);
+    const float base = m > -INFINITY ? m : 0.f;
+    float s = exp2_of((xb - base) * kLog2e);
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        s += exp2_of((x[k] - base) * kLog2e);
+        if (x[k] >= least && x[k] > -INFINITY) {
+            const Key c = make_key(x[k], k * N + tid);
+            if (c >= cut) {
+                const int g = atomicAdd(&sm.count, 1);
+                if (g < GOT) sm.got[g] = c;
+            }
+        }
+    }
+    for (int d = 16; d; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (lane == 0) sm.ws[warp] = s;
+    sync();
+    const int got = sm.count;
+    if (got <= GOT) {
+        for (int g = tid; g < got; g += N) {
+            const Key c = sm.got[g];
+            int at = 0;
+            for (int o = 0; o < got; o++) at += sm.got[o] > c;
+            if (at < K) sm.top[at] = c;
+        }
+    } else {
+        Key last = ~0ull;
+        for (int q = 0; q < K; q++) {
+            Key next = 0;
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const Key c = x[k] > -INFINITY ? make_key(x[k], k * N + tid) : 0;
+                if (c < last && c > next) next = c;
+            }
+            for (int d = 16; d; d /= 2) next = max(next, shfl_xor(next, d));
+            if (lane == 0) sm.lists[warp] = next;
+            sync();
+            for (int w = 0; w < WARPS; w++) next = max(next, sm.lists[w]);
+            if (tid == 0) sm.top[q] = next;
+            last = next;
+            sync();
+        }
+    }
+    sync();
+    if (tid < K) {
+        const Key c = sm.top[tid];
+        out.val[r * K + tid] = c ? key_value(c) : -INFINITY;
+        out.cls[r * K + tid] = c ? (int)key_place(c) : -1;
+    }
+    if (tid == 0) {
+        double sum = 0;
+        for (int w = 0; w < WARPS; w++) sum += sm.ws[w];
+        out.lse[r] = m > -INFINITY ? m + log(sum) : -INFINITY;
+    }
+}
+
+template <typename T, int N, int E>
+void rows_reg(const CtcP &p, const Step &st, int K, int64_t rows, cudaStream_t s) {
+    const int per = N == 32 ? 8 : 1;
+    k_ctc_rows_reg<T, N, E><<<(unsigned)((rows + per - 1) / per), N == 32 ? 256 : N, 0, s>>>(p, st, K, rows);
+}
+
 template <typename T>
 void run(Ctx *c, const CtcP &p, const Step &st, uint32_t *back, cudaStream_t s) {
     const int K = p.width + 1;
     const int64_t rows = (int64_t)p.lines * p.steps;
     if (rows > 0) {
-        const size_t row = (size_t)p.classes * sizeof(T);
-        const int cached = sizeof(RowSmem) + row <= kSmemMax;
-        WOCR_CUDA(cudaFuncSetAttribute(k_ctc_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
-        k_ctc_rows<T><<<(unsigned)rows, kThreads, sizeof(RowSmem) + (cached ? row : 0), s>>>(p, st, K, cached);
+        if (p.classes <= 32 * 4) {
+            rows_reg<T, 32, 4>(p, st, K, rows, s);
+        } else if (p.classes <= 32 * 16) {
+            rows_reg<T, 32, 16>(p, st, K, rows, s);
+        } else if (p.classes <= 128 * 16) {
+            rows_reg<T, 128, 16>(p, st, K, rows, s);
+        } else if (p.classes <= 256 * 24) {
+            rows_reg<T, 256, 24>(p, st, K, rows, s);
+        } else if (p.classes <= 512 * 40) {
+            rows_reg<T, 512, 40>(p, st, K, rows, s);
+        } else {
+            const size_t row = (size_t)p.classes * sizeof(T);
+            const int cached = sizeof(RowSmem) + row <= kSmemMax;
+            WOCR_CUDA(cudaFuncSetAttribute(k_ctc_rows<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
+            k_ctc_rows<T><<<(unsigned)rows, kThreads, sizeof(RowSmem) + (cached ? row : 0), s>>>(p, st, K, cached);
+        }
         WOCR_LAUNCHED(c);
     }
-    k_ctc_search<T><<<p.lines, kSearch, 0, s>>>(p, st, back);
+    const int threads = std::max(64, (4 * candidates(p.width) + 31) / 32 * 32);  // two warps load ahead
+    WOCR_CUDA(cudaFuncSetAttribute(k_ctc_search<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SearchSmem)));
+    k_ctc_search<T><<<p.lines, threads, sizeof(SearchSmem), s>>>(p, st, back);
     WOCR_LAUNCHED(c);
 }
 }  // namespace

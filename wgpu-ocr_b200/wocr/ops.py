@@ -7,6 +7,7 @@ stay allocated until the stream has passed the call.
 """
 from __future__ import annotations
 
+import math
 import struct
 from typing import Optional, Sequence, Tuple
 
@@ -40,59 +41,51 @@ class DeviceArray:
     def stride(self) -> Tuple[int, ...]:
         return self._strides
 
+    def is_contiguous(self) -> bool:
+        n = 1
+        for d, s in zip(reversed(self.shape), reversed(self._strides)):
+            if d != 1 and s != n and 0 not in self.shape:
+                return False
+            n *= d
+        return True
+
     def get_device(self) -> int:
         return self.device
 
 
 def _code(x) -> int:
-    try:
-        return _codes[x.dtype]
-    except KeyError:
+    code = _codes.get(x.dtype)
+    if code is None:
         name = str(x.dtype).rsplit(".", 1)[-1]
         if name not in _NAMES:
             raise ValueError(f"element type {x.dtype} is not supported")
-        _codes[x.dtype] = _NAMES[name]
-        return _codes[x.dtype]
+        code = _codes[x.dtype] = _NAMES[name]
+    return code
 
 
-def _ptr(gpu, x, name: str) -> int:
-    if x.get_device() != gpu.device:
-        raise ValueError(f"{name} is not on device {gpu.device}")
-    return x.data_ptr()
+def _elsewhere(gpu, name: str):
+    return ValueError(f"{name} is not on device {gpu.device}")
 
 
 def _dense(gpu, x, name: str, code: int, shape) -> int:
-    """The address of a dense tensor of one type and shape (0 for None)."""
+    """The address of a dense tensor of one type and shape."""
     if x is None:
-        return 0
-    if _code(x) != code or tuple(x.shape) != shape:
-        raise ValueError(f"{name}: expected type {code} of shape {shape}, got {x.dtype} {tuple(x.shape)}")
-    n = 1
-    for d, s in zip(reversed(shape), reversed(x.stride())):
-        if d != 1 and s != n and 0 not in shape:
-            raise ValueError(f"{name} is not contiguous")
-        n *= d
-    return _ptr(gpu, x, name)
+        raise ValueError(f"{name} is missing")
+    if _code(x) != code or tuple(x.shape) != shape or not x.is_contiguous():
+        raise ValueError(f"{name}: expected type {code}, contiguous, of shape {shape}, got {x.dtype} {tuple(x.shape)}")
+    if x.get_device() != gpu.device:
+        raise _elsewhere(gpu, name)
+    return x.data_ptr()
 
 
-def _rows(gpu, x, name: str, code: int, shape) -> Tuple[int, int]:
-    """The address and row stride of a [rows, n] tensor whose rows are contiguous."""
-    if x is None:
-        return 0, 0
-    if _code(x) != code or tuple(x.shape) != shape:
-        raise ValueError(f"{name}: expected type {code} of shape {shape}, got {x.dtype} {tuple(x.shape)}")
+def _rows(gpu, x, name: str, shape) -> Tuple[int, int]:
+    """The address and row stride of an int32 [rows, n] tensor whose rows are contiguous."""
     s = x.stride()
-    if shape[1] > 1 and s[1] != 1:
-        raise ValueError(f"{name}: rows are not contiguous")
-    return _ptr(gpu, x, name), s[0]
-
-
-def _inner(x, name: str):
-    """The strides of a tensor whose last dimension is contiguous."""
-    s = x.stride()
-    if x.shape[-1] > 1 and s[-1] != 1:
-        raise ValueError(f"{name}: the last dimension is not contiguous")
-    return s
+    if _code(x) != I32 or tuple(x.shape) != shape or (shape[1] > 1 and s[1] != 1):
+        raise ValueError(f"{name}: expected int32 rows of shape {shape}, got {x.dtype} {tuple(x.shape)}, strides {s}")
+    if x.get_device() != gpu.device:
+        raise _elsewhere(gpu, name)
+    return x.data_ptr(), s[0]
 
 
 def _stream(stream) -> Optional[int]:
@@ -112,25 +105,36 @@ class DeviceOps:
         or below prefix[b]; with documents those whose id is its own, negative ids none.  scale None: dim ** -0.5.
         slopes float32 [heads]; prefix, q_lens, kv_lens int32 [batch]; q_docs [batch, queries], kv_docs [batch, keys]
         int32.  A query that sees nothing gets zeros; rows from q_lens[b] on are left as they were."""
+        t = q.dtype
         code = _code(q)
-        if _code(k) != code or _code(v) != code or _code(out) != code:
+        if (k.dtype != t and _code(k) != code) or (v.dtype != t and _code(v) != code) or (out.dtype != t and _code(out) != code):
             raise ValueError("q, k, v and out have different types")
         qs, ks = q.shape, k.shape
         if len(qs) != 4 or len(ks) != 4 or v.shape != ks or out.shape != qs or qs[0] != ks[0] or qs[3] != ks[3]:
             raise ValueError(f"attention shapes: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)}, out {tuple(out.shape)}")
         b, h, tq, d = qs
-        hk, tk = ks[1], ks[2]
-        a, c, e, f = _inner(q, "q"), _inner(k, "k"), _inner(v, "v"), _inner(out, "out")
-        qd, qds = (0, 0) if q_docs is None else _rows(self, q_docs, "q_docs", I32, (b, tq))
-        kd, kds = (0, 0) if kv_docs is None else _rows(self, kv_docs, "kv_docs", I32, (b, tk))
-        args = _ARGS.pack(_ptr(self, q, "q"), _ptr(self, k, "k"), _ptr(self, v, "v"), _ptr(self, out, "out"),
+        _, hk, tk, _ = ks
+        q0, q1, q2, qd = q.stride()
+        k0, k1, k2, kd = k.stride()
+        v0, v1, v2, vd = v.stride()
+        o0, o1, o2, od = out.stride()
+        if d > 1 and not qd == kd == vd == od == 1:
+            raise ValueError("attention: the last dimension is not contiguous")
+        dev = self.device
+        if not (q.get_device() == k.get_device() == v.get_device() == out.get_device() == dev):
+            raise _elsewhere(self, "q, k, v or out")
+        qi, qis = (0, 0) if q_docs is None else _rows(self, q_docs, "q_docs", (b, tq))
+        ki, kis = (0, 0) if kv_docs is None else _rows(self, kv_docs, "kv_docs", (b, tk))
+        args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                           0 if slopes is None else _dense(self, slopes, "slopes", F32, (h,)),
                           0 if prefix is None else _dense(self, prefix, "prefix", I32, (b,)),
                           0 if q_lens is None else _dense(self, q_lens, "q_lens", I32, (b,)),
-                          0 if kv_lens is None else _dense(self, kv_lens, "kv_lens", I32, (b,)), qd, kd,
-                          a[0], a[1], a[2], c[0], c[1], c[2], e[0], e[1], e[2], f[0], f[1], f[2], qds, kds,
+                          0 if kv_lens is None else _dense(self, kv_lens, "kv_lens", I32, (b,)),
+                          qi, ki, q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2, qis, kis,
                           code, b, h, hk, tq, tk, d, causal, d ** -0.5 if scale is None else scale, cap)
-        L.check(L.lib().wocr_attention(self.h, args, _stream(stream)))
+        st = L.lib().wocr_attention(self.h, args, _stream(stream))
+        if st:
+            L.check(st)
 
     def beam_select(self, logits, scores, out_scores, out_parents, out_tokens, end: int = -1, finished=None,
                     out_finished=None, stream: Optional[int] = None):
@@ -142,13 +146,20 @@ class DeviceOps:
             raise ValueError("logits [batch, beams, vocab] and out_scores [batch, beams] expected")
         b, n, v = logits.shape
         m = out_scores.shape[1]
-        s = _inner(logits, "logits")
-        L.check(L.lib().wocr_beam_select(
-            self.h, _ptr(self, logits, "logits"), _code(logits), b, n, v, s[0], s[1],
-            _dense(self, scores, "scores", F32, (b, n)), _dense(self, finished, "finished", U8, (b, n)) or None, end, m,
-            _dense(self, out_scores, "out_scores", F32, (b, m)), _dense(self, out_parents, "out_parents", I32, (b, m)),
-            _dense(self, out_tokens, "out_tokens", I32, (b, m)),
-            _dense(self, out_finished, "out_finished", U8, (b, m)) or None, _stream(stream)))
+        s0, s1, s2 = logits.stride()
+        if v > 1 and s2 != 1:
+            raise ValueError("logits: the last dimension is not contiguous")
+        if logits.get_device() != self.device:
+            raise _elsewhere(self, "logits")
+        inn, out = (b, n), (b, m)
+        st = L.lib().wocr_beam_select(
+            self.h, logits.data_ptr(), _code(logits), b, n, v, s0, s1, _dense(self, scores, "scores", F32, inn),
+            None if finished is None else _dense(self, finished, "finished", U8, inn), end, m,
+            _dense(self, out_scores, "out_scores", F32, out), _dense(self, out_parents, "out_parents", I32, out),
+            _dense(self, out_tokens, "out_tokens", I32, out),
+            None if out_finished is None else _dense(self, out_finished, "out_finished", U8, out), _stream(stream))
+        if st:
+            L.check(st)
 
     def beam_reorder(self, parents, states, axis: int = 0, live: Optional[int] = None, stream: Optional[int] = None):
         """The states of the chosen beams in their new order (`wocr_beam_reorder`): `parents` int32 [batch, out_beams] as
@@ -161,26 +172,26 @@ class DeviceOps:
         n, parts = None, []
         for src, dst in states:
             shape = tuple(src.shape)
-            size = _SIZES[_code(src)]
+            code = _code(src)
             if not 0 <= axis < len(shape):
                 raise ValueError(f"axis {axis} of a state of shape {shape}")
             rows = shape[0] // b if b else 1
-            if shape[0] != rows * b or tuple(dst.shape) != (b * m,) + shape[1:] or (n is not None and rows != n):
-                raise ValueError(f"state shapes {shape} and {tuple(dst.shape)} for {b} x {m} parents")
+            if shape[0] != rows * b or (n is not None and rows != n):
+                raise ValueError(f"a state of shape {shape} for {b} x {m} parents and {n} beams")
             n = rows
-            pieces, inner = 1, 1
-            for x in shape[1:axis]:
-                pieces *= x
-            for x in shape[max(axis, 0) + 1:]:
-                inner *= x
-            full = inner * size if axis == 0 else shape[axis] * inner * size
-            part = full if axis == 0 or live is None else live * inner * size
-            if axis and live is not None and not 0 <= live <= shape[axis]:
-                raise ValueError(f"live {live} of a state of shape {shape}")
-            parts.append(_STATE.pack(_dense(self, src, "state", _code(src), shape),
-                                     _dense(self, dst, "state", _code(src), tuple(dst.shape)), pieces, part, full, pieces * full))
-        L.check(L.lib().wocr_beam_reorder(self.h, _dense(self, parents, "parents", I32, (b, m)), b, n or 1, m, b"".join(parts),
-                                          len(parts), _stream(stream)))
+            full = _SIZES[code] * math.prod(shape[axis or 1:])  # bytes of a piece and of what of it is copied
+            part = full
+            if axis and live is not None:
+                if not 0 <= live <= shape[axis]:
+                    raise ValueError(f"live {live} of a state of shape {shape}")
+                part = full // max(shape[axis], 1) * live
+            pieces = math.prod(shape[1:axis])
+            parts.append(_STATE.pack(_dense(self, src, "state", code, shape), _dense(self, dst, "state", code, (b * m,) + shape[1:]),
+                                     pieces, part, full, pieces * full))
+        st = L.lib().wocr_beam_reorder(self.h, _dense(self, parents, "parents", I32, (b, m)), b, n or 1, m, b"".join(parts),
+                                       len(parts), _stream(stream))
+        if st:
+            L.check(st)
 
     def ctc_beam(self, logits, tokens, lengths, scores, lens=None, width: int = 8, blank: int = 0,
                  stream: Optional[int] = None):
@@ -192,8 +203,15 @@ class DeviceOps:
             raise ValueError("logits [lines, steps, classes] and tokens [lines, paths, steps] expected")
         n, t, v = logits.shape
         p = tokens.shape[1]
-        s = _inner(logits, "logits")
-        L.check(L.lib().wocr_ctc_beam(
-            self.h, _ptr(self, logits, "logits"), _code(logits), n, t, v, s[0], s[1],
-            _dense(self, lens, "lens", I32, (n,)) or None, width, blank, p, _dense(self, tokens, "tokens", I32, (n, p, t)),
-            _dense(self, lengths, "lengths", I32, (n, p)), _dense(self, scores, "scores", F32, (n, p)), _stream(stream)))
+        s0, s1, s2 = logits.stride()
+        if v > 1 and s2 != 1:
+            raise ValueError("logits: the last dimension is not contiguous")
+        if logits.get_device() != self.device:
+            raise _elsewhere(self, "logits")
+        st = L.lib().wocr_ctc_beam(
+            self.h, logits.data_ptr(), _code(logits), n, t, v, s0, s1,
+            None if lens is None else _dense(self, lens, "lens", I32, (n,)), width, blank, p,
+            _dense(self, tokens, "tokens", I32, (n, p, t)), _dense(self, lengths, "lengths", I32, (n, p)),
+            _dense(self, scores, "scores", F32, (n, p)), _stream(stream))
+        if st:
+            L.check(st)
