@@ -5,6 +5,7 @@
 //   last class again); a text reached both ways adds the masses up.  The best `width` go on.
 // The steps' log-sum-exps shift every beam alike: they enter the scores only.
 #include <algorithm>
+#include <climits>
 
 #include "elem.h"
 #include "ops.h"
@@ -207,18 +208,15 @@ struct Beams {
     float xl[32];                                // the step's logit of the last class
     int live;
 };
-// What orders a candidate: the log mass in steps, its bits made monotone, and its place.
-struct __align__(16) Order {
-    int64_t key;
-    uint32_t place, unused;
-};
-constexpr int64_t kNever = INT64_MIN;
+constexpr int64_t kNever = INT64_MIN;            // the key of what is no candidate
 
 struct SearchSmem {
     LogTable log;
     Beams beams[2];
-    Order order[(kMaxCand + 7) / 8 * 8];
-    double cb[kMaxCand], cn[kMaxCand], ct[32];
+    int64_t key[kMaxCand];                       // log masses in steps, their bits made monotone
+    uint32_t place[kMaxCand];
+    double cn[kMaxCand], cb[32], ct[32];
+    int floor;                                   // high word that a candidate's key needs
     uint8_t pi[kMaxCand], pk[kMaxCand];
     uint32_t kids[2][32];                        // beams that are a beam's text and a class more
     int parent[32];                              // and the beam that a text is one class more than, or -1
@@ -233,7 +231,8 @@ struct SearchSmem {
 // among the best: each pair before (i, k) in both orders is as good, but for one class that a beam
 // repeats, and where a pair grows into a held text, that text's own candidate is as good.  Candidates
 // in the order of their places: texts kept, then (beam, class); each one's rank is the number of
-// better ones, counted by four threads.
+// better ones, counted by four threads.  With all beams alive the least of the kept texts bounds the
+// candidates that are worth a count.
 // Bound: latency.  What a step reads is loaded a step ahead: its best classes, and its logits of every
 // class that a beam may then end in (the beams' last classes and the best classes of the step before),
 // which a prefetch into L2 has asked for a step earlier still.
@@ -243,13 +242,12 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
     SearchSmem &sm = *reinterpret_cast<SearchSmem *>(dyn);
     const int line = blockIdx.x, tid = threadIdx.x, N = blockDim.x, lane = tid & 31, warp = tid >> 5, W = p.width, K = W + 1;
     const int len = p.lens ? min(max(p.lens[line], 0), p.steps) : p.steps;
-    const int cand = candidates(W), slots = (cand + 7) / 8 * 8;
+    const int cand = candidates(W), loader = N / 32 - 2;
     const T *x0 = (const T *)p.logits + line * p.ln;
     const int64_t r0 = (int64_t)line * p.steps;
     uint32_t *bk = back + r0 * W;
     sm.log.fill(tid, N);
     if (tid < 64) sm.kids[tid >> 5][lane] = 0;
-    for (int u = tid; u < slots; u += N) sm.order[u] = {kNever, 0xffffffffu, 0};
     if (tid == 0) {
         int n = 2 * W;
         for (int i = 0; i < W; i++) {
@@ -285,15 +283,15 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
         float nv = 0.f, nb = 0.f;
         int nc = -1;
         const bool more = t + 1 < len;
-        if (more && warp < 2) {
-            const int c = warp == 0 ? (lane < n ? now.last[lane] : -1) : (lane < K ? sm.cls[cur][lane] : -1);
+        if (more && warp >= loader) {
+            const int c = warp == loader ? (lane < n ? now.last[lane] : -1) : (lane < K ? sm.cls[cur][lane] : -1);
             const T *row = x0 + (t + 1) * p.lt;
             if (c >= 0) nx = row[c];
-            if (warp == 1 && lane < K) {
+            if (warp > loader && lane < K) {
                 nv = st.val[(r + 1) * K + lane];
                 nc = st.cls[(r + 1) * K + lane];
             }
-            if (tid == 0) nb = st.blank[r + 1];
+            if (warp > loader) nb = st.blank[r + 1];
             if (t + 2 < len && c >= 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + p.lt + c));
         }
         // which beams are one class more than another: a warp per longer text, lanes are the shorter
@@ -310,64 +308,84 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
         }
         if (tid == N - 1) then.live = 0;
         __syncthreads();
-        const double xb = sm.blank[cur];
-        if (tid < cand) {
-            const int u = tid, i = sm.pi[u];
-            double b = -INFINITY, q = -INFINITY, total = -INFINITY;
-            uint32_t place = 0xffffffffu;
+        auto monotone = [](double mass) -> int64_t {
+            const int64_t bits = __double_as_longlong(rint(mass * (double)kStep) + 0.0);  // -0 as 0
+            return mass > -INFINITY ? bits ^ ((bits >> 63) & INT64_MAX) : kNever;
+        };
+        if (warp == 0) {  // texts kept
+            int64_t key = kNever;
+            if (lane < n) {
+                const int o = sm.parent[lane];
+                const double b = now.tot[lane] + sm.blank[cur];
+                double q = now.pn[lane] + now.xl[lane];
+                if (o >= 0) q = sm.log.add(q, (now.last[o] == now.last[lane] ? now.pb[o] : now.tot[o]) + now.xl[lane]);
+                const double total = sm.log.add(b, q);
+                sm.cb[lane] = b;
+                sm.cn[lane] = q;
+                sm.ct[lane] = total;
+                key = monotone(total);
+            }
+            if (lane < W) {
+                sm.key[lane] = key;
+                sm.place[lane] = lane;
+            }
+            const int least = __reduce_min_sync(0xffffffffu, lane < W ? (int)(key >> 32) : INT_MAX);
+            if (lane == 0) sm.floor = least;
+        } else if (W + tid - 32 < cand) {  // texts grown
+            const int u = W + tid - 32, i = sm.pi[u];
+            double q = -INFINITY;
             if (i < n) {
-                if (u < W) {
-                    const int o = sm.parent[i];
-                    b = now.tot[i] + xb;
-                    q = now.pn[i] + now.xl[i];
-                    if (o >= 0) q = sm.log.add(q, (now.last[o] == now.last[i] ? now.pb[o] : now.tot[o]) + now.xl[i]);
-                    sm.ct[i] = total = sm.log.add(b, q);
-                    place = i;
-                } else {
-                    const bool again = u < 2 * W;
-                    const int k = sm.pk[u], c = again ? now.last[i] : sm.cls[cur][k];
-                    if (c >= 0 && (again || c != now.last[i])) {
-                        bool held = false;
-                        for (uint32_t kids = sm.kids[cur][i]; kids; kids &= kids - 1) held |= now.last[__ffs(kids) - 1] == c;
-                        if (!held) {
-                            total = q = again ? now.pb[i] + now.xl[i] : now.tot[i] + sm.val[cur][k];
-                            place = W + (uint32_t)i * p.classes + c;
-                        }
-                    }
+                const bool again = u < 2 * W;
+                const int k = sm.pk[u], c = again ? now.last[i] : sm.cls[cur][k];
+                if (c >= 0 && (again || c != now.last[i])) {
+                    bool held = false;
+                    for (uint32_t kids = sm.kids[cur][i]; kids; kids &= kids - 1) held |= now.last[__ffs(kids) - 1] == c;
+                    if (!held) q = again ? now.pb[i] + now.xl[i] : now.tot[i] + sm.val[cur][k];
+                    sm.place[u] = W + (uint32_t)i * p.classes + c;
                 }
             }
-            sm.cb[u] = b;
             sm.cn[u] = q;
-            const int64_t bits = __double_as_longlong(rint(total * (double)kStep) + 0.0);  // -0 as 0
-            sm.order[u] = {total > -INFINITY ? bits ^ ((bits >> 63) & INT64_MAX) : kNever, place, 0};
+            sm.key[u] = monotone(q);
         }
-        if (tid < 32) sm.kids[cur ^ 1][tid] = 0;
-        if (more && warp < 2) {
-            sm.next[warp][lane] = on_step(to_f(nx));
-            if (warp == 1 && lane < K) {
-                sm.val[cur ^ 1][lane] = nv;
-                sm.cls[cur ^ 1][lane] = nc;
+        if (warp >= loader) {
+            sm.kids[cur ^ 1][lane] = 0;
+            if (more) {
+                sm.next[warp - loader][lane] = on_step(to_f(nx));
+                if (warp > loader) {
+                    if (lane < K) {
+                        sm.val[cur ^ 1][lane] = nv;
+                        sm.cls[cur ^ 1][lane] = nc;
+                    }
+                    if (lane == 0) sm.blank[cur ^ 1] = nb;
+                }
             }
-            if (tid == 0) sm.blank[cur ^ 1] = nb;
         }
         __syncthreads();
         {
             const int u = tid >> 2;
-            const Order mine = u < cand ? sm.order[u] : Order{kNever, 0, 0};
-            int rank = 0;
+            const int64_t key = u < cand ? sm.key[u] : kNever;
+            const bool near = key != kNever && (int)(key >> 32) >= sm.floor;
+            int rank = 0, same = 0;
+            if (near) {
 #pragma unroll 4
-            for (int o = tid & 3; o < slots; o += 4) {
-                const Order other = sm.order[o];
-                rank += other.key > mine.key || (other.key == mine.key && other.place < mine.place);
+                for (int o = tid & 3; o < cand; o += 4) {
+                    const int64_t other = sm.key[o];
+                    rank += other > key;
+                    same += other == key;
+                }
             }
+            same += __shfl_xor_sync(0xffffffffu, same, 1);
+            same += __shfl_xor_sync(0xffffffffu, same, 2);
+            if (same > 1)
+                for (int o = tid & 3; o < cand; o += 4) rank += sm.key[o] == key && sm.place[o] < sm.place[u];
             rank += __shfl_xor_sync(0xffffffffu, rank, 1);
             rank += __shfl_xor_sync(0xffffffffu, rank, 2);
-            if (mine.key != kNever && rank < W && (tid & 3) == 0) {
+            if (near && rank < W && (tid & 3) == 0) {
                 const bool kept = u < W, again = u < 2 * W;
                 const int i = sm.pi[u], k = sm.pk[u];
                 const int c = again ? now.last[i] : sm.cls[cur][k];
                 const double q = sm.cn[u];
-                then.pb[rank] = sm.cb[u];
+                then.pb[rank] = kept ? sm.cb[u] : -INFINITY;
                 then.pn[rank] = q;
                 then.tot[rank] = kept ? sm.ct[u] : q;
                 then.hash[rank] = kept ? now.hash[i] : grow(now.hash[i], c);
@@ -417,7 +435,7 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
 // With N = 32 a block's eight warps have a row each.  Bound: the logits' bytes (18,709 classes of 32
 // bits: 17 instructions a logit are three quarters of the time that its bytes take).
 template <typename T, int N, int E>
-__global__ void __launch_bounds__(N == 32 ? 256 : N) k_ctc_rows_reg(const CtcP p, const Step out, int K, int64_t rows) {
+__global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_rows_reg(const CtcP p, const Step out, int K, int64_t rows) {
     constexpr int WARPS = N / 32, PER = N == 32 ? 8 : 1, GOT = 512;
     __shared__ struct {
         Key lists[N];
@@ -439,27 +457,23 @@ __global__ void __launch_bounds__(N == 32 ? 256 : N) k_ctc_rows_reg(const CtcP p
     if (p.lens && t >= p.lens[line]) return;
     const int lane = tid & 31, warp = tid >> 5, n = p.classes;
     const T *row = (const T *)p.logits + line * p.ln + t * p.lt;
+    // the blank is no candidate: it stays out of the row, but for the sum
+    const float xb = tid == 0 ? on_step(to_f(row[p.blank])) : -INFINITY;
     float x[E];
 #pragma unroll
-    for (int k = 0; k < E; k++) x[k] = k * N + tid < n ? to_f(row[k * N + tid]) : -INFINITY;
-    if (tid == 0) sm.count = 0;
-    float m = -INFINITY;
+    for (int k = 0; k < E; k++) {
+        const int e = k * N + tid;
+        x[k] = e < n && e != p.blank ? to_f(row[e]) : -INFINITY;
+    }
+    if (tid == 0) {
+        sm.count = 0;
+        out.blank[r] = xb;
+    }
+    float m = xb;
 #pragma unroll
     for (int k = 0; k < E; k++) {
         x[k] = on_step(x[k]);
         m = fmaxf(m, x[k]);
-    }
-    // the blank is no candidate: it leaves the row, but for the sum
-    float xb = -INFINITY;
-    const bool mine = tid == p.blank % N;
-    if (mine) {
-#pragma unroll
-        for (int k = 0; k < E; k++)
-            if (k == p.blank / N) {
-                xb = x[k];
-                x[k] = -INFINITY;
-            }
-        out.blank[r] = xb;
     }
     float bv = x[0];
     int bk = 0;
@@ -509,9 +523,9 @@ __global__ void __launch_bounds__(N == 32 ? 256 : N) k_ctc_rows_reg(const CtcP p
         Key last = ~0ull;
         for (int q = 0; q < K; q++) {
             Key next = 0;
-#pragma unroll
-            for (int k = 0; k < E; k++) {
-                const Key c = x[k] > -INFINITY ? make_key(x[k], k * N + tid) : 0;
+            for (int e = tid; e < n; e += N) {  // from memory again: seldom, and the registers are full
+                const float v = on_step(to_f(row[e]));
+                const Key c = v > -INFINITY && e != p.blank ? make_key(v, e) : 0;
                 if (c < last && c > next) next = c;
             }
             for (int d = 16; d; d /= 2) next = max(next, shfl_xor(next, d));
@@ -565,7 +579,7 @@ void run(Ctx *c, const CtcP &p, const Step &st, uint32_t *back, cudaStream_t s) 
         }
         WOCR_LAUNCHED(c);
     }
-    const int threads = std::max(64, (4 * candidates(p.width) + 31) / 32 * 32);  // two warps load ahead
+    const int threads = std::max(96, (4 * candidates(p.width) + 31) / 32 * 32);  // a warp keeps, two load ahead
     WOCR_CUDA(cudaFuncSetAttribute(k_ctc_search<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SearchSmem)));
     k_ctc_search<T><<<p.lines, threads, sizeof(SearchSmem), s>>>(p, st, back);
     WOCR_LAUNCHED(c);
