@@ -199,6 +199,22 @@ int32_t wocr_ndgraph_run_argmax(wocr_ndgraph *g, const float *x, const int64_t *
                                 uint32_t *best, float *row_max, float *row_lse, int64_t cap,
                                 int64_t *rows_out, int64_t *out_shape, int32_t *out_rank);
 
+/* No counterpart in the reference.  Attention of the graph (MatMul of queries and transposed keys,
+ * Softmax over the keys, MatMul with the values, rank 4, each read by the next alone) as one kernel
+ * that does not store the weights: wocr_attention.  Off when a graph is created (unless
+ * WOCR_FUSED_ATTENTION is set), since sums then differ in their last bits; *found (nullable) gets the
+ * number of such places.  Waits for the context's stream. */
+int32_t wocr_ndgraph_fuse_attention(wocr_ndgraph *g, int32_t on, int32_t *found);
+
+/* No counterpart in the reference, which decodes greedily (Dictionary::decode).  NdGraph::run and a
+ * CTC prefix beam search over its output, logits [lines, steps, classes] (a graph made with
+ * stop_before_softmax), which stay on the device: wocr_ctc_beam.  lens (host, nullable): the steps of
+ * each line, n_lens of them.  Host outputs: tokens [lines][paths][steps] (cap entries), lengths and
+ * scores [lines][paths] (rows_cap entries); out_shape the logits' shape. */
+int32_t wocr_ndgraph_run_beam(wocr_ndgraph *g, const float *x, const int64_t *shape, int32_t rank, const int32_t *lens,
+                              int32_t n_lens, int32_t width, int32_t blank, int32_t paths, int32_t *tokens, int64_t cap,
+                              int32_t *lengths, float *scores, int64_t rows_cap, int64_t *out_shape, int32_t *out_rank);
+
 /* ---- record, then read in one wait --------------------------------------------------------
  * The reference records NdGraph::run / NdGraph::argmax_record (src/nd.rs:1372-1380) into one
  * command encoder and reads every recorded buffer with one Gpu::read_many (src/gpu.rs:1011-1037,

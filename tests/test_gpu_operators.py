@@ -569,3 +569,89 @@ def test_a_decoder_with_beams(gpu, type):
         p, k = par.cpu().numpy(), tok.cpu().numpy()
         assert (p == want[1]).all() and (k == want[2]).all()
         texts = [[texts[b][p[b, j]] + [int(k[b, j])] for j in range(K)] for b in range(B)]
+
+
+# ---- the graphs' own paths -----------------------------------------------------------------
+def _line_batch(seed, n, w):
+    return np.random.default_rng(seed).normal(size=(n, 3, 48, w)).astype(np.float32)
+
+
+@pytest.mark.parametrize("n, w", [(1, 8), (3, 64), (2, 320), (1, 1600)])
+def test_ndgraph_with_fused_attention(gpu, n, w):
+    """The recognition neck's two attentions as one kernel each: the same logits but for sums' last bits, captured too."""
+    from wocr import NdGraph, synth
+    g = NdGraph(gpu, synth.pp_rec_model(classes=211), stop_before_softmax=True)
+    x = _line_batch(w, n, w)
+    before = g.run(x)
+    assert g.fuse_attention() == 2
+    fused = [g.run(x) for _ in range(3)]
+    launches = g.stats()[1]
+    assert g.fuse_attention(False) == 2
+    plain = [g.run(x) for _ in range(3)]
+    assert g.stats()[1] >= launches + 4  # a softmax and a product fewer for each, and copies of k^T and v
+    for p in plain:
+        assert np.array_equal(p, before)
+    for f in fused:
+        assert np.array_equal(f, fused[0])
+        # scores off by a few 2^-24 of the attention's sums, through a block and a half of the neck
+        assert np.abs(f - before).max() <= 2.0 ** -17 * max(1.0, np.abs(before).max())
+    g.close()
+
+
+def _graph(nodes, weights=None, ints=None, inp="x", out="y"):
+    from wocr import Model, Node
+    return Model([Node(o, i, [n], a) for o, i, n, a in nodes], weights or {}, ints or {}, inp, out)
+
+
+def test_ndgraph_attention_of_other_shapes(gpu):
+    """What looks like attention but is not the kernel's: values of another width, a softmax that others read."""
+    from wocr import NdGraph
+    rng = np.random.default_rng(0)
+    x = rng.normal(size=(2, 3, 6, 10)).astype(np.float32)
+    wide = [("Transpose", ["x"], "kt", {"perm": [0, 1, 3, 2]}), ("MatMul", ["x", "kt"], "s", {}), ("Softmax", ["s"], "p", {"axis": -1}),
+            ("Concat", ["x", "x"], "v", {"axis": 3}), ("MatMul", ["p", "v"], "y", {})]
+    shared = [("Transpose", ["x"], "kt", {"perm": [0, 1, 3, 2]}), ("MatMul", ["x", "kt"], "s", {}), ("Softmax", ["s"], "p", {"axis": -1}),
+              ("MatMul", ["p", "x"], "o", {}), ("MatMul", ["p", "o"], "y", {})]
+    for nodes, found in ((wide, 1), (shared, 0)):
+        g = NdGraph(gpu, _graph(nodes))
+        before = g.run(x)
+        assert g.fuse_attention() == found
+        for _ in range(3):
+            assert np.array_equal(g.run(x), before)
+        g.close()
+    # and one with keys that are no transposed view
+    own = [("Relu", ["x"], "q", {}), ("Transpose", ["x"], "t", {"perm": [0, 1, 3, 2]}), ("Relu", ["t"], "kt", {}),
+           ("MatMul", ["q", "kt"], "s", {}), ("Softmax", ["s"], "p", {"axis": 3}), ("MatMul", ["p", "x"], "y", {})]
+    g = NdGraph(gpu, _graph(own))
+    before = g.run(x)
+    assert g.fuse_attention() == 1
+    for _ in range(3):
+        assert np.abs(g.run(x) - before).max() < 1e-5
+    g.close()
+
+
+def test_ndgraph_beam(gpu):
+    """The graph and the search in one call: the texts that the search finds in the graph's own logits."""
+    import wocr
+    from wocr import NdGraph, synth
+    g = NdGraph(gpu, synth.pp_rec_model(classes=97), stop_before_softmax=True)
+    for n, w, lens in ((2, 64, None), (3, 160, [20, 7, 0]), (2, 64, None), (2, 64, None)):
+        x = _line_batch(n + w, n, w) * 3
+        logits = g.run(x)
+        got = g.beam(x, width=6, paths=4, lens=lens)
+        want = ref.ctc_beam(torch.tensor(logits), lens, 6, 0, 4)
+        assert len(got) == n
+        for i in range(n):
+            live = int(np.isfinite(want[2][i]).sum())
+            assert len(got[i]) == live
+            for j, (text, score) in enumerate(got[i]):
+                assert list(text) == list(want[0][i, j, :want[1][i, j]])
+                assert abs(score - want[2][i, j]) <= 2.0 ** -24 * abs(want[2][i, j]) + logits.shape[1] * 2.0 ** -20
+        # a width of one and a peaked step leave the greedy text
+    assert wocr.beam_text([1, 2, 500], ["", "a", "b"]) == "ab"
+    for kw, code in ((dict(width=0), 2), (dict(width=32), 2), (dict(width=2, paths=3), 1), (dict(blank=97), 1), (dict(lens=[1]), 3)):
+        with pytest.raises(wocr.WocrError) as e:
+            g.beam(x, **kw)
+        assert e.value.code == code
+    assert len(g.beam(x)) == 2  # and works on
+    g.close()

@@ -7,6 +7,7 @@
 #include <thread>
 
 #include "exec.h"
+#include "ops.h"
 #include "layout.h"
 
 using namespace wocr;
@@ -1472,6 +1473,70 @@ int32_t wocr_ndgraph_run_argmax(wocr_ndgraph *g, const float *x, const int64_t *
                        [&](void *dst, const void *src, size_t bytes) {
                            if (dst) d2h(c, dst, src, bytes);
                        });
+        sync_bounded(c, 0);
+    });
+}
+
+int32_t wocr_ndgraph_fuse_attention(wocr_ndgraph *g, int32_t on, int32_t *found) {
+    return guard([&] {
+        if (!g) fail(WOCR_ERR_INVALID, "null graph");
+        WOCR_CUDA(cudaSetDevice(g->ctx->c.device));
+        wait_stream(&g->ctx->c);
+        for (auto &r : g->replays) r.reset();  // captured with the setting before
+        g->graph->fuse_attention = on != 0;
+        if (found) *found = (int32_t)g->graph->attn.size();
+    });
+}
+
+int32_t wocr_ndgraph_run_beam(wocr_ndgraph *g, const float *x, const int64_t *shape, int32_t rank, const int32_t *lens,
+                              int32_t n_lens, int32_t width, int32_t blank, int32_t paths, int32_t *tokens, int64_t cap,
+                              int32_t *lengths, float *scores, int64_t rows_cap, int64_t *out_shape, int32_t *out_rank) {
+    return guard([&] {
+        if (width < 1 || width > k::kMaxWidth)
+            fail(WOCR_ERR_UNSUPPORTED, "beam width " + std::to_string(width) + " (1 to " + std::to_string(k::kMaxWidth) + " are supported)");
+        if (paths < 1 || paths > width) fail(WOCR_ERR_INVALID, "1 to width paths");
+        if (!tokens || !lengths || !scores || !out_shape || !out_rank) fail(WOCR_ERR_INVALID, "null argument");
+        if (!g) fail(WOCR_ERR_INVALID, "null graph");
+        Ctx *c = &g->ctx->c;
+        RunScope rs(c, &g->last);
+        // the logits stay on the device: the search reads them where the graph left them
+        nd_run_core(g, x, shape, rank, (float *)tokens, INT64_MAX, out_shape, out_rank,
+                    [&](void *, const void *logits, size_t) {
+                        if (*out_rank != 3) fail(WOCR_ERR_SHAPE, "beam search needs logits [lines, steps, classes]");
+                        const int64_t n = out_shape[0], t = out_shape[1], v = out_shape[2];
+                        if (n > INT32_MAX || t > INT32_MAX || n * t > INT32_MAX || v > (1 << 27) - 2)
+                            fail(WOCR_ERR_UNSUPPORTED, "beam search: too many steps or classes");
+                        if (blank < 0 || blank >= v) fail(WOCR_ERR_INVALID, "the blank is not one of the classes");
+                        if (lens && n_lens != n) fail(WOCR_ERR_SHAPE, std::to_string(n_lens) + " lengths for " + std::to_string(n) + " lines");
+                        if (cap < n * paths * t || rows_cap < n * paths) fail(WOCR_ERR_CAPACITY, "beam output buffers too small");
+                        if (n == 0) return;
+                        BufP tk = alloc(c, (size_t)std::max<int64_t>(n * paths * t, 1) * 4), ln = alloc(c, (size_t)n * paths * 4),
+                             sc = alloc(c, (size_t)n * paths * 4), ls;
+                        k::CtcP p;
+                        p.logits = logits;
+                        p.ln = t * v;
+                        p.lt = v;
+                        p.lens = nullptr;
+                        if (lens) {
+                            ls = alloc(c, (size_t)n * 4);
+                            WOCR_CUDA(cudaMemcpyAsync(ls->p, lens, (size_t)n * 4, cudaMemcpyHostToDevice, c->stream));
+                            p.lens = (const int *)ls->p;
+                        }
+                        p.tokens = (int *)tk->p;
+                        p.lengths = (int *)ln->p;
+                        p.scores = (float *)sc->p;
+                        p.type = WOCR_F32;
+                        p.lines = (int)n;
+                        p.steps = (int)t;
+                        p.classes = (int)v;
+                        p.width = width;
+                        p.paths = paths;
+                        p.blank = blank;
+                        k::ctc_beam(c, p, c->stream);
+                        if (t > 0) d2h(c, tokens, tk->p, (size_t)(n * paths * t) * 4);
+                        d2h(c, lengths, ln->p, (size_t)(n * paths) * 4);
+                        d2h(c, scores, sc->p, (size_t)(n * paths) * 4);
+                    });
         sync_bounded(c, 0);
     });
 }

@@ -1,6 +1,8 @@
 // The two graph executors of the reference, lowered to the sm_100a kernels.
 #include "exec.h"
 
+#include "ops.h"
+
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
@@ -930,12 +932,27 @@ DT Executor::run_to(const DT &x, int upto) {
     Value in;
     in.f = x;
     vals[input] = in;
-    for (int i = 0; i < upto; i++) {
-        exec_step(steps[i], vals);
-        for (auto &n : steps[i].inputs) {
-            auto lu = last_use.find(n);
-            if (lu != last_use.end() && lu->second == i && n != output && n != input) vals.erase(n);
+    const auto &uses = fuse_attention ? fused_use : last_use;
+    auto drop = [&](int step, int i) {  // the inputs of `step` that nothing reads after i
+        for (auto &n : steps[step].inputs) {
+            auto lu = uses.find(n);
+            if (lu != uses.end() && lu->second == i && n != output && n != input) vals.erase(n);
         }
+    };
+    for (int i = 0; i < upto; i++) {
+        const Attn *at = nullptr;
+        if (fuse_attention)
+            for (auto &a : attn)
+                if (a.out < upto && (i == a.scores || i == a.softmax || i == a.out)) at = &a;
+        if (at) {
+            if (i != at->out) continue;  // its inputs live until then
+            run_attention(*at, vals);
+            drop(at->scores, i);
+            drop(at->softmax, i);
+        } else {
+            exec_step(steps[i], vals);
+        }
+        drop(i, i);
     }
     // the whole graph: its output; a prefix: the first input of step `upto`
     const std::string &want = upto == (int)steps.size() ? output : steps[upto].inputs[0];
@@ -943,6 +960,83 @@ DT Executor::run_to(const DT &x, int upto) {
     if (it == vals.end()) fail(WOCR_ERR_MISSING, "value " + want + " not computed");
     if (it->second.is_int) fail(WOCR_ERR_SHAPE, "value " + want + " is not float");
     return to_f32(ctx, it->second.f);
+}
+
+// Chains of three generic steps that are an attention (steps and last_use are final).
+void Executor::find_attention() {
+    attn.clear();
+    fused_use = last_use;
+    std::map<std::string, int> readers, reader;
+    for (int i = 0; i < (int)steps.size(); i++)
+        for (auto &n : steps[i].inputs) {
+            readers[n]++;
+            reader[n] = i;
+        }
+    auto generic = [&](int i, const char *op) { return steps[i].kind == Step::N_GENERIC && model.nodes[steps[i].node].op == op; };
+    auto only = [&](int i) { return readers[steps[i].output] == 1 && steps[i].output != output ? reader[steps[i].output] : -1; };
+    for (int i = 0; i < (int)steps.size(); i++) {
+        if (!generic(i, "MatMul")) continue;
+        const int sm = only(i);
+        if (sm < 0 || !generic(sm, "Softmax")) continue;
+        const int64_t axis = model.nodes[steps[sm].node].int_("axis").value_or(-1);
+        const int av = only(sm);
+        if ((axis != -1 && axis != 3) || av < 0 || !generic(av, "MatMul")) continue;
+        const Step &a = steps[i], &o = steps[av];
+        if (o.inputs.size() != 2 || o.inputs[0] != steps[sm].output || a.inputs.size() != 2) continue;
+        attn.push_back({i, sm, av});
+        // run as one, the queries and keys are read at the last step
+        for (auto &n : a.inputs) fused_use[n] = std::max(fused_use[n], av);
+    }
+}
+
+void Executor::run_attention(const Attn &a, std::map<std::string, Value> &vals) {
+    DT q = getf(vals, steps[a.scores].inputs[0]), kt = getf(vals, steps[a.scores].inputs[1]),
+       v = getf(vals, steps[a.out].inputs[1]);
+    bool ok = q.rank() == 4 && kt.rank() == 4 && v.rank() == 4 && q.shape[3] == kt.shape[2] && kt.shape[3] == v.shape[2] &&
+              v.shape[3] == q.shape[3] && q.shape[3] >= 1 && q.shape[3] <= 256 && q.numel() > 0 && v.numel() > 0;
+    for (int d = 0; ok && d < 2; d++) ok = q.shape[d] == kt.shape[d] && q.shape[d] == v.shape[d];
+    if (!ok) {  // other shapes: the three steps as they are
+        exec_step(steps[a.scores], vals);
+        exec_step(steps[a.softmax], vals);
+        exec_step(steps[a.out], vals);
+        return;
+    }
+    // the kernel wants the dimension within a head contiguous; k^T usually is such a view of k
+    DT k = kt;
+    std::swap(k.shape[2], k.shape[3]);
+    std::swap(k.strides[2], k.strides[3]);
+    auto dense = [&](const DT &t) {
+        bool pos = t.shape[3] == 1 || t.strides[3] == 1;
+        for (auto st : t.strides) pos = pos && st >= 0;
+        return pos ? t : to_rowmajor(ctx, t);
+    };
+    q = dense(q);
+    k = dense(k);
+    v = dense(v);
+    DT y = new_rowmajor(ctx, q.shape);
+    k::AttnP p = {};
+    p.q = q.p;
+    p.k = k.p;
+    p.v = v.p;
+    p.o = y.p;
+    for (int d = 0; d < 3; d++) {
+        p.qs[d] = q.strides[d];
+        p.ks[d] = k.strides[d];
+        p.vs[d] = v.strides[d];
+        p.os[d] = y.strides[d];
+    }
+    p.type = WOCR_F32;
+    p.batch = (int)q.shape[0];
+    p.heads = p.kv_heads = (int)q.shape[1];
+    p.q_len = (int)q.shape[2];
+    p.kv_len = (int)k.shape[2];
+    p.dim = (int)q.shape[3];
+    p.scale = 1.f;  // the graph's own scale is in q or k
+    k::attention(ctx, p, ctx->stream);
+    ctx->flops += 4.0 * q.numel() * k.shape[2];
+    Value out;
+    out.f = y;
+    vals[steps[a.out].output] = out;
 }
 
 bool Executor::ends_in_linear() const {
@@ -2032,6 +2126,8 @@ std::unique_ptr<Executor> build_ndgraph(Ctx *c, const Model &m, bool stop_before
     ex->input = m.input;
     ex->output = output;
     ex->finalize();
+    ex->find_attention();
+    ex->fuse_attention = std::getenv("WOCR_FUSED_ATTENTION") != nullptr;
     return ex;
 }
 

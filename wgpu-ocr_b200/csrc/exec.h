@@ -115,6 +115,15 @@ class Executor {
     // Values between the convolutional steps of a Graph may be stored split (bf16 hi | lo, as
     // the tap convolution reads them); plan_split() marks the steps whose output is.
     bool allow_split = false;
+    // Attention of an N-D graph: MatMul(q, k^T), Softmax over the keys, MatMul(weights, v), each read
+    // by the next alone (step indices).  With fuse_attention the three run as one kernel that never
+    // stores the weights, where it takes the shapes; off by default: the sums differ in their last bits.
+    struct Attn {
+        int scores, softmax, out;
+    };
+    std::vector<Attn> attn;
+    std::map<std::string, int> fused_use;  // last_use when they are fused
+    bool fuse_attention = false;
 
     explicit Executor(Ctx *c) : ctx(c) {}
     // Run on `x`; returns the output tensor.
@@ -126,8 +135,10 @@ class Executor {
     // That linear layer on x (its input) with the row arg-max fused; returns the logits' shape.
     std::vector<int64_t> linear_argmax(const DT &x, uint32_t *best, float *row_max, float *row_lse);
     void finalize();  // uploads generic weights, computes last uses
+    void find_attention();
 
   protected:
+    void run_attention(const Attn &a, std::map<std::string, Value> &vals);
     void plan_split();
     DT slot_output(const std::string &name, int64_t n, int64_t c, int64_t h, int64_t w, bool split);
     DT concat_channels(const std::vector<DT> &parts, const std::string &out_name, bool split);

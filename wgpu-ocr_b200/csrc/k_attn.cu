@@ -593,6 +593,9 @@ void launch_type(Ctx *c, const AttnP &p, cudaStream_t s) {
 }  // namespace
 
 void attention(Ctx *c, const AttnP &p, cudaStream_t s) {
+    const double rows = (double)p.batch * p.heads * p.q_len;
+    OpProf pf(c, s, "attention", 4.0 * rows * p.kv_len * p.dim,
+              elem_size(p.type) * (double)p.dim * (2.0 * rows + 2.0 * p.batch * p.kv_heads * p.kv_len));
     if (p.q_len >= 128 && attention_tc_ok(p)) return attention_tc(c, p, s);
     if (p.type == WOCR_F32) launch_type<float>(c, p, s);
     else if (p.type == WOCR_F16) launch_type<__half>(c, p, s);

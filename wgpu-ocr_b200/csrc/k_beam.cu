@@ -267,6 +267,7 @@ void select_t(Ctx *c, const BeamP &p, cudaStream_t s) {
 
 void beam_select(Ctx *c, const BeamP &p, cudaStream_t s) {
     if (p.batch == 0) return;
+    OpProf pf(c, s, "beam_select", 0, (double)p.batch * p.kin * p.vocab * elem_size(p.type));
     if (p.type == WOCR_F32) select_t<float>(c, p, s);
     else if (p.type == WOCR_F16) select_t<__half>(c, p, s);
     else select_t<__nv_bfloat16>(c, p, s);
@@ -276,6 +277,9 @@ void beam_reorder(Ctx *c, const int *parents, int batch, int kin, int kout, cons
                   cudaStream_t s) {
     if (batch == 0) return;
     const int rows = batch * kout;
+    double bytes = 0;
+    for (int i = 0; i < n; i++) bytes += 2.0 * rows * st[i].pieces * st[i].bytes;
+    OpProf pf(c, s, "beam_reorder", 0, bytes);
     for (int i = 0; i < n;) {
         ReorderArgs a;
         a.parents = parents;

@@ -588,6 +588,7 @@ void run(Ctx *c, const CtcP &p, const Step &st, uint32_t *back, cudaStream_t s) 
 
 void ctc_beam(Ctx *c, const CtcP &p, cudaStream_t s) {
     if (p.lines == 0) return;
+    OpProf pf(c, s, "ctc_beam", 0, (double)p.lines * p.steps * p.classes * elem_size(p.type));
     // workspace of this call alone, ordered on the call's stream (a graph that captures the call
     // gets its own)
     const size_t rows = std::max<size_t>((size_t)p.lines * p.steps, 1), K = p.width + 1;

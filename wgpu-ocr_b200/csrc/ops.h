@@ -3,10 +3,21 @@
 // (ops.cpp) have checked every argument.
 #pragma once
 
+#include <optional>
+
 #include "common.h"
 
 namespace wocr {
 namespace k {
+
+// Brackets an operator with events when the context profiles, on the context's own stream only (a
+// caller's stream may be capturing, and is not waited for by the profile's report).
+struct OpProf {
+    std::optional<Prof> prof;
+    OpProf(Ctx *c, cudaStream_t s, const char *name, double flops, double bytes) {
+        if (c->prof && s == c->stream) prof.emplace(c, name, flops, bytes);
+    }
+};
 
 // Softmax attention (wocr_attention in wocr.h): sizes, element strides (batch, head, token; the
 // dimension within a head is contiguous) and masks.

@@ -133,6 +133,9 @@ _SIGS = [
                                 c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
     ("wocr_pp_lines", c_i32, [c_void_p, c_void_p, c_i32, c_i32, c_void_p, c_i32, c_i32, c_void_p, c_i64, c_void_p,
                               c_void_p, c_void_p, P(c_i32), P(c_i64)]),
+    ("wocr_ndgraph_fuse_attention", c_i32, [c_void_p, c_i32, P(c_i32)]),
+    ("wocr_ndgraph_run_beam", c_i32, [c_void_p, c_void_p, P(c_i64), c_i32, c_void_p, c_i32, c_i32, c_i32, c_i32, c_void_p,
+                                      c_i64, c_void_p, c_void_p, c_i64, P(c_i64), P(c_i32)]),
     ("wocr_attention", c_i32, [c_void_p, c_char_p, c_void_p]),
     ("wocr_beam_select", c_i32, [c_void_p, c_void_p, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_void_p, c_void_p, c_i32,
                                  c_i32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),

@@ -397,6 +397,42 @@ class NdGraph(_Handle):
             shape = tuple(oshape[i] for i in range(orank.value))
             return best[:r], mx[:r], (ls[:r] if lse else None), shape
 
+    def fuse_attention(self, on: bool = True) -> int:
+        """Run the graph's attention (MatMul, Softmax, MatMul) as one kernel each, without storing its
+        weights; off by default, as the sums differ in their last bits.  Returns how many there are."""
+        n = ctypes.c_int32()
+        L.check(L.lib().wocr_ndgraph_fuse_attention(self.h, int(bool(on)), ctypes.byref(n)))
+        return n.value
+
+    def beam(self, x: np.ndarray, width: int = 8, paths: int = 1, blank: int = 0, lens=None):
+        """run + CTC prefix beam search on the device (`wocr_ndgraph_run_beam`), for a graph that ends
+        in logits [lines, steps, classes] (stop_before_softmax).  lens: each line's steps (None: all).
+        Returns per line its best texts, [(classes int32, log mass)], best first; `beam_text` spells
+        one.  The reference decodes greedily (src/ppocr.rs:23-33)."""
+        x = np.ascontiguousarray(x, np.float32)
+        shp = (ctypes.c_int64 * x.ndim)(*x.shape)
+        ln = None if lens is None else np.ascontiguousarray(lens, np.int32)
+        oshape = (ctypes.c_int64 * 6)()
+        orank = ctypes.c_int32()
+        # a line's steps are at most its columns: enough in one go for images [lines, 3, 48, width]
+        cap, rows = max(x.shape[0] * x.shape[-1], 1) * paths, max(x.shape[0], 1) * paths
+        while True:
+            tokens, lengths = np.empty(cap, np.int32), np.empty(rows, np.int32)
+            scores = np.empty(rows, np.float32)
+            st = L.lib().wocr_ndgraph_run_beam(self.h, L.ptr(x), shp, x.ndim, None if ln is None else L.ptr(ln),
+                                               0 if ln is None else ln.size, int(width), int(blank), int(paths),
+                                               L.ptr(tokens), cap, L.ptr(lengths), L.ptr(scores), rows, oshape,
+                                               ctypes.byref(orank))
+            n, t = (oshape[0], oshape[1]) if orank.value == 3 else (0, 0)
+            if st == 8 and (n * t * paths > cap or n * paths > rows):
+                cap, rows = max(n * t * paths, 1), max(n * paths, 1)
+                continue
+            L.check(st)
+            break
+        tokens = tokens[:n * paths * t].reshape(n, paths, t)
+        return [[(tokens[i, j, :lengths[i * paths + j]].copy(), float(scores[i * paths + j])) for j in range(paths)
+                 if scores[i * paths + j] > -np.inf] for i in range(n)]
+
     def argmax_enqueue(self, batch: "Batch", x: np.ndarray) -> "Pending":
         """NdGraph::run + argmax_record (src/nd.rs:1372-1380): queued on the device, read by
         `batch.wait()`.  Returns a `Pending` whose best / row_max / row_lse ([rows]) and shape
@@ -755,3 +791,9 @@ def pp_decode(best: Sequence[int], chars: List[str]) -> str:
             out.append(chars[c] if c < len(chars) else "")
         prev = c
     return "".join(out)
+
+
+def beam_text(classes: Sequence[int], chars: List[str]) -> str:
+    """The text of a beam search's classes (repeats are already merged, blanks gone), spelt as
+    `pp_decode` spells them."""
+    return "".join(chars[int(c)] if int(c) < len(chars) else "" for c in classes)
