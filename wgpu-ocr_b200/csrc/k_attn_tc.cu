@@ -98,6 +98,48 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t at, const float (&f)[32]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+#pragma unroll
+        for (int x = 0; x < 16; x++) r[x] = __float_as_uint(f[y * 16 + x]);
+        tmem_st16(at + y * 16, r);
+    }
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// the greatest of 32 values and t, in four chains
+__device__ __forceinline__ float max32(const float (&f)[32], float t) {
+    float a[4] = {t, f[0], f[1], f[2]};
+#pragma unroll
+    for (int x = 3; x + 1 < 32; x += 2) a[(x >> 1) & 3] = max3(a[(x >> 1) & 3], f[x], f[x + 1]);
+    return fmaxf(max3(a[0], a[1], a[2]), fmaxf(a[3], f[31]));
+}
+__device__ constexpr float kTanh[6] = {1.f, -0.333332121f, 0.133305937f, -0.0536993034f, 0.0205612238f, -0.00565812876f};
+// cap tanh(scale f / cap) in units of log 2.  |y| < 0.6, the rule for capped scores, takes y times a
+// polynomial in y^2 (least squares in Chebyshev points, within 2^-24 of tanh); a warp with a larger
+// one takes the exponential and the quotient.
+template <typename T>
+__device__ __forceinline__ void cap32(float (&f)[32], float scale, float cap) {
+    const float to_y = scale / cap, to_s = scale * kLog2e;
+    float a = 0.f;
+#pragma unroll
+    for (int x = 0; x < 32; x += 2) a = max3(a, fabsf(f[x]), fabsf(f[x + 1]));
+    if (__any_sync(0xffffffffu, !(a * fabsf(to_y) < 0.6f))) {
+#pragma unroll
+        for (int x = 0; x < 32; x++) f[x] = capped2<T>(f[x] * scale, cap);
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < 32; x++) {
+        const float y = f[x] * to_y, t = y * y;
+        f[x] = f[x] * to_s * fmaf(fmaf(fmaf(fmaf(fmaf(kTanh[5], t, kTanh[4]), t, kTanh[3]), t, kTanh[2]), t, kTanh[1]), t, kTanh[0]);
+    }
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename T, int DP>
@@ -328,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = row && (!p.q_docs || doc >= 0);
         const int end = live ? key_end(p, sp, i) : 0, pos = sp.off + i;
         const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.f, scale2 = p.scale * kLog2e;
+        const bool special = p.cap > 0.f || p.slopes || !(scale2 > 0.f);
         int *dk = docs + warp * 128;
         float m = -INFINITY, l = 0.f;
         int n = 0;
@@ -345,44 +388,57 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = warp_wait(&s_full[my], n & 1, ta.status, stop, 48, ta.budget);
             if (!ok) break;
             tc_fence_after();
-            float f[128];
+            // First pass: the maximum.  What is not a plain product (capped, biased, masked) is worked
+            // out here and stored back, so that the second pass is the same for every tile.
+            float top = -INFINITY, mul = scale2;
+            if (plain && !special) {
+                float f[2][32];
+                tmem_ld32(ts, f[0]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32(ts + c * 32, f + c * 32);
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_wait32(f + c * 32);
-            float mul = scale2;
-            if (p.cap > 0.f) {
+                for (int c = 0; c < 4; c++) {
+                    tmem_wait32(f[c & 1]);
+                    if (c < 3) tmem_ld32(ts + (c + 1) * 32, f[(c + 1) & 1]);
+                    top = max32(f[c & 1], top);
+                }
+                top *= mul;
+            } else {
                 mul = 1.f;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    float f[32];
+                    tmem_ld32(ts + c * 32, f);
+                    tmem_wait32(f);
+                    const int jc = j0 + c * 32;
+                    if (p.cap > 0.f) cap32<T>(f, p.scale, p.cap);
+                    else
 #pragma unroll
-                for (int x = 0; x < 128; x++) f[x] = capped2<T>(f[x] * p.scale, p.cap);
-            } else if (p.slopes || !(scale2 > 0.f)) {
-                mul = 1.f;
+                        for (int x = 0; x < 32; x++) f[x] *= scale2;
+                    if (p.slopes) {
+                        const float far = (float)(pos - jc);
 #pragma unroll
-                for (int x = 0; x < 128; x++) f[x] *= scale2;
-            }
-            if (p.slopes) {
-                const float far = (float)(pos - j0);
-#pragma unroll
-                for (int x = 0; x < 128; x++) f[x] = fmaf(-slope, fabsf(far - (float)x), f[x]);
-            }
-            if (!plain) {
-#pragma unroll
-                for (int x = 0; x < 128; x++)
-                    if (j0 + x >= end) f[x] = -INFINITY;
-                if (p.q_docs)
-#pragma unroll
-                    for (int x = 0; x < 128; x += 4) {
-                        const int4 d = *(const int4 *)(dk + x);
-                        if (d.x != doc) f[x] = -INFINITY;
-                        if (d.y != doc) f[x + 1] = -INFINITY;
-                        if (d.z != doc) f[x + 2] = -INFINITY;
-                        if (d.w != doc) f[x + 3] = -INFINITY;
+                        for (int x = 0; x < 32; x++) f[x] = fmaf(-slope, fabsf(far - (float)x), f[x]);
                     }
-            }
-            float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (!plain) {
+                        const int left = end - jc;
 #pragma unroll
-            for (int x = 0; x < 128; x++) a[x & 3] = fmaxf(a[x & 3], f[x]);
-            const float top = fmaxf(m, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * mul);
+                        for (int x = 0; x < 32; x++)
+                            if (x >= left) f[x] = -INFINITY;
+                        if (p.q_docs)
+#pragma unroll
+                            for (int x = 0; x < 32; x += 4) {
+                                const int4 d = *(const int4 *)(dk + c * 32 + x);
+                                if (d.x != doc) f[x] = -INFINITY;
+                                if (d.y != doc) f[x + 1] = -INFINITY;
+                                if (d.z != doc) f[x + 2] = -INFINITY;
+                                if (d.w != doc) f[x + 3] = -INFINITY;
+                            }
+                    }
+                    top = max32(f, top);
+                    tmem_st32(ts + c * 32, f);
+                }
+                tmem_st_wait();
+            }
+            top = fmaxf(m, top);
             if (m == -INFINITY) m = top;  // nothing seen so far: nothing to rescale
             const bool grown = m > -INFINITY && top - m > kSlack;
             if (__any_sync(0xffffffffu, grown) && n > 0) {
@@ -390,36 +446,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float c = grown ? ex2(m - top) : 1.f;
                 if (grown) m = top;
                 l *= c;
-#pragma unroll
-                for (int c0 = 0; c0 < DP; c0 += 32) {
-                    if (c0 >= p.dim) break;
+#pragma unroll 1
+                for (int c0 = 0; c0 < p.dim; c0 += 32) {
                     float o[32];
-                    uint32_t w[16];
                     tmem_ld32(to + c0, o);
                     tmem_wait32(o);
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-#pragma unroll
-                        for (int x = 0; x < 16; x++) w[x] = __float_as_uint(o[y * 16 + x] * c);
-                        tmem_st16(to + c0 + y * 16, w);
-                    }
+                    for (int x = 0; x < 32; x++) o[x] *= c;
+                    tmem_st32(to + c0, o);
                 }
             }
+            // Second pass: weights, their sum, and the weights as 16-bit operands over the scores
+            // that have been read (16 columns behind 32).
             const float base = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 mul2 = make_float2(mul, mul), off2 = make_float2(-base, -base);
+            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+            {
+                float f[2][32];
+                tmem_ld32(ts, f[0]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t w[16];
+                for (int c = 0; c < 4; c++) {
+                    tmem_wait32(f[c & 1]);
+                    if (c < 3) tmem_ld32(ts + (c + 1) * 32, f[(c + 1) & 1]);
+                    uint32_t w[16];
 #pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const float u = ex2(fmaf(f[c * 32 + 2 * x], mul, -base)), v = ex2(fmaf(f[c * 32 + 2 * x + 1], mul, -base));
-                    sum[(2 * x) & 3] += u;
-                    sum[(2 * x + 1) & 3] += v;
-                    w[x] = pack2<T>(u, v);  // the one rounding of a weight: the matrix instruction takes 16 bits
+                    for (int x = 0; x < 16; x++) {
+                        float2 e = __ffma2_rn(make_float2(f[c & 1][2 * x], f[c & 1][2 * x + 1]), mul2, off2);
+                        e.x = ex2(e.x);
+                        e.y = ex2(e.y);
+                        if (x & 1) sum1 = __fadd2_rn(sum1, e);
+                        else sum0 = __fadd2_rn(sum0, e);
+                        w[x] = pack2<T>(e.x, e.y);  // the one rounding of a weight: the matrix instruction takes 16 bits
+                    }
+                    tmem_st16(ts + c * 16, w);
                 }
-                tmem_st16(ts + c * 16, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            sum0 = __fadd2_rn(sum0, sum1);
+            l += sum0.x + sum0.y;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
