@@ -9,6 +9,7 @@
 //   warp 8          (one thread) issues S = Q K^T and O += P V.  While one tile's softmax runs, the
 //                   other tile's products do, so the matrix pipe and the exponentials overlap
 //   warp 9          (one thread) TMA loads of queries, keys and values, two stages each
+//   warps 10, 11    help to look at documents before the loop
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 since it was last used
 // (the weights stay below 2^8, the quotient is the same), so the accumulator is seldom touched
 // between products.
@@ -28,7 +29,9 @@ namespace {
 using namespace attn;
 using namespace tc;
 
-constexpr int kThreads = 320, kMmaWarp = 8, kTmaWarp = 9;
+constexpr int kThreads = 384, kMmaWarp = 8, kTmaWarp = 9;  // 10 and 11 fill the warpgroup
+// registers: softmax warps hold a row's 128 scores; 256 x 224 + 128 x 56 = 384 x 168, what the block has
+constexpr int kSoftmaxRegs = 224, kIssueRegs = 56;
 constexpr int kMaxTiles = 8192;              // key tiles of a call (2^20 keys): their bits fit in shared memory
 constexpr int kWords = kMaxTiles / 32;
 constexpr float kSlack = 8.f;                // growth of a maximum (log 2) that leaves the sums alone
@@ -113,7 +116,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 // the greatest of 32 values and t, in four chains
-__device__ __forceinline__ float max32(const float (&f)[32], float t) {
+__device__ __forceinline__ float max32(const float *f, float t) {
     float a[4] = {t, f[0], f[1], f[2]};
 #pragma unroll
     for (int x = 3; x + 1 < 32; x += 2) a[(x >> 1) & 3] = max3(a[(x >> 1) & 3], f[x], f[x + 1]);
@@ -124,7 +127,7 @@ __device__ constexpr float kTanh[6] = {1.f, -0.333332121f, 0.133305937f, -0.0536
 // polynomial in y^2 (least squares in Chebyshev points, within 2^-24 of tanh); a warp with a larger
 // one takes the exponential and the quotient.
 template <typename T>
-__device__ __forceinline__ void cap32(float (&f)[32], float scale, float cap) {
+__device__ __forceinline__ void cap32(float *f, float scale, float cap) {
     const float to_y = scale / cap, to_s = scale * kLog2e;
     float a = 0.f;
 #pragma unroll
@@ -155,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int *docs = (int *)(sm + L::docs);
     uint64_t *bars = (uint64_t *)(sm + L::bars);
     uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
-             *s_full = bars + 9, *p_full = bars + 11, *o_full = bars + 13, *tail = bars + 15;
-    uint32_t *slot = (uint32_t *)(bars + 16);
+             *s_full = bars + 9, *o_full = bars + 11, *tail = bars + 13, *p_half = bars + 14, *p_full = bars + 16;
+    uint32_t *slot = (uint32_t *)(bars + 18);
     volatile int *stop = (volatile int *)(slot + 1);
     int *lim = (int *)(slot + 2);  // [4] least and greatest document of the two query tiles
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const int ntiles = (max(emax[0], emax[1]) + 127) / 128;
     if (tid == 0) {
-        for (int i = 0; i < 16; i++) mbar_init(bars + i, i == 11 || i == 12 ? 4 : 1);  // p_full: a warp each
+        for (int i = 0; i < 18; i++) mbar_init(bars + i, i < 14 ? 1 : 4);  // weights: four warps
         *stop = 0;
         for (int i = 0; i < 4; i++) lim[i] = i & 1 ? -1 : 0x7fffffff;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -195,12 +198,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int w = tid; w < 4 * kWords; w += kThreads) act[w] = 0;
         __syncthreads();
         if (row) doc = p.q_docs[b * p.qds + i];
-        if (doc >= 0) {
-            atomicMin(&lim[2 * my], doc);
-            atomicMax(&lim[2 * my + 1], doc);
+        if (warp < kMmaWarp) {
+            // -1: a row that sees nothing, no tile goes without its mask
+            const int lo = __reduce_min_sync(0xffffffffu, row ? max(doc, -1) : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, doc);
+            if (lane == 0) {
+                atomicMin(&lim[2 * my], lo);
+                atomicMax(&lim[2 * my + 1], hi);
+            }
         }
-        bool neg = row && doc < 0;
-        if (neg) atomicMin(&lim[2 * my], -1);  // a row that sees nothing: no tile goes without its mask
         __syncthreads();
         // a key tile's documents against the query tiles': none shared, all the same, or some
         for (int j = warp; j < ntiles; j += kThreads / 32) {
@@ -236,13 +241,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         return p.q_docs ? (full[t * kWords + j / 32] >> (j & 31)) & 1 : (j + 1) * 128 <= emin[t];
     };
 
+    // the next key tile from j on that a query tile (2: either) visits
+    auto next = [&](int t, int j) -> int {
+        if (!p.q_docs) return j * 128 < (t == 2 ? max(emax[0], emax[1]) : emax[t]) ? j : ntiles;
+        for (; j < ntiles; j = (j | 31) + 1) {
+            const uint32_t w = ((t == 1 ? 0 : act[j / 32]) | (t == 0 ? 0 : act[kWords + j / 32])) >> (j & 31);
+            if (w) return j + __ffs(w) - 1;
+        }
+        return ntiles;
+    };
+
+    if (warp >= kMmaWarp) {
+    // (a warpgroup changes its registers as one)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == kTmaWarp) {
         const uint32_t qbytes = 128 * DP * 2;
         bool any = false;
         int it = 0;
         bool ok = true;
-        for (int j = 0; j < ntiles && ok; j++) {
-            if (!visits(0, j) && !visits(1, j)) continue;
+        for (int j = next(2, 0); j < ntiles && ok; j = next(2, j + 1)) {
             const int s = it & 1;
             const uint32_t par = (it >> 1) & 1;
             uint8_t *sk = sm + L::k + s * L::tile, *sv = sm + L::v + s * L::tile;
@@ -313,22 +330,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto product = [&](int t) {  // O_t += P_t V
                 if (pend[t] < 0) return;
                 const int s = pend[t] & 1;
-                ok = ok && mbar_wait_spin(&p_full[t], np[t] & 1, ta.status, stop, 44, ta.budget) &&
-                     mbar_wait_spin(&v_full[s], (pend[t] >> 1) & 1, ta.status, stop, 45, ta.budget);
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t v = smem_u32(sm + L::v + s * L::tile);
+                const uint64_t v = desc_n_major(smem_u32(sm + L::v + s * L::tile), kPanel);
 #pragma unroll
-                for (int x = 0; x < 8; x++)
-                    umma_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + x * 8, desc_n_major(v + x * 2048, kPanel), id_o,
-                            begun[t] || x > 0);
+                for (int half = 0; half < 2; half++) {
+                    ok = ok && mbar_wait_spin(half ? &p_full[t] : &p_half[t], np[t] & 1, ta.status, stop, 44, ta.budget);
+                    if (half == 0) ok = ok && mbar_wait_spin(&v_full[s], (pend[t] >> 1) & 1, ta.status, stop, 45, ta.budget);
+                    if (!ok) return;
+                    tc_fence_after();
+#pragma unroll
+                    for (int x = half * 4; x < half * 4 + 4; x++)
+                        umma_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + x * 8, v + x * (2048 / 16), id_o,
+                                begun[t] || x > 0);
+                }
                 begun[t] = true;
                 pend[t] = -1;
                 np[t]++;
             };
-            for (int j = 0; j < ntiles && ok; j++) {
+            for (int j = next(2, 0); j < ntiles && ok; j = next(2, j + 1)) {
                 const bool v0 = visits(0, j), v1 = visits(1, j);
-                if (!v0 && !v1) continue;
                 const int s = it & 1;
                 if (first) ok = mbar_wait_spin(q_full, 0, ta.status, stop, 46, ta.budget);
                 first = false;
@@ -340,10 +359,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     product(t);
                     if (!ok) break;
                     if (!(t ? v1 : v0)) continue;
-                    const uint32_t q = smem_u32(sm + L::q + t * L::tile), k = smem_u32(sm + L::k + s * L::tile);
-                    for (int x = 0; x < ksteps; x++) {
-                        const uint32_t off = (x >> 2) * kPanel + (x & 3) * 32;
-                        umma(tmem + kColS + t * 128, smem_desc(q + off), smem_desc(k + off), id_s, x > 0);
+                    const uint64_t q = smem_desc(smem_u32(sm + L::q + t * L::tile)), k = smem_desc(smem_u32(sm + L::k + s * L::tile));
+                    // (unrolled: a loop's address arithmetic takes longer than the products)
+#pragma unroll
+                    for (int x = 0; x < DP / 16; x++) {
+                        constexpr int kUnit = 16;  // descriptors count 16 bytes
+                        const int off = ((x >> 2) * kPanel + (x & 3) * 32) / kUnit;
+                        if (x < ksteps) umma(tmem + kColS + t * 128, q + off, k + off, id_s, x > 0);
                     }
                     umma_commit(&s_full[t]);
                     pend[t] = it & 3;
@@ -364,7 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
         }
         __syncwarp();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 tensor-memory lanes
         const uint32_t ts = tmem + lanes + kColS + my * 128, to = tmem + lanes + kColO + my * 128;
         const bool live = row && (!p.q_docs || doc >= 0);
@@ -375,8 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, l = 0.f;
         int n = 0;
         bool ok = true;
-        for (int j = 0; j < ntiles && ok; j++) {
-            if (!visits(my, j)) continue;
+        for (int j = next(my, 0); j < ntiles && ok; j = next(my, j + 1)) {
             const int j0 = j * 128;
             const bool plain = unmasked(my, j);
             if (p.q_docs && !plain) {
@@ -385,23 +408,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int x = lane; x < 128; x += 32) dk[x] = j0 + x < sp.nk ? p.kv_docs[b * p.kds + j0 + x] : -1;
                 __syncwarp();
             }
-            ok = warp_wait(&s_full[my], n & 1, ta.status, stop, 48, ta.budget);
+            ok = mbar_wait_spin(&s_full[my], n & 1, ta.status, stop, 48, ta.budget);
             if (!ok) break;
             tc_fence_after();
-            // First pass: the maximum.  What is not a plain product (capped, biased, masked) is worked
-            // out here and stored back, so that the second pass is the same for every tile.
-            float top = -INFINITY, mul = scale2;
-            if (plain && !special) {
-                float f[2][32];
-                tmem_ld32(ts, f[0]);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tmem_wait32(f[c & 1]);
-                    if (c < 3) tmem_ld32(ts + (c + 1) * 32, f[(c + 1) & 1]);
-                    top = max32(f[c & 1], top);
-                }
-                top *= mul;
-            } else {
+            // What is not a plain product (capped, biased, masked) is worked out first and stored back, 32
+            // columns at a time: the loop that every tile takes stays short enough for the instruction
+            // caches (unrolled over a row's 128 scores in registers these paths cost plain tiles 15 %).
+            float mul = scale2;
+            if (special || !plain) {
                 mul = 1.f;
 #pragma unroll 1
                 for (int c = 0; c < 4; c++) {
@@ -409,10 +423,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32(ts + c * 32, f);
                     tmem_wait32(f);
                     const int jc = j0 + c * 32;
-                    if (p.cap > 0.f) cap32<T>(f, p.scale, p.cap);
-                    else
+                    if (p.cap > 0.f) {
+                        cap32<T>(f, p.scale, p.cap);
+                    } else {
 #pragma unroll
                         for (int x = 0; x < 32; x++) f[x] *= scale2;
+                    }
                     if (p.slopes) {
                         const float far = (float)(pos - jc);
 #pragma unroll
@@ -423,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int x = 0; x < 32; x++)
                             if (x >= left) f[x] = -INFINITY;
-                        if (p.q_docs)
+                        if (p.q_docs) {
 #pragma unroll
                             for (int x = 0; x < 32; x += 4) {
                                 const int4 d = *(const int4 *)(dk + c * 32 + x);
@@ -432,12 +448,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if (d.z != doc) f[x + 2] = -INFINITY;
                                 if (d.w != doc) f[x + 3] = -INFINITY;
                             }
+                        }
                     }
-                    top = max32(f, top);
                     tmem_st32(ts + c * 32, f);
                 }
                 tmem_st_wait();
             }
+            float f[128], top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(ts + c * 32, f + c * 32);
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_wait32(f + c * 32);
+#pragma unroll
+            for (int c = 0; c < 4; c++) top = max32(f + c * 32, top);
+            top *= mul;
             top = fmaxf(m, top);
             if (m == -INFINITY) m = top;  // nothing seen so far: nothing to rescale
             const bool grown = m > -INFINITY && top - m > kSlack;
@@ -456,29 +480,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_st32(to + c0, o);
                 }
             }
-            // Second pass: weights, their sum, and the weights as 16-bit operands over the scores
-            // that have been read (16 columns behind 32).
+            // Weights, their sum, and the weights as 16-bit operands where the scores were.
             const float base = m == -INFINITY ? 0.f : m;
             const float2 mul2 = make_float2(mul, mul), off2 = make_float2(-base, -base);
             float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-            {
-                float f[2][32];
-                tmem_ld32(ts, f[0]);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tmem_wait32(f[c & 1]);
-                    if (c < 3) tmem_ld32(ts + (c + 1) * 32, f[(c + 1) & 1]);
-                    uint32_t w[16];
+            for (int c = 0; c < 4; c++) {
+                uint32_t w[16];
 #pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        float2 e = __ffma2_rn(make_float2(f[c & 1][2 * x], f[c & 1][2 * x + 1]), mul2, off2);
-                        e.x = ex2(e.x);
-                        e.y = ex2(e.y);
-                        if (x & 1) sum1 = __fadd2_rn(sum1, e);
-                        else sum0 = __fadd2_rn(sum0, e);
-                        w[x] = pack2<T>(e.x, e.y);  // the one rounding of a weight: the matrix instruction takes 16 bits
-                    }
-                    tmem_st16(ts + c * 16, w);
+                for (int x = 0; x < 16; x++) {
+                    float2 e = __ffma2_rn(make_float2(f[c * 32 + 2 * x], f[c * 32 + 2 * x + 1]), mul2, off2);
+                    e.x = ex2(e.x);
+                    e.y = ex2(e.y);
+                    if (x & 1) sum1 = __fadd2_rn(sum1, e);
+                    else sum0 = __fadd2_rn(sum0, e);
+                    w[x] = pack2<T>(e.x, e.y);  // the one rounding of a weight: the matrix instruction takes 16 bits
+                }
+                tmem_st16(ts + c * 16, w);
+                if (c == 1) {  // the product of the first 64 keys may begin
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_half[my]);
                 }
             }
             sum0 = __fadd2_rn(sum0, sum1);
@@ -493,11 +516,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) {
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            bool bad = !(fabsf(l) <= 3.4028234e38f);
-            T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
-#pragma unroll
-            for (int c0 = 0; c0 < DP; c0 += 32) {
-                if (c0 >= p.dim) break;
+            bool bad = !finite(l);
+            // rows through shared memory (the queries' tile is done with), 16-byte pieces XORed with the
+            // row against bank conflicts, so that a warp's stores cover whole rows
+            T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)(i - lane) * p.os[2];
+            uint8_t *stage = sm + L::q + my * L::tile + (warp & 3) * (L::tile / 4);
+            constexpr int kPieces = DP / 8;
+#pragma unroll 1
+            for (int c0 = 0; c0 < p.dim; c0 += 32) {
                 float f[32];
                 if (n > 0) {
                     tmem_ld32(to + c0, f);
@@ -508,23 +534,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll
                 for (int x = 0; x < 32; x++) {
-                    bad |= c0 + x < p.dim && !(fabsf(f[x]) <= 3.4028234e38f);
+                    bad |= c0 + x < p.dim && !finite(f[x]);
                     f[x] *= inv;
                 }
-                if (row) {
-                    if (ta.vec_out) {
 #pragma unroll
-                        for (int x = 0; x < 32; x += 8)
-                            if (c0 + x < p.dim)
-                                *(uint4 *)(o + c0 + x) = make_uint4(pack2<T>(f[x], f[x + 1]), pack2<T>(f[x + 2], f[x + 3]),
-                                                                    pack2<T>(f[x + 4], f[x + 5]), pack2<T>(f[x + 6], f[x + 7]));
-                    } else {
+                for (int x = 0; x < 4; x++)
+                    *(uint4 *)(stage + lane * DP * 2 + ((c0 / 8 + x) ^ (lane & 7)) * 16) =
+                        make_uint4(pack2<T>(f[8 * x], f[8 * x + 1]), pack2<T>(f[8 * x + 2], f[8 * x + 3]),
+                                   pack2<T>(f[8 * x + 4], f[8 * x + 5]), pack2<T>(f[8 * x + 6], f[8 * x + 7]));
+            }
+            __syncwarp();
+            const int pieces = p.dim / 8, rows_left = sp.nq - (i - lane);
+#pragma unroll 4
+            for (int u = lane; u < 32 * kPieces; u += 32) {
+                const int r = u / kPieces, c = u % kPieces;
+                if (r >= rows_left || c >= pieces) continue;
+                const uint4 v = *(const uint4 *)(stage + r * DP * 2 + (c ^ (r & 7)) * 16);
+                T *at = o + r * p.os[2] + c * 8;
+                if (ta.vec_out) {
+                    *(uint4 *)at = v;
+                } else {
+                    const T *e = (const T *)&v;
 #pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (c0 + x < p.dim) o[c0 + x] = from_f<T>(f[x]);
-                    }
+                    for (int x = 0; x < 8; x++) at[x] = e[x];
                 }
             }
+            __syncwarp();
             uint32_t rows = __ballot_sync(0xffffffffu, bad && row);
             while (rows) {
                 const int r = __ffs(rows) - 1;
