@@ -101,7 +101,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const float (&f)[32]) {
+__device__ __forceinline__ void tmem_st32(uint32_t at, const float *f) {
     uint32_t r[16];
 #pragma unroll
     for (int y = 0; y < 2; y++) {
@@ -137,10 +137,16 @@ __device__ __forceinline__ void cap32(float *f, float scale, float cap) {
         for (int x = 0; x < 32; x++) f[x] = capped2<T>(f[x] * scale, cap);
         return;
     }
+    const float2 yy = make_float2(to_y, to_y), ss = make_float2(to_s, to_s);
 #pragma unroll
-    for (int x = 0; x < 32; x++) {
-        const float y = f[x] * to_y, t = y * y;
-        f[x] = f[x] * to_s * fmaf(fmaf(fmaf(fmaf(fmaf(kTanh[5], t, kTanh[4]), t, kTanh[3]), t, kTanh[2]), t, kTanh[1]), t, kTanh[0]);
+    for (int x = 0; x < 32; x += 2) {
+        const float2 v = make_float2(f[x], f[x + 1]), y = __fmul2_rn(v, yy), t = __fmul2_rn(y, y);
+        float2 r = make_float2(kTanh[5], kTanh[5]);
+#pragma unroll
+        for (int k = 4; k >= 0; k--) r = __ffma2_rn(r, t, make_float2(kTanh[k], kTanh[k]));
+        r = __fmul2_rn(r, __fmul2_rn(v, ss));
+        f[x] = r.x;
+        f[x + 1] = r.y;
     }
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -234,22 +240,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    auto visits = [&](int t, int j) -> bool {
-        return p.q_docs ? (act[t * kWords + j / 32] >> (j & 31)) & 1 : j * 128 < emax[t];
-    };
-    auto unmasked = [&](int t, int j) -> bool {
-        return p.q_docs ? (full[t * kWords + j / 32] >> (j & 31)) & 1 : (j + 1) * 128 <= emin[t];
-    };
+    const bool by_doc = p.q_docs != nullptr;
+    const int whole = my == 0 ? emin[0] : emin[1], reach = my == 0 ? emax[0] : emax[1];  // of the thread's query tile
+    auto visits = [&](int t, int e, int j) -> bool { return by_doc ? (act[t * kWords + j / 32] >> (j & 31)) & 1 : j * 128 < e; };
 
-    // the next key tile from j on that a query tile (2: either) visits
-    auto next = [&](int t, int j) -> int {
-        if (!p.q_docs) return j * 128 < (t == 2 ? max(emax[0], emax[1]) : emax[t]) ? j : ntiles;
+    // the next key tile from j on that is visited by the query tiles of `tiles` (bits), which reach to key e
+    auto next = [&](int tiles, int e, int j) -> int {
+        if (!by_doc) return j * 128 < e ? j : ntiles;
         for (; j < ntiles; j = (j | 31) + 1) {
-            const uint32_t w = ((t == 1 ? 0 : act[j / 32]) | (t == 0 ? 0 : act[kWords + j / 32])) >> (j & 31);
+            const uint32_t w = ((tiles & 1 ? act[j / 32] : 0) | (tiles & 2 ? act[kWords + j / 32] : 0)) >> (j & 31);
             if (w) return j + __ffs(w) - 1;
         }
         return ntiles;
     };
+    const int ends = max(emax[0], emax[1]);
 
     if (warp >= kMmaWarp) {
     // (a warpgroup changes its registers as one)
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool any = false;
         int it = 0;
         bool ok = true;
-        for (int j = next(2, 0); j < ntiles && ok; j = next(2, j + 1)) {
+        for (int j = next(3, ends, 0); j < ntiles && ok; j = next(3, ends, j + 1)) {
             const int s = it & 1;
             const uint32_t par = (it >> 1) & 1;
             uint8_t *sk = sm + L::k + s * L::tile, *sv = sm + L::v + s * L::tile;
@@ -346,8 +350,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pend[t] = -1;
                 np[t]++;
             };
-            for (int j = next(2, 0); j < ntiles && ok; j = next(2, j + 1)) {
-                const bool v0 = visits(0, j), v1 = visits(1, j);
+            for (int j = next(3, ends, 0); j < ntiles && ok; j = next(3, ends, j + 1)) {
+                const bool v0 = visits(0, emax[0], j), v1 = visits(1, emax[1], j);
                 const int s = it & 1;
                 if (first) ok = mbar_wait_spin(q_full, 0, ta.status, stop, 46, ta.budget);
                 first = false;
@@ -394,15 +398,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = row && (!p.q_docs || doc >= 0);
         const int end = live ? key_end(p, sp, i) : 0, pos = sp.off + i;
         const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.f, scale2 = p.scale * kLog2e;
-        const bool special = p.cap > 0.f || p.slopes || !(scale2 > 0.f);
+        const bool capped = p.cap > 0.f, special = capped || p.slopes || !(scale2 > 0.f);
         int *dk = docs + warp * 128;
         float m = -INFINITY, l = 0.f;
         int n = 0;
         bool ok = true;
-        for (int j = next(my, 0); j < ntiles && ok; j = next(my, j + 1)) {
+        for (int j = next(1 << my, reach, 0); j < ntiles && ok; j = next(1 << my, reach, j + 1)) {
             const int j0 = j * 128;
-            const bool plain = unmasked(my, j);
-            if (p.q_docs && !plain) {
+            const bool plain = by_doc ? (full[my * kWords + j / 32] >> (j & 31)) & 1 : j0 + 128 <= whole;
+            if (by_doc && !plain) {
                 __syncwarp();  // the ids of the tile before have been read
 #pragma unroll
                 for (int x = lane; x < 128; x += 32) dk[x] = j0 + x < sp.nk ? p.kv_docs[b * p.kds + j0 + x] : -1;
@@ -417,13 +421,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             float mul = scale2;
             if (special || !plain) {
                 mul = 1.f;
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    float f[32];
-                    tmem_ld32(ts + c * 32, f);
-                    tmem_wait32(f);
+                float g[2][32];
+                tmem_ld32(ts, g[0]);
+                auto work = [&](int c, float *f) {
                     const int jc = j0 + c * 32;
-                    if (p.cap > 0.f) {
+                    if (capped) {
                         cap32<T>(f, p.scale, p.cap);
                     } else {
 #pragma unroll
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int x = 0; x < 32; x++)
                             if (x >= left) f[x] = -INFINITY;
-                        if (p.q_docs) {
+                        if (by_doc) {
 #pragma unroll
                             for (int x = 0; x < 32; x += 4) {
                                 const int4 d = *(const int4 *)(dk + c * 32 + x);
@@ -451,6 +453,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     tmem_st32(ts + c * 32, f);
+                };
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
+                    tmem_wait32(g[0]);
+                    tmem_ld32(ts + (c + 1) * 32, g[1]);
+                    work(c, g[0]);
+                    tmem_wait32(g[1]);
+                    if (c == 0) tmem_ld32(ts + 64, g[0]);
+                    work(c + 1, g[1]);
                 }
                 tmem_st_wait();
             }
