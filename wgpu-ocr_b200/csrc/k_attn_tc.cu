@@ -151,6 +151,15 @@ __device__ __forceinline__ void cap32(float *f, float scale, float cap) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// the value of lane 0, known to be the same in every lane
+__device__ __forceinline__ int same(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t same(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ bool elect() {  // one lane of the warp, always the same
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attn_tc(const __grid_constant__ TcArgs ta, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -322,73 +331,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
-        if (lane == 0) {
-            constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-            const int ksteps = (p.dim + 15) / 16;
-            const uint32_t id_s = idesc(bf, 128, false), id_o = idesc(bf, ksteps * 16, true);
-            bool ok = true, first = true;
-            bool begun[2] = {false, false};
-            int pend[2] = {-1, -1};      // stage (and phase) of the values that a tile's weights wait for
-            int np[2] = {0, 0};          // weights consumed
-            int it = 0, prev = -1;
-            auto product = [&](int t) {  // O_t += P_t V
-                if (pend[t] < 0) return;
-                const int s = pend[t] & 1;
-                const uint64_t v = desc_n_major(smem_u32(sm + L::v + s * L::tile), kPanel);
+        // The whole warp walks the loop, on values that are the same in every lane, and one lane
+        // issues: an instruction's descriptors are uniform registers, and from one lane's own ones
+        // they took 75 to 100 cycles an instruction to move there.
+        constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+        const int ksteps = (p.dim + 15) / 16;
+        const uint32_t id_s = idesc(bf, 128, false), id_o = idesc(bf, ksteps * 16, true), tm = same(tmem);
+        const uint64_t dq = smem_desc(same(smem_u32(sm + L::q))), dk = smem_desc(same(smem_u32(sm + L::k))),
+                       dv = desc_n_major(same(smem_u32(sm + L::v)), kPanel);
+        const int e0 = same(emax[0]), e1 = same(emax[1]), eb = max(e0, e1), nt = (eb + 127) / 128;
+        constexpr int kUnits = L::tile / 16;  // descriptors count 16 bytes
+        bool ok = true;
+        int pend[2] = {-1, -1};  // number of the key tile whose values a tile's weights wait for
+        int np[2] = {0, 0};      // weights consumed
+        int it = 0;
+        auto wait = [&](uint64_t *bar, int parity, int code) -> bool {
+            return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity & 1, ta.status, stop, code, ta.budget));
+        };
+        auto product = [&](int t) {  // O_t += P_t V
+            if (pend[t] < 0) return;
+            const int s = pend[t] & 1;
+            const uint64_t v = dv + s * kUnits;
+            const uint32_t weights = tm + kColS + t * 128, sums = tm + kColO + t * 128, more = np[t] > 0;
+            ok = ok && wait(&v_full[s], pend[t] >> 1, 45) && wait(&p_half[t], np[t], 44);
+            if (!ok) return;
+            tc_fence_after();
+            if (elect()) {
+                umma_ts(sums, weights, v, id_o, more);
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    ok = ok && mbar_wait_spin(half ? &p_full[t] : &p_half[t], np[t] & 1, ta.status, stop, 44, ta.budget);
-                    if (half == 0) ok = ok && mbar_wait_spin(&v_full[s], (pend[t] >> 1) & 1, ta.status, stop, 45, ta.budget);
-                    if (!ok) return;
-                    tc_fence_after();
-#pragma unroll
-                    for (int x = half * 4; x < half * 4 + 4; x++)
-                        umma_ts(tmem + kColO + t * 128, tmem + kColS + t * 128 + x * 8, v + x * (2048 / 16), id_o,
-                                begun[t] || x > 0);
-                }
-                begun[t] = true;
-                pend[t] = -1;
-                np[t]++;
-            };
-            for (int j = next(3, ends, 0); j < ntiles && ok; j = next(3, ends, j + 1)) {
-                const bool v0 = visits(0, emax[0], j), v1 = visits(1, emax[1], j);
-                const int s = it & 1;
-                if (first) ok = mbar_wait_spin(q_full, 0, ta.status, stop, 46, ta.budget);
-                first = false;
-                ok = ok && mbar_wait_spin(&k_full[s], (it >> 1) & 1, ta.status, stop, 47, ta.budget);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    product(t);
-                    if (!ok) break;
-                    if (!(t ? v1 : v0)) continue;
-                    const uint64_t q = smem_desc(smem_u32(sm + L::q + t * L::tile)), k = smem_desc(smem_u32(sm + L::k + s * L::tile));
-                    // (unrolled: a loop's address arithmetic takes longer than the products)
-#pragma unroll
-                    for (int x = 0; x < DP / 16; x++) {
-                        constexpr int kUnit = 16;  // descriptors count 16 bytes
-                        const int off = ((x >> 2) * kPanel + (x & 3) * 32) / kUnit;
-                        if (x < ksteps) umma(tmem + kColS + t * 128, q + off, k + off, id_s, x > 0);
-                    }
-                    umma_commit(&s_full[t]);
-                    pend[t] = it & 3;
-                }
-                if (!ok) break;
-                umma_commit(&k_empty[s]);
-                if (prev >= 0) umma_commit(&v_empty[prev]);
-                prev = s;
-                it++;
+                for (int x = 1; x < 4; x++) umma_ts(sums, weights + x * 8, v + x * (2048 / 16), id_o, 1);
             }
+            __syncwarp();
+            ok = wait(&p_full[t], np[t], 44);
+            if (!ok) return;
+            tc_fence_after();
+            if (elect()) {
+#pragma unroll
+                for (int x = 4; x < 8; x++) umma_ts(sums, weights + x * 8, v + x * (2048 / 16), id_o, 1);
+            }
+            __syncwarp();
+            pend[t] = -1;
+            np[t]++;
+        };
+        for (int j = same(next(3, eb, 0)); j < nt && ok; j = same(next(3, eb, j + 1)), it++) {
+            const bool v0 = same((int)visits(0, e0, j)), v1 = same((int)visits(1, e1, j));
+            const int s = it & 1;
+            if (it == 0) ok = wait(q_full, 0, 46);
+            ok = ok && wait(&k_full[s], it >> 1, 47);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
             for (int t = 0; t < 2; t++) {
                 product(t);
-                umma_commit(&o_full[t]);
-            }
-            const long long t0 = clock64();
-            for (int t = 0; t < 2; t++)
-                while (!mbar_try(&o_full[t], 0) && clock64() - t0 < ta.budget) {
+                if (!ok) break;
+                if (!(t ? v1 : v0)) continue;
+                const uint64_t q = dq + t * kUnits, k = dk + s * kUnits;
+                const uint32_t scores = tm + kColS + t * 128;
+                if (elect()) {
+                    umma(scores, q, k, id_s, 0);
+#pragma unroll
+                    for (int x = 1; x < DP / 16; x++) {
+                        const int off = ((x >> 2) * kPanel + (x & 3) * 32) / 16;
+                        if (x < ksteps) umma(scores, q + off, k + off, id_s, 1);
+                    }
+                    umma_commit(&s_full[t]);
                 }
+                __syncwarp();
+                pend[t] = it;
+            }
+            if (!ok) break;
+            if (elect()) {
+                umma_commit(&k_empty[s]);
+                if (it > 0) umma_commit(&v_empty[s ^ 1]);
+            }
+            __syncwarp();
         }
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            product(t);
+            if (elect()) umma_commit(&o_full[t]);
+            __syncwarp();
+        }
+        const long long t0 = clock64();
+        for (int t = 0; t < 2; t++)
+            while (!mbar_try(&o_full[t], 0) && clock64() - t0 < ta.budget) {
+            }
         __syncwarp();
     }
     } else {
