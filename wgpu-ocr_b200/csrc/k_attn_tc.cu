@@ -16,6 +16,7 @@
 // Bound: 4 D flops and one exponential a pair.  An SM's matrix pipe takes 128 x 128 x 128 in 512
 // cycles and its 16 exponentials a cycle take as long for two such products (D = 128).
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "attn.h"
@@ -30,8 +31,9 @@ using namespace attn;
 using namespace tc;
 
 constexpr int kThreads = 384, kMmaWarp = 8, kTmaWarp = 9;  // 10 and 11 fill the warpgroup
-// registers: softmax warps hold a row's 128 scores; 256 x 224 + 128 x 56 = 384 x 168, what the block has
-constexpr int kSoftmaxRegs = 224, kIssueRegs = 56;
+// registers: softmax warps hold a row's 128 scores; 256 x 192 + 128 x 120 = 384 x 168, what the block has
+// (224 and 56 left the issuing warp 15 % of the kernel's time in spills)
+constexpr int kSoftmaxRegs = 192, kIssueRegs = 120;
 constexpr int kMaxTiles = 8192;              // key tiles of a call (2^20 keys): their bits fit in shared memory
 constexpr int kWords = kMaxTiles / 32;
 constexpr float kSlack = 8.f;                // growth of a maximum (log 2) that leaves the sums alone
@@ -160,7 +162,10 @@ __device__ __forceinline__ bool elect() {  // one lane of the warp, always the s
     return one != 0;
 }
 
-template <typename T, int DP>
+// EXTRA: scores that are more than a plain product (capped, biased by distance, a scale that is not
+// positive), or documents.  Apart, since their code, unrolled over a row, cost plain tiles 15 % in
+// the instruction caches.
+template <typename T, int DP, bool EXTRA>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attn_tc(const __grid_constant__ TcArgs ta, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv) {
@@ -209,7 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int i = i_first + my * 128 + (tid & 127);
     const bool row = warp < 8 && i < sp.nq;
     int doc = -1;
-    if (p.q_docs) {
+    const bool by_doc = EXTRA && p.q_docs != nullptr;
+    if (by_doc) {
         for (int w = tid; w < 4 * kWords; w += kThreads) act[w] = 0;
         __syncthreads();
         if (row) doc = p.q_docs[b * p.qds + i];
@@ -249,7 +255,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
-    const bool by_doc = p.q_docs != nullptr;
     const int whole = my == 0 ? emin[0] : emin[1], reach = my == 0 ? emax[0] : emax[1];  // of the thread's query tile
     auto visits = [&](int t, int e, int j) -> bool { return by_doc ? (act[t * kWords + j / 32] >> (j & 31)) & 1 : j * 128 < e; };
 
@@ -422,8 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 tensor-memory lanes
         const uint32_t ts = tmem + lanes + kColS + my * 128, to = tmem + lanes + kColO + my * 128;
-        const bool live = row && (!p.q_docs || doc >= 0);
+        const bool live = row && (!by_doc || doc >= 0);
         const int end = live ? key_end(p, sp, i) : 0, pos = sp.off + i;
+        if (doc < 0) doc = INT_MIN;  // sees nothing: the ids staged below are -1 or more
         const float slope = p.slopes ? p.slopes[h] * kLog2e : 0.f, scale2 = p.scale * kLog2e;
         const bool capped = p.cap > 0.f, special = capped || p.slopes || !(scale2 > 0.f);
         int *dk = docs + warp * 128;
@@ -436,67 +442,50 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (by_doc && !plain) {
                 __syncwarp();  // the ids of the tile before have been read
 #pragma unroll
-                for (int x = lane; x < 128; x += 32) dk[x] = j0 + x < sp.nk ? p.kv_docs[b * p.kds + j0 + x] : -1;
+                for (int x = lane; x < 128; x += 32) dk[x] = j0 + x < sp.nk ? max(p.kv_docs[b * p.kds + j0 + x], -1) : -1;
                 __syncwarp();
             }
             ok = mbar_wait_spin(&s_full[my], n & 1, ta.status, stop, 48, ta.budget);
             if (!ok) break;
             tc_fence_after();
-            // What is not a plain product (capped, biased, masked) is worked out first and stored back, 32
-            // columns at a time: the loop that every tile takes stays short enough for the instruction
-            // caches (unrolled over a row's 128 scores in registers these paths cost plain tiles 15 %).
-            float mul = scale2;
-            if (special || !plain) {
-                mul = 1.f;
-                float g[2][32];
-                tmem_ld32(ts, g[0]);
-                auto work = [&](int c, float *f) {
-                    const int jc = j0 + c * 32;
-                    if (capped) {
-                        cap32<T>(f, p.scale, p.cap);
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 32; x++) f[x] *= scale2;
-                    }
-                    if (p.slopes) {
-                        const float far = (float)(pos - jc);
-#pragma unroll
-                        for (int x = 0; x < 32; x++) f[x] = fmaf(-slope, fabsf(far - (float)x), f[x]);
-                    }
-                    if (!plain) {
-                        const int left = end - jc;
-#pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (x >= left) f[x] = -INFINITY;
-                        if (by_doc) {
-#pragma unroll
-                            for (int x = 0; x < 32; x += 4) {
-                                const int4 d = *(const int4 *)(dk + c * 32 + x);
-                                if (d.x != doc) f[x] = -INFINITY;
-                                if (d.y != doc) f[x + 1] = -INFINITY;
-                                if (d.z != doc) f[x + 2] = -INFINITY;
-                                if (d.w != doc) f[x + 3] = -INFINITY;
-                            }
-                        }
-                    }
-                    tmem_st32(ts + c * 32, f);
-                };
-#pragma unroll 1
-                for (int c = 0; c < 4; c += 2) {
-                    tmem_wait32(g[0]);
-                    tmem_ld32(ts + (c + 1) * 32, g[1]);
-                    work(c, g[0]);
-                    tmem_wait32(g[1]);
-                    if (c == 0) tmem_ld32(ts + 64, g[0]);
-                    work(c + 1, g[1]);
-                }
-                tmem_st_wait();
-            }
-            float f[128], top = -INFINITY;
+            float f[128], top = -INFINITY, mul = scale2;
 #pragma unroll
             for (int c = 0; c < 4; c++) tmem_ld32(ts + c * 32, f + c * 32);
 #pragma unroll
             for (int c = 0; c < 4; c++) tmem_wait32(f + c * 32);
+            if (EXTRA && special) {
+                mul = 1.f;
+                if (capped) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) cap32<T>(f + c * 32, p.scale, p.cap);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 128; x++) f[x] *= scale2;
+                }
+                if (p.slopes) {
+                    const float far = (float)(pos - j0);
+#pragma unroll
+                    for (int x = 0; x < 128; x++) f[x] = fmaf(-slope, fabsf(far - (float)x), f[x]);
+                }
+            }
+            if (!plain) {
+                const int left = end - j0;
+                if (!by_doc || p.causal) {  // (documents' ids end with the keys)
+#pragma unroll
+                    for (int x = 0; x < 128; x++)
+                        if (x >= left) f[x] = -INFINITY;
+                }
+                if (EXTRA && by_doc) {
+#pragma unroll
+                    for (int x = 0; x < 128; x += 4) {
+                        const int4 d = *(const int4 *)(dk + x);
+                        if (d.x != doc) f[x] = -INFINITY;
+                        if (d.y != doc) f[x + 1] = -INFINITY;
+                        if (d.z != doc) f[x + 2] = -INFINITY;
+                        if (d.w != doc) f[x + 3] = -INFINITY;
+                    }
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 4; c++) top = max32(f + c * 32, top);
             top *= mul;
@@ -632,12 +621,24 @@ void make_map(CUtensorMap &m, bool bf16, const void *p, const int64_t *st, int b
     if (r != CUDA_SUCCESS) fail(WOCR_ERR_CUDA, "cuTensorMapEncodeTiled (attention) failed: " + std::to_string((int)r));
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool EXTRA>
 void launch(Ctx *c, const TcArgs &ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
     const int bytes = Smem<DP>::bytes;
-    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tc<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    k_attn_tc<T, DP><<<(unsigned)(ta.tiles * ta.a.batch * ta.a.heads), kThreads, bytes, s>>>(ta, mq, mk, mv);
+    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tc<T, DP, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    k_attn_tc<T, DP, EXTRA><<<(unsigned)(ta.tiles * ta.a.batch * ta.a.heads), kThreads, bytes, s>>>(ta, mq, mk, mv);
     WOCR_LAUNCHED(c);
+}
+template <typename T>
+void launch_dim(Ctx *c, const TcArgs &ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
+    const AttnP &p = ta.a;
+    const bool extra = p.cap > 0.f || p.slopes || !(p.scale > 0.f) || p.q_docs;
+    if (p.dim <= 64) {
+        if (extra) launch<T, 64, true>(c, ta, mq, mk, mv, s);
+        else launch<T, 64, false>(c, ta, mq, mk, mv, s);
+    } else {
+        if (extra) launch<T, 128, true>(c, ta, mq, mk, mv, s);
+        else launch<T, 128, false>(c, ta, mq, mk, mv, s);
+    }
 }
 }  // namespace
 
@@ -668,13 +669,8 @@ void attention_tc(Ctx *c, const AttnP &p, cudaStream_t s) {
     make_map(mq, bf, p.q, p.qs, p.batch, p.heads, p.q_len, p.dim);
     make_map(mk, bf, p.k, p.ks, p.batch, p.kv_heads, p.kv_len, p.dim);
     make_map(mv, bf, p.v, p.vs, p.batch, p.kv_heads, p.kv_len, p.dim);
-    if (p.dim <= 64) {
-        if (bf) launch<__nv_bfloat16, 64>(c, ta, mq, mk, mv, s);
-        else launch<__half, 64>(c, ta, mq, mk, mv, s);
-    } else {
-        if (bf) launch<__nv_bfloat16, 128>(c, ta, mq, mk, mv, s);
-        else launch<__half, 128>(c, ta, mq, mk, mv, s);
-    }
+    if (bf) launch_dim<__nv_bfloat16>(c, ta, mq, mk, mv, s);
+    else launch_dim<__half>(c, ta, mq, mk, mv, s);
 }
 
 }  // namespace k
