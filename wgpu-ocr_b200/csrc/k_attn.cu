@@ -24,39 +24,64 @@ struct TileSmem {
     static constexpr int LD = DP + 8;  // elements per row: eight rows start in eight different 16-byte banks
     static constexpr bool q_in_regs = P * DP <= 128;
     static constexpr int q_rows = q_in_regs ? 0 : 64;
+    static constexpr int stages = P == 1 ? 2 : 1;  // 16-bit tiles arrive behind the one in work
     static constexpr size_t q = (size_t)P * q_rows * LD * 2, kv = (size_t)P * BK * LD * 2;
-    static constexpr size_t tiles = q + 2 * kv, parts = 4 * sizeof(PartSums<DP>);
+    static constexpr size_t tiles = q + 2 * stages * kv, parts = 4 * sizeof(PartSums<DP>);
     static constexpr size_t bytes = tiles > parts ? tiles : parts;
 };
 
-// `rows` rows of a [.., dim] tensor from row r0 on, split into parts in shared memory; rows from
-// `end` on and dimensions from dim on become zero.
-template <typename T, int DP>
-__device__ __forceinline__ void load_rows(uint16_t *dst, int rows, const T *src, int64_t stride, int r0, int end, int dim, bool vec) {
-    constexpr int P = Parts<T>::n, LD = DP + 8;
-#pragma unroll 2
-    for (int u = threadIdx.x; u < rows * (DP / 8); u += 128) {
+// ROWS rows of a [.., dim] tensor from row r0 on for shared memory, 8 elements a unit: fetched into a
+// thread's registers, all loads under way together, and put as parts.  Rows from `end` on and
+// dimensions from dim on become zero.
+template <typename T, int DP, int ROWS>
+struct Units {
+    static constexpr int n = ROWS * DP / 8 / 128;
+    T v[n][8];
+    __device__ __forceinline__ void fetch(const T *src, int64_t stride, int r0, int end, int dim, bool vec) {
+#pragma unroll
+        for (int y = 0; y < n; y++) {
+            const int u = y * 128 + threadIdx.x, r = u / (DP / 8), d0 = u % (DP / 8) * 8;
+            const bool in = r0 + r < end;
+            const T *s = src + (int64_t)(r0 + r) * stride + d0;
+            if (in && vec && d0 + 8 <= dim) {
+#pragma unroll
+                for (int x = 0; x < (int)sizeof(T) / 2; x++) reinterpret_cast<uint4 *>(v[y])[x] = reinterpret_cast<const uint4 *>(s)[x];
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; x++) v[y][x] = in && d0 + x < dim ? s[x] : from_f<T>(0.f);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(uint16_t *dst) const {
+        constexpr int P = Parts<T>::n, LD = DP + 8;
+#pragma unroll
+        for (int y = 0; y < n; y++) {
+            const int u = y * 128 + threadIdx.x, r = u / (DP / 8), d0 = u % (DP / 8) * 8;
+            if constexpr (P == 1) {
+                *reinterpret_cast<uint4 *>(dst + r * LD + d0) = *reinterpret_cast<const uint4 *>(v[y]);
+            } else {
+                uint32_t w[4][P];
+#pragma unroll
+                for (int x = 0; x < 4; x++) split2<T>(v[y][2 * x], v[y][2 * x + 1], w[x]);
+#pragma unroll
+                for (int z = 0; z < P; z++)
+                    *reinterpret_cast<uint4 *>(dst + (z * ROWS + r) * LD + d0) = make_uint4(w[0][z], w[1][z], w[2][z], w[3][z]);
+            }
+        }
+    }
+};
+// The same of 16-bit rows with 16-byte loads, straight to shared memory behind the thread's back.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void copy_rows(uint16_t *dst, const T *src, int64_t stride, int r0, int end, int dim) {
+#pragma unroll
+    for (int u = threadIdx.x; u < ROWS * DP / 8; u += 128) {
         const int r = u / (DP / 8), d0 = u % (DP / 8) * 8;
-        const bool in = r0 + r < end;
-        const T *s = src + (int64_t)(r0 + r) * stride + d0;
-        T v[8];
-        if (in && vec && d0 + 8 <= dim) {
-#pragma unroll
-            for (int x = 0; x < (int)sizeof(T) / 2; x++) reinterpret_cast<uint4 *>(v)[x] = reinterpret_cast<const uint4 *>(s)[x];
-        } else {
-#pragma unroll
-            for (int x = 0; x < 8; x++) v[x] = in && d0 + x < dim ? s[x] : from_f<T>(0.f);
-        }
-        if constexpr (P == 1) {
-            *reinterpret_cast<uint4 *>(dst + r * LD + d0) = *reinterpret_cast<const uint4 *>(v);
-        } else {
-            uint32_t w[4][P];
-#pragma unroll
-            for (int x = 0; x < 4; x++) split2<T>(v[2 * x], v[2 * x + 1], w[x]);
-#pragma unroll
-            for (int y = 0; y < P; y++)
-                *reinterpret_cast<uint4 *>(dst + (y * rows + r) * LD + d0) = make_uint4(w[0][y], w[1][y], w[2][y], w[3][y]);
-        }
+        const int bytes = r0 + r < end ? min(max(dim - d0, 0), 8) * 2 : 0;  // the rest is filled with zeros
+        const T *s = bytes ? src + (int64_t)(r0 + r) * stride + d0 : src;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(dst + r * (DP + 8) + d0)),
+                     "l"(s), "r"(bytes)
+                     : "memory");
     }
 }
 
@@ -83,7 +108,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ JoinSmem js;
     __shared__ int ends[64], seen;
-    uint16_t *sq = (uint16_t *)dyn, *sk = (uint16_t *)(dyn + S::q), *sv = (uint16_t *)(dyn + S::q + S::kv);
+    uint16_t *sq = (uint16_t *)dyn, *tiles = (uint16_t *)(dyn + S::q);
     cg::cluster_group cl = cg::this_cluster();
     const int cs = cl.num_blocks(), rank = cl.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -141,7 +166,9 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
             for (int y = 0; y < P; y++) *reinterpret_cast<uint32_t *>(sq + (y * 64 + r) * LD + d) = w[y];
         }
     } else {
-        load_rows<T, DP>(sq, 64, (const T *)p.q + b * p.qs[0] + hq * p.qs[1], p.qs[2], tile * 64, sp.nq, p.dim, vec);
+        Units<T, DP, 64> u;
+        u.fetch((const T *)p.q + b * p.qs[0] + hq * p.qs[1], p.qs[2], tile * 64, sp.nq, p.dim, vec);
+        u.put(sq);
     }
     __syncthreads();
     const int last = seen;  // keys that any row sees
@@ -163,11 +190,41 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
 #pragma unroll
         for (int x = 0; x < 4; x++) acc[n][x] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    for (int j0 = rank * BK; j0 < last; j0 += cs * BK) {
-        __syncthreads();  // the tile before has been read
-        load_rows<T, DP>(sk, BK, kb, p.ks[2], j0, sp.nk, p.dim, vec);
-        load_rows<T, DP>(sv, BK, vb, p.vs[2], j0, sp.nk, p.dim, vec);
-        __syncthreads();
+    const bool async = P == 1 && vec;
+    // 32-bit tiles of up to 64 dimensions wait in registers while the tile before is in work
+    constexpr bool AHEAD = P == 3 && DP <= 64;
+    Units<T, DP, BK> nk, nv;
+    auto copy = [&](int j, int stage) {
+        if constexpr (P == 1) {
+            copy_rows<T, DP, BK>(tiles + stage * S::kv, kb, p.ks[2], j, sp.nk, p.dim);  // (kv bytes: two stages' elements)
+            copy_rows<T, DP, BK>(tiles + stage * S::kv + S::kv / 2, vb, p.vs[2], j, sp.nk, p.dim);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int stage = 0;
+    if (async) copy(rank * BK, 0);
+    else if (AHEAD && rank * BK < last) {
+        nk.fetch(kb, p.ks[2], rank * BK, sp.nk, p.dim, vec);
+        nv.fetch(vb, p.vs[2], rank * BK, sp.nk, p.dim, vec);
+    }
+    for (int j0 = rank * BK; j0 < last; j0 += cs * BK, stage ^= async) {
+        uint16_t *sk = tiles + stage * S::kv, *sv = sk + S::kv / 2;
+        if (async) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();  // this tile is there, and the one before has been read
+            if (j0 + cs * BK < last) copy(j0 + cs * BK, stage ^ 1);
+        } else {
+            __syncthreads();  // the tile before has been read
+            if (!AHEAD) nk.fetch(kb, p.ks[2], j0, sp.nk, p.dim, vec);
+            nk.put(sk);
+            if (!AHEAD) nv.fetch(vb, p.vs[2], j0, sp.nk, p.dim, vec);
+            nv.put(sv);
+            __syncthreads();
+            if (AHEAD && j0 + cs * BK < last) {
+                nk.fetch(kb, p.ks[2], j0 + cs * BK, sp.nk, p.dim, vec);
+                nv.fetch(vb, p.vs[2], j0 + cs * BK, sp.nk, p.dim, vec);
+            }
+        }
         const int jw = j0 + (FEW ? warp * WK : 0), kw = FEW ? warp * WK : 0;
         float s[NT][4];
 #pragma unroll
@@ -309,6 +366,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
         l0 += __shfl_xor_sync(0xffffffffu, l0, d);
         l1 += __shfl_xor_sync(0xffffffffu, l1, d);
     }
+    if (async) asm volatile("cp.async.wait_group 0;" ::: "memory");
     T *ob = (T *)p.o + b * p.os[0];
     if (!FEW && cs == 1) {
         const float v0 = l0 == 0.f ? 0.f : 1.f / l0, v1 = l1 == 0.f ? 0.f : 1.f / l1;
@@ -596,7 +654,10 @@ void attention(Ctx *c, const AttnP &p, cudaStream_t s) {
     const double rows = (double)p.batch * p.heads * p.q_len;
     OpProf pf(c, s, "attention", 4.0 * rows * p.kv_len * p.dim,
               elem_size(p.type) * (double)p.dim * (2.0 * rows + 2.0 * p.batch * p.kv_heads * p.kv_len));
-    if (p.q_len >= 128 && attention_tc_ok(p)) return attention_tc(c, p, s);
+    // Tiles of 128 queries on tcgen05 once they are half full, or the keys are many: 64 queries over 64
+    // keys, 128 x 8 heads of 64: 25 us against 33, 40 over 40: 37 both; 20 over 4,096, 16 x 16 heads of
+    // 128: 113 us against 617.
+    if (p.q_len > 16 && (p.q_len >= 64 || p.kv_len >= 512) && attention_tc_ok(p)) return attention_tc(c, p, s);
     if (p.type == WOCR_F32) launch_type<float>(c, p, s);
     else if (p.type == WOCR_F16) launch_type<__half>(c, p, s);
     else launch_type<__nv_bfloat16>(c, p, s);

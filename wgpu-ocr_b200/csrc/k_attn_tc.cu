@@ -1,8 +1,9 @@
 // Attention of many queries over 16-bit keys and values on the tensor cores: tcgen05 with scores,
 // weights and sums in tensor memory, tiles fed by TMA.
 //
-// A block takes 256 queries of one head as two tiles of 128 (one tensor-memory lane each) and walks
-// the keys in tiles of 128.  Roles:
+// A block takes NT tiles of 128 queries of one head (one tensor-memory lane each) and walks the keys in
+// tiles of 128: two tiles, or, for short sequences of heads of up to 64 dimensions, one, with two
+// blocks on an SM, which hide each other's start and end as well.  Roles (of two tiles):
 //   warps 0-3, 4-7  softmax of query tile 0 and 1, a thread per row: scores from tensor memory, mask,
 //                   running maximum and sum, weights back into tensor memory as the left operand of
 //                   the second product, in the columns of the scores they came from
@@ -30,28 +31,26 @@ namespace {
 using namespace attn;
 using namespace tc;
 
-constexpr int kThreads = 384, kMmaWarp = 8, kTmaWarp = 9;  // 10 and 11 fill the warpgroup
 // registers: softmax warps hold a row's 128 scores; 256 x 192 + 128 x 120 = 384 x 168, what the block has
 // (224 and 56 left the issuing warp 15 % of the kernel's time in spills)
 constexpr int kSoftmaxRegs = 192, kIssueRegs = 120;
 constexpr int kMaxTiles = 8192;              // key tiles of a call (2^20 keys): their bits fit in shared memory
 constexpr int kWords = kMaxTiles / 32;
 constexpr float kSlack = 8.f;                // growth of a maximum (log 2) that leaves the sums alone
-constexpr uint32_t kColS = 0, kColO = 256;   // tensor-memory columns: two score tiles, two sums of 128
 
-template <int DP>
+template <int DP, int NT>
 struct Smem {
     static constexpr int tile = 128 * DP * 2;
     // values first: a stage ends inside the block's shared memory whatever follows it
-    static constexpr int v = 0, k = v + 2 * tile, q = k + 2 * tile, bits = q + 2 * tile, docs = bits + 4 * kWords * 4,
-                         bars = docs + 8 * 128 * 4, bytes = bars + 256 + 1024;  // 1,024: alignment of the start
+    static constexpr int v = 0, k = v + 2 * tile, q = k + 2 * tile, bits = q + NT * tile, docs = bits + 2 * NT * kWords * 4,
+                         bars = docs + 4 * NT * 128 * 4, bytes = bars + 256 + 1024;  // 1,024: alignment of the start
 };
 
 struct TcArgs {
     AttnP a;
     int *status;
     long long budget;
-    int tiles, vec_out;  // query tile pairs of a head; rows of out take 16-byte stores
+    int tiles, vec_out;  // blocks of a head; rows of out take 16-byte stores
 };
 
 // kind::f16, D fp32, M = 128; B is K-major (scores) or N-major (values: dimensions contiguous)
@@ -165,16 +164,20 @@ __device__ __forceinline__ bool elect() {  // one lane of the warp, always the s
 // EXTRA: scores that are more than a plain product (capped, biased by distance, a scale that is not
 // positive), or documents.  Apart, since their code, unrolled over a row, cost plain tiles 15 % in
 // the instruction caches.
-template <typename T, int DP, bool EXTRA>
-__global__ void __launch_bounds__(kThreads, 1)
+constexpr int threads_of(int nt) { return nt == 2 ? 384 : 192; }
+
+template <typename T, int DP, int NT, bool EXTRA>
+__global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     k_attn_tc(const __grid_constant__ TcArgs ta, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv) {
-    using L = Smem<DP>;
+    using L = Smem<DP, NT>;
+    constexpr int kThreads = threads_of(NT), kMmaWarp = 4 * NT, kTmaWarp = kMmaWarp + 1;  // (NT 2: two more fill the warpgroup)
+    constexpr uint32_t kColS = 0, kColO = NT * 128, kCols = NT * 256;  // tensor-memory columns: scores, sums
     constexpr int kPanels = DP / 64, kPanel = 128 * 128;  // 64 dimensions of 128 rows
     extern __shared__ uint8_t raw[];
     uint8_t *sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const AttnP &p = ta.a;
-    uint32_t *act = (uint32_t *)(sm + L::bits), *full = act + 2 * kWords;  // per query tile: key tiles to visit, without masks
+    uint32_t *act = (uint32_t *)(sm + L::bits), *full = act + NT * kWords;  // per query tile: key tiles to visit, without masks
     int *docs = (int *)(sm + L::docs);
     uint64_t *bars = (uint64_t *)(sm + L::bars);
     uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
@@ -188,12 +191,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tile = ta.tiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
     const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kv_heads);
     const Span sp = span_of(p, b);
-    const int i_first = tile * 256;
+    const int i_first = tile * 128 * NT;
     if (i_first >= sp.nq) return;
     // keys that the first and the last row of each query tile may see
-    int emin[2], emax[2];
+    int emin[2] = {0, 0}, emax[2] = {0, 0};
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
+    for (int t = 0; t < NT; t++) {
         const int a = i_first + t * 128, z = min(a + 127, sp.nq - 1);
         emin[t] = a < sp.nq ? max(key_end(p, sp, a), 0) : 0;
         emax[t] = a < sp.nq ? max(key_end(p, sp, z), 0) : 0;
@@ -207,16 +210,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_async_smem();
     }
     if (warp == kMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     const int my = warp >> 2;  // softmax: the thread's query tile and row
     const int i = i_first + my * 128 + (tid & 127);
-    const bool row = warp < 8 && i < sp.nq;
+    const bool row = warp < kMmaWarp && i < sp.nq;
     int doc = -1;
     const bool by_doc = EXTRA && p.q_docs != nullptr;
     if (by_doc) {
-        for (int w = tid; w < 4 * kWords; w += kThreads) act[w] = 0;
+        for (int w = tid; w < 2 * NT * kWords; w += kThreads) act[w] = 0;
         __syncthreads();
         if (row) doc = p.q_docs[b * p.qds + i];
         if (warp < kMmaWarp) {
@@ -228,27 +231,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncthreads();
-        // a key tile's documents against the query tiles': none shared, all the same, or some
-        for (int j = warp; j < ntiles; j += kThreads / 32) {
-            int lo = 0x7fffffff, hi = -1;
-            bool odd = false;
+        // a key tile's documents against the query tiles': none shared, all the same, or some; four key
+        // tiles of a warp at a time, their loads under way together
+        const int *ids = p.kv_docs + b * p.kds;
+        for (int j0 = warp * 4; j0 < ntiles; j0 += kThreads / 32 * 4) {
+            int d[4][4];
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int key = j * 128 + x * 32 + lane;
-                const int d = key < sp.nk ? p.kv_docs[b * p.kds + key] : -1;
-                if (d >= 0) lo = min(lo, d), hi = max(hi, d);
-                else odd = true;
-            }
-            lo = __reduce_min_sync(0xffffffffu, lo);
-            hi = __reduce_max_sync(0xffffffffu, hi);
-            odd = __any_sync(0xffffffffu, odd);
-            if (lane == 0)
-                for (int t = 0; t < 2; t++) {
-                    const int ql = max(lim[2 * t], 0), qh = lim[2 * t + 1];
-                    if (j * 128 < emax[t] && lo <= qh && hi >= ql) atomicOr(&act[t * kWords + j / 32], 1u << (j & 31));
-                    if (!odd && lo == hi && lim[2 * t] == lo && qh == lo && (j + 1) * 128 <= emin[t])
+            for (int y = 0; y < 4; y++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int key = (j0 + y) * 128 + x * 32 + lane;
+                    d[y][x] = key < sp.nk ? ids[key] : -1;
+                }
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int j = j0 + y;
+                int lo = 0x7fffffff, hi = -1;
+                bool odd = false;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    odd |= d[y][x] < 0;
+                    if (d[y][x] >= 0) lo = min(lo, d[y][x]);
+                    hi = max(hi, d[y][x]);
+                }
+                lo = __reduce_min_sync(0xffffffffu, lo);
+                hi = __reduce_max_sync(0xffffffffu, hi);
+                odd = __any_sync(0xffffffffu, odd);
+                if (lane < NT && j < ntiles) {
+                    const int t = lane, ql = max(lim[2 * t], 0), qh = lim[2 * t + 1];
+                    if (j * 128 < (t ? emax[1] : emax[0]) && lo <= qh && hi >= ql) atomicOr(&act[t * kWords + j / 32], 1u << (j & 31));
+                    if (!odd && lo == hi && lim[2 * t] == lo && qh == lo && (j + 1) * 128 <= (t ? emin[1] : emin[0]))
                         atomicOr(&full[t * kWords + j / 32], 1u << (j & 31));
                 }
+            }
         }
     }
     tc_fence_before();
@@ -260,18 +275,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // the next key tile from j on that is visited by the query tiles of `tiles` (bits), which reach to key e
     auto next = [&](int tiles, int e, int j) -> int {
-        if (!by_doc) return j * 128 < e ? j : ntiles;
-        for (; j < ntiles; j = (j | 31) + 1) {
-            const uint32_t w = ((tiles & 1 ? act[j / 32] : 0) | (tiles & 2 ? act[kWords + j / 32] : 0)) >> (j & 31);
-            if (w) return j + __ffs(w) - 1;
-        }
-        return ntiles;
+        if constexpr (EXTRA)
+            if (by_doc) {
+                for (; j < ntiles; j = (j | 31) + 1) {
+                    const uint32_t w = ((tiles & 1 ? act[j / 32] : 0) | (NT == 2 && tiles & 2 ? act[kWords + j / 32] : 0)) >> (j & 31);
+                    if (w) return j + __ffs(w) - 1;
+                }
+                return ntiles;
+            }
+        return j * 128 < e ? j : ntiles;
     };
     const int ends = max(emax[0], emax[1]);
 
     if (warp >= kMmaWarp) {
     // (a warpgroup changes its registers as one)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (warp == kTmaWarp) {
         const uint32_t qbytes = 128 * DP * 2;
         bool any = false;
@@ -285,8 +303,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool edge = sp.nk < (j + 1) * 128 && sp.nk < p.kv_len;
             if (lane == 0) {
                 if (!any) {
-                    mbar_expect_tx(q_full, 2 * qbytes);
-                    for (int t = 0; t < 2; t++)
+                    mbar_expect_tx(q_full, NT * qbytes);
+                    for (int t = 0; t < NT; t++)
                         for (int x = 0; x < kPanels; x++)
                             tma_load_4d(sm + L::q + t * L::tile + x * kPanel, &mq, q_full, x * 64, i_first + t * 128, h, b);
                     any = true;
@@ -386,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < NT; t++) {
                 product(t);
                 if (!ok) break;
                 if (!(t ? v1 : v0)) continue;
@@ -412,19 +430,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < NT; t++) {
             product(t);
             if (elect()) umma_commit(&o_full[t]);
             __syncwarp();
         }
         const long long t0 = clock64();
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < NT; t++)
             while (!mbar_try(&o_full[t], 0) && clock64() - t0 < ta.budget) {
             }
         __syncwarp();
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 tensor-memory lanes
         const uint32_t ts = tmem + lanes + kColS + my * 128, to = tmem + lanes + kColO + my * 128;
         const bool live = row && (!by_doc || doc >= 0);
@@ -601,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
     }
 }
 
@@ -621,11 +639,12 @@ void make_map(CUtensorMap &m, bool bf16, const void *p, const int64_t *st, int b
     if (r != CUDA_SUCCESS) fail(WOCR_ERR_CUDA, "cuTensorMapEncodeTiled (attention) failed: " + std::to_string((int)r));
 }
 
-template <typename T, int DP, bool EXTRA>
-void launch(Ctx *c, const TcArgs &ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
-    const int bytes = Smem<DP>::bytes;
-    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tc<T, DP, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    k_attn_tc<T, DP, EXTRA><<<(unsigned)(ta.tiles * ta.a.batch * ta.a.heads), kThreads, bytes, s>>>(ta, mq, mk, mv);
+template <typename T, int DP, int NT, bool EXTRA>
+void launch(Ctx *c, TcArgs ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
+    const int bytes = Smem<DP, NT>::bytes;
+    ta.tiles = (ta.a.q_len + 128 * NT - 1) / (128 * NT);
+    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tc<T, DP, NT, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    k_attn_tc<T, DP, NT, EXTRA><<<(unsigned)(ta.tiles * ta.a.batch * ta.a.heads), threads_of(NT), bytes, s>>>(ta, mq, mk, mv);
     WOCR_LAUNCHED(c);
 }
 template <typename T>
@@ -633,18 +652,25 @@ void launch_dim(Ctx *c, const TcArgs &ta, const CUtensorMap &mq, const CUtensorM
     const AttnP &p = ta.a;
     const bool extra = p.cap > 0.f || p.slopes || !(p.scale > 0.f) || p.q_docs;
     if (p.dim <= 64) {
-        if (extra) launch<T, 64, true>(c, ta, mq, mk, mv, s);
-        else launch<T, 64, false>(c, ta, mq, mk, mv, s);
+        // one tile a block up to 1,024 queries: 128 sequences of 128 queries, 8 heads of 64: 26 us
+        // against 48; 16 of 1,024: 70 us both; 8 of 2,048: 121 us against 118
+        if (p.q_len <= 1024) {
+            if (extra) launch<T, 64, 1, true>(c, ta, mq, mk, mv, s);
+            else launch<T, 64, 1, false>(c, ta, mq, mk, mv, s);
+        } else {
+            if (extra) launch<T, 64, 2, true>(c, ta, mq, mk, mv, s);
+            else launch<T, 64, 2, false>(c, ta, mq, mk, mv, s);
+        }
     } else {
-        if (extra) launch<T, 128, true>(c, ta, mq, mk, mv, s);
-        else launch<T, 128, false>(c, ta, mq, mk, mv, s);
+        if (extra) launch<T, 128, 2, true>(c, ta, mq, mk, mv, s);
+        else launch<T, 128, 2, false>(c, ta, mq, mk, mv, s);
     }
 }
 }  // namespace
 
 bool attention_tc_ok(const AttnP &p) {
     if (p.type == WOCR_F32 || p.dim % 8 || p.dim > 128 || p.kv_len < 1) return false;
-    if (p.kv_len > kMaxTiles * 128 || (int64_t)p.batch * p.heads * ((p.q_len + 255) / 256) > 0x7fffffff) return false;
+    if (p.kv_len > kMaxTiles * 128 || (int64_t)p.batch * p.heads * ((p.q_len + 127) / 128) > 0x7fffffff) return false;
     // TMA: 16-byte rows, at most 2^40 bytes apart, and no broadcast dimension
     auto fits = [](const void *x, const int64_t *st, int batch, int heads, int tokens) {
         const int n[3] = {batch, heads, tokens};
@@ -663,7 +689,6 @@ void attention_tc(Ctx *c, const AttnP &p, cudaStream_t s) {
     ta.a = p;
     ta.status = c->status;
     ta.budget = kWaitBudget;
-    ta.tiles = (p.q_len + 255) / 256;
     ta.vec_out = (uintptr_t)p.o % 16 == 0 && p.os[0] % 8 == 0 && p.os[1] % 8 == 0 && p.os[2] % 8 == 0;
     CUtensorMap mq, mk, mv;
     make_map(mq, bf, p.q, p.qs, p.batch, p.heads, p.q_len, p.dim);
