@@ -44,12 +44,16 @@ __device__ __forceinline__ int key_end(const AttnP &p, const Span &s, int i) {
 // cap tanh(y / cap) in units of log 2.  A score's error is a relative error of its weight: with
 // 32-bit values tanhf (within 2 ulp), with 16-bit values 1 - 2 / (1 + e^2y) from two approximate
 // instructions (within 2^-21).
+static __device__ __noinline__ float capped32(float y, float cap) { return cap * tanhf(y / cap) * kLog2e; }
 template <typename T>
 __device__ __forceinline__ float capped2(float y, float cap) {
+    if (sizeof(T) == 4) return capped32(y, cap);  // a call: inlined over a tile it fills the instruction caches
     y /= cap;
-    if (sizeof(T) == 4) return cap * tanhf(y) * kLog2e;
     return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + ex2(fminf(y * (2.f * kLog2e), 126.f))));
 }
+// Scores that are more than a product, or documents: kernels are built with and without them, since
+// the code of all of them together, unrolled over a tile, does not fit in the instruction caches.
+inline bool extra_scores(const AttnP &p) { return p.cap > 0.f || p.slopes || p.q_docs; }
 // A score in units of log 2 from the dot product: cap tanh(scale dot / cap) (or scale dot) less
 // slope |distance|.
 template <typename T>

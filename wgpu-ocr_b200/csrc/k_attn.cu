@@ -98,7 +98,7 @@ __device__ __forceinline__ void mma_parts(float (&c)[4], const uint32_t (&a)[N][
 // r: head r / q_len, query r % q_len), and each a quarter of a tile's keys; otherwise 64 queries of
 // one head, 16 to a warp.  A cluster's blocks share the keys out tile by tile; partial
 // results are joined in shared memory.
-template <typename T, int DP, bool FEW>
+template <typename T, int DP, bool FEW, bool EXTRA>
 __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ AttnP p, int vec) {
     using S = TileSmem<T, DP>;
     using E = typename Parts<T>::E;
@@ -178,10 +178,10 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
         int e = min(i0 >= 0 ? e0 : 0x7fffffff, i1 >= 0 ? e1 : 0x7fffffff);
         all = __reduce_min_sync(0xffffffffu, e);
     }
-    const float sl0 = p.slopes ? p.slopes[row_head(r0)] * kLog2e : 0.f;
-    const float sl1 = p.slopes ? p.slopes[row_head(r1)] * kLog2e : 0.f;
-    const int d0 = p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
-    const int *kd = p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
+    const float sl0 = EXTRA && p.slopes ? p.slopes[row_head(r0)] * kLog2e : 0.f;
+    const float sl1 = EXTRA && p.slopes ? p.slopes[row_head(r1)] * kLog2e : 0.f;
+    const int d0 = EXTRA && p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = EXTRA && p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
+    const int *kd = EXTRA && p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
     const int pos0 = sp.off + i0, pos1 = sp.off + i1;
     const float scale2 = p.scale * kLog2e;
     float acc[DP / 8][4];
@@ -278,14 +278,14 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
             for (int x = 0; x < 2; x++) {
                 const int j = jw + n * 8 + (lane & 3) * 2 + x;
                 float u = s[n][x], w = s[n][2 + x];
-                if (p.cap > 0.f) {
+                if (EXTRA && p.cap > 0.f) {
                     u = capped2<T>(u * p.scale, p.cap);
                     w = capped2<T>(w * p.scale, p.cap);
                 } else {
                     u *= scale2;
                     w *= scale2;
                 }
-                if (p.slopes) {
+                if (EXTRA && p.slopes) {
                     u -= sl0 * fabsf((float)(pos0 - j));
                     w -= sl1 * fabsf((float)(pos1 - j));
                 }
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
 // weights' keys hold dimensions DP / 8 (lane / 4) .., paired by byte permutes.  No shared memory or
 // barrier until the parts are joined; keys of the next 16 are loaded while the softmax of these runs.
 // Bound: the keys' and values' bytes.  16 rows of the queries of all heads that share a key head.
-template <typename T, int DP>
+template <typename T, int DP, bool EXTRA>
 __global__ void __launch_bounds__(128) k_attn_token(const __grid_constant__ AttnP p) {
     constexpr int C = DP / 32, VW = DP / 64;  // 32-dimension chunks; 16-byte words of a value row per thread
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -449,9 +449,9 @@ __global__ void __launch_bounds__(128) k_attn_token(const __grid_constant__ Attn
         q0[c] = i0 >= 0 && d < p.dim ? *(const uint4 *)(qb + row_head(g) * p.qs[1] + (int64_t)i0 * p.qs[2] + d) : none;
         q1[c] = i1 >= 0 && d < p.dim ? *(const uint4 *)(qb + row_head(g + 8) * p.qs[1] + (int64_t)i1 * p.qs[2] + d) : none;
     }
-    const float sl0 = p.slopes ? p.slopes[row_head(g)] * kLog2e : 0.f, sl1 = p.slopes ? p.slopes[row_head(g + 8)] * kLog2e : 0.f;
-    const int d0 = p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
-    const int *kd = p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
+    const float sl0 = EXTRA && p.slopes ? p.slopes[row_head(g)] * kLog2e : 0.f, sl1 = EXTRA && p.slopes ? p.slopes[row_head(g + 8)] * kLog2e : 0.f;
+    const int d0 = EXTRA && p.q_docs && i0 >= 0 ? p.q_docs[b * p.qds + i0] : 0, d1 = EXTRA && p.q_docs && i1 >= 0 ? p.q_docs[b * p.qds + i1] : 0;
+    const int *kd = EXTRA && p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
     const int pos0 = sp.off + i0, pos1 = sp.off + i1;
     const float scale2 = p.scale * kLog2e;
     const T *kb = (const T *)p.k + b * p.ks[0] + hk * p.ks[1] + q4 * 8;
@@ -507,14 +507,14 @@ __global__ void __launch_bounds__(128) k_attn_token(const __grid_constant__ Attn
             for (int x = 0; x < 2; x++) {
                 const int j = j0 + t * 8 + q4 * 2 + x;
                 float u = s[t][x], w = s[t][2 + x];
-                if (p.cap > 0.f) {
+                if (EXTRA && p.cap > 0.f) {
                     u = capped2<T>(u * p.scale, p.cap);
                     w = capped2<T>(w * p.scale, p.cap);
                 } else {
                     u *= scale2;
                     w *= scale2;
                 }
-                if (p.slopes) {
+                if (EXTRA && p.slopes) {
                     u -= sl0 * fabsf((float)(pos0 - j));
                     w -= sl1 * fabsf((float)(pos1 - j));
                 }
@@ -611,7 +611,8 @@ void launch_tiles(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
     const int64_t units = (int64_t)p.batch * (FEW ? p.kv_heads : p.heads);
     const int tiles = FEW ? (p.heads / p.kv_heads * p.q_len + 15) / 16 : (p.q_len + 63) / 64;
     const int cs = key_split(c, units * tiles, 2, p.kv_len, 2 * S::BK);
-    launch_cluster<const AttnP, int>(k_attn_tiles<T, DP, FEW>, grid_of(units, cs, tiles), 128, cs, S::bytes, s, p, vec);
+    auto kernel = extra_scores(p) ? k_attn_tiles<T, DP, FEW, true> : k_attn_tiles<T, DP, FEW, false>;
+    launch_cluster<AttnP, int>(kernel, grid_of(units, cs, tiles), 128, cs, S::bytes, s, p, vec);
     WOCR_LAUNCHED(c);
 }
 
@@ -620,7 +621,8 @@ void launch_token(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int64_t units = (int64_t)p.batch * p.kv_heads;
     const int tiles = (p.heads / p.kv_heads * p.q_len + 15) / 16;
     const int cs = key_split(c, units * tiles, 4, p.kv_len, 128);  // two blocks of 16 keys a warp
-    launch_cluster<const AttnP>(k_attn_token<T, DP>, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
+    auto kernel = extra_scores(p) ? k_attn_token<T, DP, true> : k_attn_token<T, DP, false>;
+    launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
     WOCR_LAUNCHED(c);
 }
 

@@ -650,7 +650,7 @@ void launch(Ctx *c, TcArgs ta, const CUtensorMap &mq, const CUtensorMap &mk, con
 template <typename T>
 void launch_dim(Ctx *c, const TcArgs &ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
     const AttnP &p = ta.a;
-    const bool extra = p.cap > 0.f || p.slopes || !(p.scale > 0.f) || p.q_docs;
+    const bool extra = extra_scores(p) || !(p.scale > 0.f);
     if (p.dim <= 64) {
         // one tile a block up to 1,024 queries: 128 sequences of 128 queries, 8 heads of 64: 26 us
         // against 48; 16 of 1,024: 70 us both; 8 of 2,048: 121 us against 118
