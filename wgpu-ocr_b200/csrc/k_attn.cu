@@ -600,6 +600,163 @@ __global__ void __launch_bounds__(128) k_attn_token(const __grid_constant__ Attn
     join_parts<T, DP, 4>(p, b, parts, js, row_head, row_query);
 }
 
+// A few queries over 32-bit keys and values, in 32-bit multiply-adds: eight lanes have a key, DP / 8
+// dimensions each, so a key's row is read in 128-byte pieces and its score takes three exchanges; a
+// warp's four groups of lanes go over keys of their own, two at a time, with running maxima and sums
+// of their own, joined at the end.  Bound: the keys' and values' bytes.  R rows of the queries of all
+// heads that share a key head.
+template <int DP, int R, bool EXTRA>
+__global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ AttnP p) {
+    constexpr int W = DP / 32, U = 2;  // 16-byte words of a key per lane; keys under way
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ JoinSmem js;
+    PartSums<DP> *parts = (PartSums<DP> *)dyn;
+    cg::cluster_group cl = cg::this_cluster();
+    const int cs = cl.num_blocks(), rank = cl.block_rank();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 3, e = lane & 7;
+    const int group = p.heads / p.kv_heads, nrows = group * p.q_len, tile = blockIdx.y;
+    const int b = blockIdx.x / cs / p.kv_heads, hk = blockIdx.x / cs % p.kv_heads;
+    const Span sp = span_of(p, b);
+    auto row_head = [&](int r) { return hk * group + min(tile * R + r, nrows - 1) / p.q_len; };
+    auto row_query = [&](int r) {
+        const int i = (tile * R + r) % p.q_len;
+        return r < R && tile * R + r < nrows && i < sp.nq ? i : -1;
+    };
+    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 q[R][W], o[R][W];
+    float m[R], l[R], slope[R];
+    int end[R], pos[R], doc[R], last = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int i = row_query(r), h = row_head(r);
+        const float *qr = (const float *)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)i * p.qs[2];
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const int d = w * 32 + e * 4;
+            q[r][w] = o[r][w] = none;
+            if (i >= 0 && d < p.dim) q[r][w] = *(const float4 *)(qr + d);
+        }
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        end[r] = i >= 0 ? key_end(p, sp, i) : 0;
+        pos[r] = sp.off + i;
+        last = max(last, end[r]);
+        slope[r] = EXTRA && p.slopes ? p.slopes[h] : 0.f;
+        doc[r] = EXTRA && p.q_docs && i >= 0 ? p.q_docs[b * p.qds + i] : 0;
+    }
+    const float *kb = (const float *)p.k + b * p.ks[0] + hk * p.ks[1] + e * 4;
+    const float *vb = (const float *)p.v + b * p.vs[0] + hk * p.vs[1] + e * 4;
+    const int *kd = EXTRA && p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
+    const float scale2 = p.scale * kLog2e;
+    float4 kw[U][W], vw[U][W];
+    auto load = [&](float4(&x)[U][W], const float *base, int64_t stride, int j0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int j = j0 + u * 4;
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                x[u][w] = j < last && w * 32 + e * 4 < p.dim ? __ldg((const float4 *)(base + j * stride + w * 32)) : none;
+        }
+    };
+    const int step = cs * 16 * U;
+    int j0 = (rank * 4 + warp) * 4 * U + g;
+    load(kw, kb, p.ks[2], j0);
+    load(vw, vb, p.vs[2], j0);
+    for (int base = (rank * 4 + warp) * 4 * U; base < last; base += step, j0 += step) {
+        float s[U][R];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float x = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    x = fmaf(q[r][w].x, kw[u][w].x, x);
+                    x = fmaf(q[r][w].y, kw[u][w].y, x);
+                    x = fmaf(q[r][w].z, kw[u][w].z, x);
+                    x = fmaf(q[r][w].w, kw[u][w].w, x);
+                }
+                s[u][r] = x;
+            }
+        load(kw, kb, p.ks[2], j0 + step);
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2)
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int r = 0; r < R; r++) s[u][r] += __shfl_xor_sync(0xffffffffu, s[u][r], d);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float top = m[r];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int j = j0 + u * 4;
+                float x = EXTRA ? score2<float>(p, s[u][r], slope[r], pos[r] - j) : s[u][r] * scale2;
+                bool in = j < end[r];
+                if (kd) {
+                    const int d = j < sp.nk ? kd[j] : -1;
+                    in = in && d == doc[r] && d >= 0;
+                }
+                s[u][r] = in ? x : -INFINITY;
+                top = fmaxf(top, s[u][r]);
+            }
+            const float z = top == -INFINITY ? 0.f : top, c = ex2(m[r] - z);
+            m[r] = top;
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                s[u][r] = ex2(s[u][r] - z);
+                sum += s[u][r];
+            }
+            l[r] = fmaf(l[r], c, sum);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                float4 &a = o[r][w];
+                a.x *= c;
+                a.y *= c;
+                a.z *= c;
+                a.w *= c;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    a.x = fmaf(s[u][r], vw[u][w].x, a.x);
+                    a.y = fmaf(s[u][r], vw[u][w].y, a.y);
+                    a.z = fmaf(s[u][r], vw[u][w].z, a.z);
+                    a.w = fmaf(s[u][r], vw[u][w].w, a.w);
+                }
+            }
+        }
+        load(vw, vb, p.vs[2], j0 + step);
+    }
+    PartSums<DP> &pt = parts[warp];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float top = m[r];
+#pragma unroll
+        for (int d = 8; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float z = top == -INFINITY ? 0.f : top, c = ex2(m[r] - z);
+        float sum = l[r] * c;
+#pragma unroll
+        for (int d = 8; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            float4 a = make_float4(o[r][w].x * c, o[r][w].y * c, o[r][w].z * c, o[r][w].w * c);
+#pragma unroll
+            for (int d = 8; d < 32; d *= 2) {
+                a.x += __shfl_xor_sync(0xffffffffu, a.x, d);
+                a.y += __shfl_xor_sync(0xffffffffu, a.y, d);
+                a.z += __shfl_xor_sync(0xffffffffu, a.z, d);
+                a.w += __shfl_xor_sync(0xffffffffu, a.w, d);
+            }
+            if (g == 0) *(float4 *)&pt.o[r][w * 32 + e * 4] = a;
+        }
+        if (lane == 0) {
+            pt.m[r] = top;
+            pt.l[r] = sum;
+        }
+    }
+    join_parts<float, DP, 4>(p, b, parts, js, row_head, row_query);
+}
+
 dim3 grid_of(int64_t units, int cs, int64_t tiles) {
     if (units * cs > 0x7fffffff || tiles > 65535) fail(WOCR_ERR_UNSUPPORTED, "attention: too many heads or queries");
     return dim3((unsigned)(units * cs), (unsigned)tiles);
@@ -626,6 +783,23 @@ void launch_token(Ctx *c, const AttnP &p, cudaStream_t s) {
     WOCR_LAUNCHED(c);
 }
 
+template <int DP, int R>
+void launch_token32(Ctx *c, const AttnP &p, cudaStream_t s) {
+    const int64_t units = (int64_t)p.batch * p.kv_heads;
+    const int tiles = (p.heads / p.kv_heads * p.q_len + R - 1) / R;
+    const int cs = key_split(c, units * tiles, 4, p.kv_len, 64);  // two steps of a warp
+    auto kernel = extra_scores(p) ? k_attn_token32<DP, R, true> : k_attn_token32<DP, R, false>;
+    launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
+    WOCR_LAUNCHED(c);
+}
+template <int DP>
+void launch_token32(Ctx *c, const AttnP &p, cudaStream_t s) {
+    const int rows = p.heads / p.kv_heads * p.q_len;
+    if (rows == 1) launch_token32<DP, 1>(c, p, s);
+    else if (rows == 2) launch_token32<DP, 2>(c, p, s);
+    else launch_token32<DP, 4>(c, p, s);
+}
+
 // The queries of the heads that share a key head are taken together: a few tokens of a decoder.
 bool few_rows(const AttnP &p) { return p.q_len <= 16 && (int64_t)p.heads / p.kv_heads * p.q_len <= 64; }
 
@@ -644,6 +818,9 @@ void launch_type(Ctx *c, const AttnP &p, cudaStream_t s) {
     if constexpr (Parts<T>::n == 1)
         if (few_rows(p) && vec && p.dim % 8 == 0 && p.dim <= 128)
             return p.dim <= 64 ? launch_token<T, 64>(c, p, s) : launch_token<T, 128>(c, p, s);
+    if constexpr (Parts<T>::n == 3)
+        if (few_rows(p) && vec && p.dim % 4 == 0 && p.dim <= 128)
+            return p.dim <= 32 ? launch_token32<32>(c, p, s) : (p.dim <= 64 ? launch_token32<64>(c, p, s) : launch_token32<128>(c, p, s));
     if (p.dim <= 16) launch_dim<T, 16>(c, p, vec, s);
     else if (p.dim <= 32) launch_dim<T, 32>(c, p, vec, s);
     else if (p.dim <= 64) launch_dim<T, 64>(c, p, vec, s);
