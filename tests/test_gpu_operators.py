@@ -204,6 +204,19 @@ def test_attention_over_long_caches(gpu, type, TQ, TK, D):
     attention_check(gpu, q, k, v, causal=True, cap=20.0, slopes=torch.full((H,), 0.01, device="cuda"), kv_lens=i32([TQ, TK - 3]))
 
 
+@pytest.mark.parametrize("type, TQ, TK, D", [("f16", 20, 2500, 128), ("bf16", 150, 3300, 72), ("f16", 260, 1700, 64), ("bf16", 100, 900, 128)])
+@pytest.mark.parametrize("kind", ["", "prefix", "docs", "causal lens", "all"])
+def test_attention_with_keys_shared_out(gpu, kind, type, TQ, TK, D):
+    """Few query tiles over many keys: the blocks of a cluster each take some of the key tiles (none, for short rows)."""
+    B, H, HK = 2, 2, 1
+    q, k, v = qkv(B, H, HK, TQ, TK, D, type, 55)
+    attention_check(gpu, q, k, v, **masks(kind, B, H, TQ, TK))
+    v[0, 0, TK // 3] = float("inf")
+    k[1, 0, TK // 2, 0] = float("nan")
+    if kind == "causal lens":
+        attention_check(gpu, q, k, v, causal=True, kv_lens=i32([TK // 3, TK // 2 + TQ // 2]))
+
+
 @pytest.mark.parametrize("type", ["f16", "f32"])
 def test_attention_offsets_beyond_32_bits(gpu, type):
     """A head that starts more than 2^32 elements (f16) or bytes (f32) into the cache."""

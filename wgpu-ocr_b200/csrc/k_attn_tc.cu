@@ -11,6 +11,8 @@
 //                   other tile's products do, so the matrix pipe and the exponentials overlap
 //   warp 9          (one thread) TMA loads of queries, keys and values, two stages each
 //   warps 10, 11    help to look at documents before the loop
+// Where there are fewer blocks than SMs, a cluster's blocks share a query tile's keys out, tile by
+// tile, and join their sums through distributed shared memory.
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 since it was last used
 // (the weights stay below 2^8, the quotient is the same), so the accumulator is seldom touched
 // between products.
@@ -188,7 +190,9 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // long rows first: with a causal mask the last queries see the most keys
     const int heads = p.heads * p.batch;
-    const int tile = ta.tiles - 1 - blockIdx.x / heads, bh = blockIdx.x % heads;
+    cg::cluster_group cl = cg::this_cluster();
+    const int cs = cl.num_blocks(), rank = cl.block_rank(), unit = blockIdx.x / cs;
+    const int tile = ta.tiles - 1 - unit / heads, bh = unit % heads;
     const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kv_heads);
     const Span sp = span_of(p, b);
     const int i_first = tile * 128 * NT;
@@ -273,19 +277,23 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     const int whole = my == 0 ? emin[0] : emin[1], reach = my == 0 ? emax[0] : emax[1];  // of the thread's query tile
     auto visits = [&](int t, int e, int j) -> bool { return by_doc ? (act[t * kWords + j / 32] >> (j & 31)) & 1 : j * 128 < e; };
 
-    // the next key tile from j on that is visited by the query tiles of `tiles` (bits), which reach to key e
+    // the next key tile from j on that is this block's and is visited by the query tiles of `tiles` (bits), which reach to key e
     auto next = [&](int tiles, int e, int j) -> int {
         if constexpr (EXTRA)
             if (by_doc) {
                 for (; j < ntiles; j = (j | 31) + 1) {
-                    const uint32_t w = ((tiles & 1 ? act[j / 32] : 0) | (NT == 2 && tiles & 2 ? act[kWords + j / 32] : 0)) >> (j & 31);
+                    const uint32_t mine = cs == 8 ? 0x01010101u : cs == 4 ? 0x11111111u : cs == 2 ? 0x55555555u : ~0u;
+                    const uint32_t w = (((tiles & 1 ? act[j / 32] : 0) | (NT == 2 && tiles & 2 ? act[kWords + j / 32] : 0)) & mine << rank) >> (j & 31);
                     if (w) return j + __ffs(w) - 1;
                 }
                 return ntiles;
             }
+        j += (rank - j) & (cs - 1);
         return j * 128 < e ? j : ntiles;
     };
     const int ends = max(emax[0], emax[1]);
+    float row_m = -INFINITY, row_l = 0.f;  // a softmax thread's row
+    bool got = false;
 
     if (warp >= kMmaWarp) {
     // (a warpgroup changes its registers as one)
@@ -560,17 +568,80 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
         if (ok) ok = warp_wait(&o_full[my], 0, ta.status, stop, 49, ta.budget);
         if (ok) {
             tc_fence_after();
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            bool bad = !finite(l);
-            // rows through shared memory (the queries' tile is done with), 16-byte pieces XORed with the
-            // row against bank conflicts, so that a warp's stores cover whole rows
-            T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)(i - lane) * p.os[2];
-            uint8_t *stage = sm + L::q + my * L::tile + (warp & 3) * (L::tile / 4);
-            constexpr int kPieces = DP / 8;
+            if (cs == 1) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                bool bad = !finite(l);
+                // rows through shared memory (the queries' tile is done with), 16-byte pieces XORed with the
+                // row against bank conflicts, so that a warp's stores cover whole rows
+                T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)(i - lane) * p.os[2];
+                uint8_t *stage = sm + L::q + my * L::tile + (warp & 3) * (L::tile / 4);
+                constexpr int kPieces = DP / 8;
+#pragma unroll 1
+                for (int c0 = 0; c0 < p.dim; c0 += 32) {
+                    float f[32];
+                    if (n > 0) {
+                        tmem_ld32(to + c0, f);
+                        tmem_wait32(f);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 32; x++) f[x] = 0.f;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x++) {
+                        bad |= c0 + x < p.dim && !finite(f[x]);
+                        f[x] *= inv;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        *(uint4 *)(stage + lane * DP * 2 + ((c0 / 8 + x) ^ (lane & 7)) * 16) =
+                            make_uint4(pack2<T>(f[8 * x], f[8 * x + 1]), pack2<T>(f[8 * x + 2], f[8 * x + 3]),
+                                       pack2<T>(f[8 * x + 4], f[8 * x + 5]), pack2<T>(f[8 * x + 6], f[8 * x + 7]));
+                }
+                __syncwarp();
+                const int pieces = p.dim / 8, rows_left = sp.nq - (i - lane);
+#pragma unroll 4
+                for (int u = lane; u < 32 * kPieces; u += 32) {
+                    const int r = u / kPieces, c = u % kPieces;
+                    if (r >= rows_left || c >= pieces) continue;
+                    const uint4 v = *(const uint4 *)(stage + r * DP * 2 + (c ^ (r & 7)) * 16);
+                    T *at = o + r * p.os[2] + c * 8;
+                    if (ta.vec_out) {
+                        *(uint4 *)at = v;
+                    } else {
+                        const T *e = (const T *)&v;
+#pragma unroll
+                        for (int x = 0; x < 8; x++) at[x] = e[x];
+                    }
+                }
+                __syncwarp();
+                uint32_t rows = __ballot_sync(0xffffffffu, bad && row);
+                while (rows) {
+                    const int r = __ffs(rows) - 1;
+                    rows &= rows - 1;
+                    __syncwarp();
+                    row_by_warp<T>(p, b, h, i - lane + r);
+                }
+            }
+        }
+        got = ok && n > 0;
+        row_m = m;
+        row_l = l;
+        tc_fence_before();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (cs > 1) {
+        // every product and load of the block is done: values and keys make room for the sums, rows of
+        // 32-bit pieces of 16 bytes XORed with the row
+        tc_fence_after();
+        float *sums = (float *)sm, *ml = (float *)(sm + L::docs);
+        if (warp < kMmaWarp) {
+            const int r = my * 128 + (tid & 127);
+            const uint32_t to = tmem + ((uint32_t)(warp & 3) << 21) + kColO + my * 128;
 #pragma unroll 1
             for (int c0 = 0; c0 < p.dim; c0 += 32) {
                 float f[32];
-                if (n > 0) {
+                if (got) {
                     tmem_ld32(to + c0, f);
                     tmem_wait32(f);
                 } else {
@@ -578,45 +649,51 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
                     for (int x = 0; x < 32; x++) f[x] = 0.f;
                 }
 #pragma unroll
-                for (int x = 0; x < 32; x++) {
-                    bad |= c0 + x < p.dim && !finite(f[x]);
-                    f[x] *= inv;
-                }
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    *(uint4 *)(stage + lane * DP * 2 + ((c0 / 8 + x) ^ (lane & 7)) * 16) =
-                        make_uint4(pack2<T>(f[8 * x], f[8 * x + 1]), pack2<T>(f[8 * x + 2], f[8 * x + 3]),
-                                   pack2<T>(f[8 * x + 4], f[8 * x + 5]), pack2<T>(f[8 * x + 6], f[8 * x + 7]));
+                for (int x = 0; x < 8; x++)
+                    *(float4 *)(sums + r * DP + ((c0 / 4 + x) ^ (r & 7)) * 4) = make_float4(f[4 * x], f[4 * x + 1], f[4 * x + 2], f[4 * x + 3]);
             }
-            __syncwarp();
-            const int pieces = p.dim / 8, rows_left = sp.nq - (i - lane);
-#pragma unroll 4
-            for (int u = lane; u < 32 * kPieces; u += 32) {
-                const int r = u / kPieces, c = u % kPieces;
-                if (r >= rows_left || c >= pieces) continue;
-                const uint4 v = *(const uint4 *)(stage + r * DP * 2 + (c ^ (r & 7)) * 16);
-                T *at = o + r * p.os[2] + c * 8;
-                if (ta.vec_out) {
-                    *(uint4 *)at = v;
-                } else {
-                    const T *e = (const T *)&v;
-#pragma unroll
-                    for (int x = 0; x < 8; x++) at[x] = e[x];
-                }
-            }
-            __syncwarp();
-            uint32_t rows = __ballot_sync(0xffffffffu, bad && row);
-            while (rows) {
-                const int r = __ffs(rows) - 1;
-                rows &= rows - 1;
-                __syncwarp();
-                row_by_warp<T>(p, b, h, i - lane + r);
-            }
+            ml[2 * r] = row_m;
+            ml[2 * r + 1] = row_l;
         }
         tc_fence_before();
+        cl.sync();
+        // a warp per row, the rows shared out
+        for (int r = rank * (kThreads / 32) + warp; r < 128 * NT; r += cs * (kThreads / 32)) {
+            const int at = i_first + r;
+            if (at >= sp.nq) continue;
+            float top = -INFINITY, total = 0.f, share[8];
+            for (int c = 0; c < cs; c++) top = fmaxf(top, cl.map_shared_rank(ml, c)[2 * r]);
+            const float z = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+                share[c] = 0.f;
+                if (c >= cs) continue;
+                const float *of = cl.map_shared_rank(ml, c) + 2 * r;
+                share[c] = ex2(of[0] - z);
+                total = fmaf(share[c], of[1], total);
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            bool bad = !finite(total);
+            T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)at * p.os[2];
+            if (lane * 4 < p.dim) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    if (c >= cs) continue;
+                    const float4 x = *(const float4 *)(cl.map_shared_rank(sums, c) + r * DP + (lane ^ (r & 7)) * 4);
+                    const float f = share[c] * inv;
+                    v = make_float4(fmaf(f, x.x, v.x), fmaf(f, x.y, v.y), fmaf(f, x.z, v.z), fmaf(f, x.w, v.w));
+                }
+                bad |= !finite(v.x) || !finite(v.y) || !finite(v.z) || !finite(v.w);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[lane * 4 + x] = from_f<T>(e[x]);
+            }
+            __syncwarp();
+            if (__any_sync(0xffffffffu, bad)) row_by_warp<T>(p, b, h, at);
+        }
+        cl.sync();  // the sums are read until here
     }
-    tc_fence_before();
-    __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
@@ -643,8 +720,18 @@ template <typename T, int DP, int NT, bool EXTRA>
 void launch(Ctx *c, TcArgs ta, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t s) {
     const int bytes = Smem<DP, NT>::bytes;
     ta.tiles = (ta.a.q_len + 128 * NT - 1) / (128 * NT);
-    WOCR_CUDA(cudaFuncSetAttribute(k_attn_tc<T, DP, NT, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    k_attn_tc<T, DP, NT, EXTRA><<<(unsigned)(ta.tiles * ta.a.batch * ta.a.heads), threads_of(NT), bytes, s>>>(ta, mq, mk, mv);
+    const int64_t units = (int64_t)ta.tiles * ta.a.batch * ta.a.heads;
+    // while there is room on the GPU and a block keeps three key tiles (8 heads of 128, 20 queries over
+    // 4,096 keys: 55 us in one block a head)
+    int cs = 1;
+    while (cs < 8 && units * cs * 2 <= c->sm_count * (3 - NT) && ta.a.kv_len >= 2 * cs * 384) cs *= 2;
+    auto kernel = k_attn_tc<T, DP, NT, EXTRA>;
+    if (cs > 1) {
+        launch_cluster<TcArgs, CUtensorMap, CUtensorMap, CUtensorMap>(kernel, dim3((unsigned)(units * cs)), threads_of(NT), cs, bytes, s, ta, mq, mk, mv);
+    } else {
+        WOCR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        kernel<<<(unsigned)units, threads_of(NT), bytes, s>>>(ta, mq, mk, mv);
+    }
     WOCR_LAUNCHED(c);
 }
 template <typename T>
