@@ -165,10 +165,10 @@ __device__ __forceinline__ bool elect() {  // one lane of the warp, always the s
 
 // EXTRA: scores that are more than a plain product (capped, biased by distance, a scale that is not
 // positive), or documents.  Apart, since their code, unrolled over a row, cost plain tiles 15 % in
-// the instruction caches.
+// the instruction caches.  SPLIT: a cluster shares the keys out (its code costs the others 7 %).
 constexpr int threads_of(int nt) { return nt == 2 ? 384 : 192; }
 
-template <typename T, int DP, int NT, bool EXTRA>
+template <typename T, int DP, int NT, bool EXTRA, bool SPLIT>
 __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     k_attn_tc(const __grid_constant__ TcArgs ta, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     // long rows first: with a causal mask the last queries see the most keys
     const int heads = p.heads * p.batch;
     cg::cluster_group cl = cg::this_cluster();
-    const int cs = cl.num_blocks(), rank = cl.block_rank(), unit = blockIdx.x / cs;
+    const int cs = SPLIT ? cl.num_blocks() : 1, rank = SPLIT ? cl.block_rank() : 0, unit = blockIdx.x / cs;
     const int tile = ta.tiles - 1 - unit / heads, bh = unit % heads;
     const int b = bh / p.heads, h = bh % p.heads, hk = h / (p.heads / p.kv_heads);
     const Span sp = span_of(p, b);
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
                 }
                 return ntiles;
             }
-        j += (rank - j) & (cs - 1);
+        if (SPLIT) j += (rank - j) & (cs - 1);
         return j * 128 < e ? j : ntiles;
     };
     const int ends = max(emax[0], emax[1]);
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
         if (ok) ok = warp_wait(&o_full[my], 0, ta.status, stop, 49, ta.budget);
         if (ok) {
             tc_fence_after();
-            if (cs == 1) {
+            if (!SPLIT) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 bool bad = !finite(l);
                 // rows through shared memory (the queries' tile is done with), 16-byte pieces XORed with the
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     }
     tc_fence_before();
     __syncthreads();
-    if (cs > 1) {
+    if constexpr (SPLIT) {
         // every product and load of the block is done: values and keys make room for the sums, rows of
         // 32-bit pieces of 16 bytes XORed with the row
         tc_fence_after();
@@ -725,10 +725,11 @@ void launch(Ctx *c, TcArgs ta, const CUtensorMap &mq, const CUtensorMap &mk, con
     // 4,096 keys: 55 us in one block a head)
     int cs = 1;
     while (cs < 8 && units * cs * 2 <= c->sm_count * (3 - NT) && ta.a.kv_len >= 2 * cs * 384) cs *= 2;
-    auto kernel = k_attn_tc<T, DP, NT, EXTRA>;
     if (cs > 1) {
+        auto kernel = k_attn_tc<T, DP, NT, EXTRA, true>;
         launch_cluster<TcArgs, CUtensorMap, CUtensorMap, CUtensorMap>(kernel, dim3((unsigned)(units * cs)), threads_of(NT), cs, bytes, s, ta, mq, mk, mv);
     } else {
+        auto kernel = k_attn_tc<T, DP, NT, EXTRA, false>;
         WOCR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         kernel<<<(unsigned)units, threads_of(NT), bytes, s>>>(ta, mq, mk, mv);
     }
