@@ -85,13 +85,16 @@ __device__ __forceinline__ void copy_rows(uint16_t *dst, const T *src, int64_t s
     }
 }
 
-// The weights' products: part pairs (x, y) with x + y < the number of parts.
+// Products of parts (x, y) with x + y < the number of parts, the pair of leading parts into c and the
+// others into low: the matrix instruction cuts its sums off instead of rounding them, so the small
+// products do not go through the large sums (32-bit results over 400 keys were 1e-6 off with one sum).
 template <typename T, int N>
-__device__ __forceinline__ void mma_parts(float (&c)[4], const uint32_t (&a)[N][4], const uint32_t (&b0)[N], const uint32_t (&b1)[N]) {
+__device__ __forceinline__ void mma_parts(float (&c)[4], float (&low)[4], const uint32_t (&a)[N][4], const uint32_t (&b0)[N],
+                                          const uint32_t (&b1)[N]) {
 #pragma unroll
-    for (int y = N - 1; y >= 0; y--)  // the small products first
+    for (int y = N - 1; y >= 0; y--)
 #pragma unroll
-        for (int x = N - 1 - y; x >= 0; x--) mma16816<typename Parts<T>::E>(c, a[x], b0[y], b1[y]);
+        for (int x = N - 1 - y; x >= 0; x--) mma16816<typename Parts<T>::E>(x + y ? low : c, a[x], b0[y], b1[y]);
 }
 
 // Four warps.  FEW: all have the same 16 rows of the queries of all heads that share a key head (row
@@ -226,11 +229,11 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
             }
         }
         const int jw = j0 + (FEW ? warp * WK : 0), kw = FEW ? warp * WK : 0;
-        float s[NT][4];
+        float s[NT][4], low[P > 1 ? NT : 1][4];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) s[n][x] = 0.f;
+            for (int x = 0; x < 4; x++) s[n][x] = low[P > 1 ? n : 0][x] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             uint32_t a[P][4];
@@ -253,10 +256,10 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
                         ldsm4(bb[y], sk + (y * BK + kw + n * 8 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8);
 #pragma unroll
                     for (int y = 0; y < P; y++) b0[y] = bb[y][0], b1[y] = bb[y][1];
-                    mma_parts<T, P>(s[n], a, b0, b1);
+                    mma_parts<T, P>(s[n], low[P > 1 ? n : 0], a, b0, b1);
 #pragma unroll
                     for (int y = 0; y < P; y++) b0[y] = bb[y][2], b1[y] = bb[y][3];
-                    mma_parts<T, P>(s[n + 1], a, b0, b1);
+                    mma_parts<T, P>(s[n + 1], low[P > 1 ? n + 1 : 0], a, b0, b1);
                 }
             } else {
                 uint32_t b0[P], b1[P];
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
                     b0[y] = *reinterpret_cast<const uint32_t *>(at);
                     b1[y] = *reinterpret_cast<const uint32_t *>(at + 8);
                 }
-                mma_parts<T, P>(s[0], a, b0, b1);
+                mma_parts<T, P>(s[0], low[0], a, b0, b1);
             }
         }
         // scores in units of log 2, masked
@@ -278,6 +281,10 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
             for (int x = 0; x < 2; x++) {
                 const int j = jw + n * 8 + (lane & 3) * 2 + x;
                 float u = s[n][x], w = s[n][2 + x];
+                if constexpr (P > 1) {
+                    u += low[n][x];
+                    w += low[n][2 + x];
+                }
                 if (EXTRA && p.cap > 0.f) {
                     u = capped2<T>(u * p.scale, p.cap);
                     w = capped2<T>(w * p.scale, p.cap);
@@ -326,27 +333,35 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
                 l1 += s[n][2 + x];
             }
         }
+        // the weights as the left operand, 16 keys at a time, rounded to the parts (16-bit types: once,
+        // to the values' type, as the matrix instruction asks)
+        constexpr int KN = (NT + 1) / 2;
+        uint32_t a[KN][P][4];
 #pragma unroll
-        for (int n = 0; n < DP / 8; n++) {
-            acc[n][0] *= c0;
-            acc[n][1] *= c0;
-            acc[n][2] *= c1;
-            acc[n][3] *= c1;
-        }
-        // the weights as the left operand, 16 keys at a time, rounded to the parts (16-bit types:
-        // once, to the values' type, as the matrix instruction asks)
-#pragma unroll
-        for (int n = 0; n < (NT + 1) / 2; n++) {
-            uint32_t a[P][4], w[P];
+        for (int n = 0; n < KN; n++)
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int nt = 2 * n + (x >> 1);
+                uint32_t w[P];
                 if (nt < NT) split2<T>(s[nt < NT ? nt : 0][(x & 1) * 2], s[nt < NT ? nt : 0][(x & 1) * 2 + 1], w);
 #pragma unroll
-                for (int y = 0; y < P; y++) a[y][x] = nt < NT ? w[y] : 0u;
+                for (int y = 0; y < P; y++) a[n][y][x] = nt < NT ? w[y] : 0u;
             }
 #pragma unroll
-            for (int dn = 0; dn < DP / 16; dn++) {
+        for (int dn = 0; dn < DP / 16; dn++) {
+            // 32 bits: a tile's sums on their own, added to the row's in ordinary (rounded) arithmetic
+            float t[2][4], tl[2][4];
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                float (&o)[4] = acc[2 * dn + z];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    t[z][x] = P > 1 ? 0.f : o[x] * (x < 2 ? c0 : c1);
+                    tl[z][x] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < KN; n++) {
                 uint32_t bb[P][4], b0[P], b1[P];
                 // keys (lane & 15), dims 8 (lane >> 4); with 8 keys only, the upper half repeats the lower
                 const int key = kw + n * 16 + (NT == 1 ? lane & 7 : lane & 15);
@@ -354,10 +369,16 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
                 for (int y = 0; y < P; y++) ldsm4t(bb[y], sv + (y * BK + key) * LD + dn * 16 + (lane >> 4) * 8);
 #pragma unroll
                 for (int y = 0; y < P; y++) b0[y] = bb[y][0], b1[y] = bb[y][1];
-                mma_parts<T, P>(acc[2 * dn], a, b0, b1);
+                mma_parts<T, P>(t[0], tl[0], a[n], b0, b1);
 #pragma unroll
                 for (int y = 0; y < P; y++) b0[y] = bb[y][2], b1[y] = bb[y][3];
-                mma_parts<T, P>(acc[2 * dn + 1], a, b0, b1);
+                mma_parts<T, P>(t[1], tl[1], a[n], b0, b1);
+            }
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                float (&o)[4] = acc[2 * dn + z];
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[x] = P > 1 ? fmaf(o[x], x < 2 ? c0 : c1, t[z][x] + tl[z][x]) : t[z][x];
             }
         }
     }
