@@ -199,8 +199,8 @@ struct PartSums {
     float m[16], l[16];
 };
 struct JoinSmem {
-    float weight[64 * 32];  // a part's share of a row
-    uint8_t odd[64];        // rows whose sums are not finite
+    float weight[512], l[512];  // per part and row of the cluster: maximum, then share; sum
+    uint8_t odd[64];            // rows whose sums are not finite
 };
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
 
@@ -213,33 +213,44 @@ __device__ __forceinline__ void join_parts(const AttnP &p, int b, PartSums<DP> *
     cg::cluster_group cl = cg::this_cluster();
     const int cs = cl.num_blocks(), rank = cl.block_rank();
     cl.sync();
+    // the loads from other blocks go out together: one after another they take longer than the sums
+    const int n = cs * PER;  // parts of a row
+    for (int x = threadIdx.x; x < n * ROWS; x += 128) {
+        const int r = x % ROWS, c = x / ROWS / PER, w = PER == 4 ? x / ROWS % 4 : r / 16;
+        const PartSums<DP> &pt = cl.map_shared_rank(parts, c)[w];
+        js.weight[x] = pt.m[r % 16];
+        js.l[x] = pt.l[r % 16];
+    }
+    __syncthreads();
     if (threadIdx.x < ROWS) {
         const int r = threadIdx.x;
         float m = -INFINITY, l = 0.f;
         js.odd[r] = 0;
-        auto part = [&](int c, int w) -> const PartSums<DP> & { return cl.map_shared_rank(parts, c)[PER == 4 ? w : r / 16]; };
-        for (int c = 0; c < cs; c++)
-            for (int w = 0; w < PER; w++) m = fmaxf(m, part(c, w).m[r % 16]);
+        for (int x = 0; x < n; x++) m = fmaxf(m, js.weight[x * ROWS + r]);
         const float z = m == -INFINITY ? 0.f : m;
-        for (int c = 0; c < cs; c++)
-            for (int w = 0; w < PER; w++) {
-                const float f = ex2(part(c, w).m[r % 16] - z);
-                l += f * part(c, w).l[r % 16];
-                js.weight[(c * PER + w) * ROWS + r] = f;
-            }
+        for (int x = 0; x < n; x++) {
+            const float f = ex2(js.weight[x * ROWS + r] - z);
+            l += f * js.l[x * ROWS + r];
+            js.weight[x * ROWS + r] = f;
+        }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        for (int x = 0; x < cs * PER; x++) js.weight[x * ROWS + r] *= inv;
+        for (int x = 0; x < n; x++) js.weight[x * ROWS + r] *= inv;
     }
     __syncthreads();
     for (int u = rank * 128 + threadIdx.x; u < ROWS * DP; u += cs * 128) {
         const int r = u / DP, d = u % DP, i = query(r);
         if (i < 0 || d >= p.dim) continue;
-        float v = 0.f;
-        for (int c = 0; c < cs; c++) {
-            const PartSums<DP> *pc = cl.map_shared_rank(parts, c);
+        float of[8][PER], v = 0.f;
 #pragma unroll
-            for (int w = 0; w < PER; w++) v += js.weight[(c * PER + w) * ROWS + r] * pc[PER == 4 ? w : r / 16].o[r % 16][d];
-        }
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+            for (int w = 0; w < PER; w++)
+                of[c][w] = c < cs ? cl.map_shared_rank(parts, c)[PER == 4 ? w : r / 16].o[r % 16][d] : 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+#pragma unroll
+            for (int w = 0; w < PER; w++)
+                if (c < cs) v += js.weight[(c * PER + w) * ROWS + r] * of[c][w];
         if (!finite(v)) js.odd[r] = 1;
         ((T *)p.o)[b * p.os[0] + head(r) * p.os[1] + (int64_t)i * p.os[2] + d] = from_f<T>(v);
     }
@@ -248,12 +259,28 @@ __device__ __forceinline__ void join_parts(const AttnP &p, int b, PartSums<DP> *
         if (js.odd[r] && query(r) >= 0) row_by_warp<T>(p, b, head(r), query(r));
 }
 
-// Blocks of a cluster that share the keys of one unit of work: while the GPU has room and each
-// keeps `least` keys or more.
-inline int key_split(const Ctx *c, int64_t units, int per_sm, int kv_len, int least) {
-    int cs = 1;
-    while (cs < 8 && units * cs < (int64_t)per_sm * c->sm_count && kv_len >= 2 * cs * least) cs *= 2;
-    return cs;
+// Blocks of `kernel` that an SM holds at a time, or four: more do not read faster.
+template <typename K>
+inline int resident(K *kernel, int threads, size_t smem) {
+    int n = 0;
+    if (smem > 48 * 1024) WOCR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    WOCR_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem));
+    return n < 1 ? 1 : (n > 4 ? 4 : n);
+}
+// Blocks of a cluster that share the keys of one unit of work: the number whose rounds of blocks
+// (`per_sm` at a time on an SM) over its keys, and 512 keys' worth of beginning and joining, take
+// least (8,192 keys, 32 x 8 key heads, four rows: of 128, 208 us with one block a unit against 236 with
+// four; of 64, 123 us with four against 157 with eight).
+inline int key_split(const Ctx *c, int64_t units, int per_sm, int kv_len) {
+    constexpr int start = 512;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int cs = 1; cs <= 8; cs *= 2) {
+        const int64_t at_once = (int64_t)per_sm * c->sm_count, rounds = (units * cs + at_once - 1) / at_once;
+        const int64_t cost = rounds * ((kv_len + cs - 1) / cs + start);
+        if (cost < least) least = cost, best = cs;
+    }
+    return best;
 }
 template <typename... A>
 inline void launch_cluster(void (*kernel)(A...), dim3 grid, int threads, int cs, size_t smem, cudaStream_t s, A... args) {

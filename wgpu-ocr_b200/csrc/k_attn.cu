@@ -621,14 +621,31 @@ __global__ void __launch_bounds__(128) k_attn_token(const __grid_constant__ Attn
     join_parts<T, DP, 4>(p, b, parts, js, row_head, row_query);
 }
 
-// A few queries over 32-bit keys and values, in 32-bit multiply-adds: eight lanes have a key, DP / 8
-// dimensions each, so a key's row is read in 128-byte pieces and its score takes three exchanges; a
-// warp's four groups of lanes go over keys of their own, two at a time, with running maxima and sums
-// of their own, joined at the end.  Bound: the keys' and values' bytes.  R rows of the queries of all
-// heads that share a key head.
-template <int DP, int R, bool EXTRA>
-__global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ AttnP p) {
-    constexpr int W = DP / 32, U = 2;  // 16-byte words of a key per lane; keys under way
+// One query (32 bits: up to four), in 32-bit multiply-adds: eight lanes have a key, 16-byte words of it in turn, so
+// a key's row is read in 128-byte pieces and its score takes three exchanges; a warp's four groups of
+// lanes go over keys of their own, two at a time, with running maxima and sums of their own, joined at
+// the end.  Bound: the keys' and values' bytes (32 x 8,192 keys, 8 key heads of 128, four rows: 6.0 TB/s
+// in 32 bits).  R rows of the queries of all heads that share a key head.
+template <typename T>
+__device__ __forceinline__ void widen(const uint4 &w, float (&f)[16 / sizeof(T)]) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = __uint_as_float(x[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        } else {
+            f[2 * i] = __uint_as_float(x[i] << 16);
+            f[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+        }
+    }
+}
+template <typename T, int DP, int R, bool EXTRA>
+__global__ void __launch_bounds__(128) k_attn_row(const __grid_constant__ AttnP p) {
+    constexpr int E = 16 / sizeof(T), W = DP / (8 * E), U = 2;  // elements of a word; words of a key per lane; keys under way
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ JoinSmem js;
     PartSums<DP> *parts = (PartSums<DP> *)dyn;
@@ -643,19 +660,19 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
         const int i = (tile * R + r) % p.q_len;
         return r < R && tile * R + r < nrows && i < sp.nq ? i : -1;
     };
-    const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-    float4 q[R][W], o[R][W];
-    float m[R], l[R], slope[R];
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    float q[R][W][E], o[R][W][E], m[R], l[R], slope[R];
     int end[R], pos[R], doc[R], last = 0;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const int i = row_query(r), h = row_head(r);
-        const float *qr = (const float *)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)i * p.qs[2];
+        const T *qr = (const T *)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)i * p.qs[2];
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            const int d = w * 32 + e * 4;
-            q[r][w] = o[r][w] = none;
-            if (i >= 0 && d < p.dim) q[r][w] = *(const float4 *)(qr + d);
+            const int d = (w * 8 + e) * E;
+            widen<T>(i >= 0 && d < p.dim ? *(const uint4 *)(qr + d) : none, q[r][w]);
+#pragma unroll
+            for (int x = 0; x < E; x++) o[r][w][x] = 0.f;
         }
         m[r] = -INFINITY;
         l[r] = 0.f;
@@ -665,18 +682,18 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
         slope[r] = EXTRA && p.slopes ? p.slopes[h] : 0.f;
         doc[r] = EXTRA && p.q_docs && i >= 0 ? p.q_docs[b * p.qds + i] : 0;
     }
-    const float *kb = (const float *)p.k + b * p.ks[0] + hk * p.ks[1] + e * 4;
-    const float *vb = (const float *)p.v + b * p.vs[0] + hk * p.vs[1] + e * 4;
+    const T *kb = (const T *)p.k + b * p.ks[0] + hk * p.ks[1] + e * E;
+    const T *vb = (const T *)p.v + b * p.vs[0] + hk * p.vs[1] + e * E;
     const int *kd = EXTRA && p.kv_docs ? p.kv_docs + b * p.kds : nullptr;
     const float scale2 = p.scale * kLog2e;
-    float4 kw[U][W], vw[U][W];
-    auto load = [&](float4(&x)[U][W], const float *base, int64_t stride, int j0) {
+    uint4 kw[U][W], vw[U][W];
+    auto load = [&](uint4(&x)[U][W], const T *base, int64_t stride, int j0) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int j = j0 + u * 4;
 #pragma unroll
             for (int w = 0; w < W; w++)
-                x[u][w] = j < last && w * 32 + e * 4 < p.dim ? __ldg((const float4 *)(base + j * stride + w * 32)) : none;
+                x[u][w] = j < last && (w * 8 + e) * E < p.dim ? __ldg((const uint4 *)(base + j * stride + w * 8 * E)) : none;
         }
     };
     const int step = cs * 16 * U;
@@ -686,19 +703,19 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
     for (int base = (rank * 4 + warp) * 4 * U; base < last; base += step, j0 += step) {
         float s[U][R];
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < U; u++) {
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                float x = 0.f;
+            for (int r = 0; r < R; r++) s[u][r] = 0.f;
 #pragma unroll
-                for (int w = 0; w < W; w++) {
-                    x = fmaf(q[r][w].x, kw[u][w].x, x);
-                    x = fmaf(q[r][w].y, kw[u][w].y, x);
-                    x = fmaf(q[r][w].z, kw[u][w].z, x);
-                    x = fmaf(q[r][w].w, kw[u][w].w, x);
-                }
-                s[u][r] = x;
+            for (int w = 0; w < W; w++) {
+                float f[E];
+                widen<T>(kw[u][w], f);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int x = 0; x < E; x++) s[u][r] = fmaf(q[r][w][x], f[x], s[u][r]);
             }
+        }
         load(kw, kb, p.ks[2], j0 + step);
 #pragma unroll
         for (int d = 1; d < 8; d *= 2)
@@ -706,13 +723,14 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int r = 0; r < R; r++) s[u][r] += __shfl_xor_sync(0xffffffffu, s[u][r], d);
+        float c[R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             float top = m[r];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int j = j0 + u * 4;
-                float x = EXTRA ? score2<float>(p, s[u][r], slope[r], pos[r] - j) : s[u][r] * scale2;
+                const float x = EXTRA ? score2<T>(p, s[u][r], slope[r], pos[r] - j) : s[u][r] * scale2;
                 bool in = j < end[r];
                 if (kd) {
                     const int d = j < sp.nk ? kd[j] : -1;
@@ -721,7 +739,8 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
                 s[u][r] = in ? x : -INFINITY;
                 top = fmaxf(top, s[u][r]);
             }
-            const float z = top == -INFINITY ? 0.f : top, c = ex2(m[r] - z);
+            const float z = top == -INFINITY ? 0.f : top;
+            c[r] = ex2(m[r] - z);
             m[r] = top;
             float sum = 0.f;
 #pragma unroll
@@ -729,21 +748,22 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
                 s[u][r] = ex2(s[u][r] - z);
                 sum += s[u][r];
             }
-            l[r] = fmaf(l[r], c, sum);
+            l[r] = fmaf(l[r], c[r], sum);
+        }
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                float4 &a = o[r][w];
-                a.x *= c;
-                a.y *= c;
-                a.z *= c;
-                a.w *= c;
+        for (int w = 0; w < W; w++) {
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    a.x = fmaf(s[u][r], vw[u][w].x, a.x);
-                    a.y = fmaf(s[u][r], vw[u][w].y, a.y);
-                    a.z = fmaf(s[u][r], vw[u][w].z, a.z);
-                    a.w = fmaf(s[u][r], vw[u][w].w, a.w);
-                }
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int x = 0; x < E; x++) o[r][w][x] *= c[r];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float f[E];
+                widen<T>(vw[u][w], f);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int x = 0; x < E; x++) o[r][w][x] = fmaf(s[u][r], f[x], o[r][w][x]);
             }
         }
         load(vw, vb, p.vs[2], j0 + step);
@@ -754,28 +774,25 @@ __global__ void __launch_bounds__(128) k_attn_token32(const __grid_constant__ At
         float top = m[r];
 #pragma unroll
         for (int d = 8; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const float z = top == -INFINITY ? 0.f : top, c = ex2(m[r] - z);
-        float sum = l[r] * c;
+        const float z = top == -INFINITY ? 0.f : top, f = ex2(m[r] - z);
+        float sum = l[r] * f;
 #pragma unroll
         for (int d = 8; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            float4 a = make_float4(o[r][w].x * c, o[r][w].y * c, o[r][w].z * c, o[r][w].w * c);
+        for (int w = 0; w < W; w++)
 #pragma unroll
-            for (int d = 8; d < 32; d *= 2) {
-                a.x += __shfl_xor_sync(0xffffffffu, a.x, d);
-                a.y += __shfl_xor_sync(0xffffffffu, a.y, d);
-                a.z += __shfl_xor_sync(0xffffffffu, a.z, d);
-                a.w += __shfl_xor_sync(0xffffffffu, a.w, d);
+            for (int x = 0; x < E; x++) {
+                float a = o[r][w][x] * f;
+#pragma unroll
+                for (int d = 8; d < 32; d *= 2) a += __shfl_xor_sync(0xffffffffu, a, d);
+                if (g == 0) pt.o[r][(w * 8 + e) * E + x] = a;
             }
-            if (g == 0) *(float4 *)&pt.o[r][w * 32 + e * 4] = a;
-        }
         if (lane == 0) {
             pt.m[r] = top;
             pt.l[r] = sum;
         }
     }
-    join_parts<float, DP, 4>(p, b, parts, js, row_head, row_query);
+    join_parts<T, DP, 4>(p, b, parts, js, row_head, row_query);
 }
 
 dim3 grid_of(int64_t units, int cs, int64_t tiles) {
@@ -788,8 +805,9 @@ void launch_tiles(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
     using S = TileSmem<T, DP>;
     const int64_t units = (int64_t)p.batch * (FEW ? p.kv_heads : p.heads);
     const int tiles = FEW ? (p.heads / p.kv_heads * p.q_len + 15) / 16 : (p.q_len + 63) / 64;
-    const int cs = key_split(c, units * tiles, 2, p.kv_len, 2 * S::BK);
     auto kernel = extra_scores(p) ? k_attn_tiles<T, DP, FEW, true> : k_attn_tiles<T, DP, FEW, false>;
+    static const int per_sm = resident(k_attn_tiles<T, DP, FEW, false>, 128, S::bytes);
+    const int cs = key_split(c, units * tiles, per_sm, p.kv_len);
     launch_cluster<AttnP, int>(kernel, grid_of(units, cs, tiles), 128, cs, S::bytes, s, p, vec);
     WOCR_LAUNCHED(c);
 }
@@ -798,27 +816,31 @@ template <typename T, int DP>
 void launch_token(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int64_t units = (int64_t)p.batch * p.kv_heads;
     const int tiles = (p.heads / p.kv_heads * p.q_len + 15) / 16;
-    const int cs = key_split(c, units * tiles, 4, p.kv_len, 128);  // two blocks of 16 keys a warp
+    static const int per_sm = resident(k_attn_token<T, DP, false>, 128, 4 * sizeof(PartSums<DP>));
+    const int cs = key_split(c, units * tiles, per_sm, p.kv_len);
     auto kernel = extra_scores(p) ? k_attn_token<T, DP, true> : k_attn_token<T, DP, false>;
     launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
     WOCR_LAUNCHED(c);
 }
 
-template <int DP, int R>
-void launch_token32(Ctx *c, const AttnP &p, cudaStream_t s) {
+template <typename T, int DP, int R>
+void launch_row(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int64_t units = (int64_t)p.batch * p.kv_heads;
     const int tiles = (p.heads / p.kv_heads * p.q_len + R - 1) / R;
-    const int cs = key_split(c, units * tiles, 4, p.kv_len, 64);  // two steps of a warp
-    auto kernel = extra_scores(p) ? k_attn_token32<DP, R, true> : k_attn_token32<DP, R, false>;
+    static const int per_sm = resident(k_attn_row<T, DP, R, false>, 128, 4 * sizeof(PartSums<DP>));
+    const int cs = key_split(c, units * tiles, per_sm, p.kv_len);
+    auto kernel = extra_scores(p) ? k_attn_row<T, DP, R, true> : k_attn_row<T, DP, R, false>;
     launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
     WOCR_LAUNCHED(c);
 }
-template <int DP>
-void launch_token32(Ctx *c, const AttnP &p, cudaStream_t s) {
+template <typename T, int DP>
+void launch_row(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int rows = p.heads / p.kv_heads * p.q_len;
-    if (rows == 1) launch_token32<DP, 1>(c, p, s);
-    else if (rows == 2) launch_token32<DP, 2>(c, p, s);
-    else launch_token32<DP, 4>(c, p, s);
+    if constexpr (Parts<T>::n == 3) {
+        if (rows == 2) return launch_row<T, DP, 2>(c, p, s);
+        if (rows > 2) return launch_row<T, DP, 4>(c, p, s);
+    }
+    launch_row<T, DP, 1>(c, p, s);
 }
 
 // The queries of the heads that share a key head are taken together: a few tokens of a decoder.
@@ -837,11 +859,15 @@ void launch_type(Ctx *c, const AttnP &p, cudaStream_t s) {
     bool vec = ((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v) % 16 == 0;
     for (int i = 0; i < 3; i++) vec = vec && p.qs[i] % n == 0 && p.ks[i] % n == 0 && p.vs[i] % n == 0;
     if constexpr (Parts<T>::n == 1)
-        if (few_rows(p) && vec && p.dim % 8 == 0 && p.dim <= 128)
+        // (16 x 4,096 keys, 8 key heads of 128: two rows 62 us in this one, 77 in the row's; 32 x 8,192: one row
+        // 208 us in this one, 164 in the row's)
+        if (few_rows(p) && p.heads / p.kv_heads * p.q_len > 1 && vec && p.dim % 8 == 0 && p.dim <= 128)
             return p.dim <= 64 ? launch_token<T, 64>(c, p, s) : launch_token<T, 128>(c, p, s);
-    if constexpr (Parts<T>::n == 3)
-        if (few_rows(p) && vec && p.dim % 4 == 0 && p.dim <= 128)
-            return p.dim <= 32 ? launch_token32<32>(c, p, s) : (p.dim <= 64 ? launch_token32<64>(c, p, s) : launch_token32<128>(c, p, s));
+    if (few_rows(p) && vec && p.dim % n == 0 && p.dim <= 128) {
+        if constexpr (Parts<T>::n == 3)
+            if (p.dim <= 32) return launch_row<T, 32>(c, p, s);
+        return p.dim <= 64 ? launch_row<T, 64>(c, p, s) : launch_row<T, 128>(c, p, s);
+    }
     if (p.dim <= 16) launch_dim<T, 16>(c, p, vec, s);
     else if (p.dim <= 32) launch_dim<T, 32>(c, p, vec, s);
     else if (p.dim <= 64) launch_dim<T, 64>(c, p, vec, s);
