@@ -268,14 +268,14 @@ inline int resident(K *kernel, int threads, size_t smem) {
     return n < 1 ? 1 : (n > 4 ? 4 : n);
 }
 // Blocks of a cluster that share the keys of one unit of work: the number whose rounds of blocks
-// (`per_sm` at a time on an SM) over its keys, and 512 keys' worth of beginning and joining, take
+// (`per_sm` at a time on an SM, `step` keys at a time) over its keys, and 512 keys' worth of beginning and joining, take
 // least (8,192 keys, 32 x 8 key heads, four rows: of 128, 208 us with one block a unit against 236 with
 // four; of 64, 123 us with four against 157 with eight).
-inline int key_split(const Ctx *c, int64_t units, int per_sm, int kv_len) {
+inline int key_split(const Ctx *c, int64_t units, int per_sm, int kv_len, int step) {
     constexpr int start = 512;
     int best = 1;
     int64_t least = INT64_MAX;
-    for (int cs = 1; cs <= 8; cs *= 2) {
+    for (int cs = 1; cs <= 8 && (cs == 1 || kv_len >= cs * step); cs *= 2) {
         const int64_t at_once = (int64_t)per_sm * c->sm_count, rounds = (units * cs + at_once - 1) / at_once;
         const int64_t cost = rounds * ((kv_len + cs - 1) / cs + start);
         if (cost < least) least = cost, best = cs;

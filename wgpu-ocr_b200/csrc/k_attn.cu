@@ -807,7 +807,7 @@ void launch_tiles(Ctx *c, const AttnP &p, int vec, cudaStream_t s) {
     const int tiles = FEW ? (p.heads / p.kv_heads * p.q_len + 15) / 16 : (p.q_len + 63) / 64;
     auto kernel = extra_scores(p) ? k_attn_tiles<T, DP, FEW, true> : k_attn_tiles<T, DP, FEW, false>;
     static const int per_sm = resident(k_attn_tiles<T, DP, FEW, false>, 128, S::bytes);
-    const int cs = key_split(c, units * tiles, per_sm, p.kv_len);
+    const int cs = key_split(c, units * tiles, per_sm, p.kv_len, S::BK);
     launch_cluster<AttnP, int>(kernel, grid_of(units, cs, tiles), 128, cs, S::bytes, s, p, vec);
     WOCR_LAUNCHED(c);
 }
@@ -817,7 +817,7 @@ void launch_token(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int64_t units = (int64_t)p.batch * p.kv_heads;
     const int tiles = (p.heads / p.kv_heads * p.q_len + 15) / 16;
     static const int per_sm = resident(k_attn_token<T, DP, false>, 128, 4 * sizeof(PartSums<DP>));
-    const int cs = key_split(c, units * tiles, per_sm, p.kv_len);
+    const int cs = key_split(c, units * tiles, per_sm, p.kv_len, 64);
     auto kernel = extra_scores(p) ? k_attn_token<T, DP, true> : k_attn_token<T, DP, false>;
     launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
     WOCR_LAUNCHED(c);
@@ -828,7 +828,7 @@ void launch_row(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int64_t units = (int64_t)p.batch * p.kv_heads;
     const int tiles = (p.heads / p.kv_heads * p.q_len + R - 1) / R;
     static const int per_sm = resident(k_attn_row<T, DP, R, false>, 128, 4 * sizeof(PartSums<DP>));
-    const int cs = key_split(c, units * tiles, per_sm, p.kv_len);
+    const int cs = key_split(c, units * tiles, per_sm, p.kv_len, 32);
     auto kernel = extra_scores(p) ? k_attn_row<T, DP, R, true> : k_attn_row<T, DP, R, false>;
     launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
     WOCR_LAUNCHED(c);

@@ -22,15 +22,13 @@ constexpr int kGather = 2048;  // candidates a block gathers before it falls bac
 constexpr size_t kSmemMax = 227 * 1024;
 
 struct SelectSmem {
-    Cand lists[kWarps * 32];
+    Cand lists[32];
     Cand got[kGather];
     Cand top[kMaxBeams];                                     // the block's best, read by its cluster
     double base[kMaxBeams];                                  // score - log-sum-exp
     float wm[kMaxBeams][kWarps], ws[kMaxBeams][kWarps];      // per warp: maximum, sum of exponentials
     float bm[kMaxBeams], bs[kMaxBeams];                      // per block, read by its cluster
-    float least[kMaxBeams];                                  // logits below it cannot be among the best
     uint8_t fin[kMaxBeams];
-    Cand cut;
     int count;
 };
 
@@ -123,23 +121,14 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int sli
             if (better(c, best)) best = c;
         }
     }
-    const Cand sorted = block_best32<kWarps>(best, sm.lists);
-    if (warp == 0) {
-        const Cand cut = shfl(sorted, p.kout - 1);
-        if (lane == 0) sm.cut = cut;
-        if (lane < p.kin) {
-            // x must reach cut - base; rounded down, and a step more for the sum's own rounding
-            const double base = sm.base[lane];
-            float t = -INFINITY;
-            if (cut.v > -INFINITY) t = base > -INFINITY ? nextafterf(__double2float_rd(cut.v - base), -INFINITY) : INFINITY;
-            sm.least[lane] = t;
-        }
-    }
+    best_slots<kThreads>(best, tid, sm.lists);
     __syncthreads();
-    const Cand cut = sm.cut;
+    const Cand cut = kth_slot(sm.lists, p.kout);
     for (int j = 0; j < p.kin; j++) {
+        // x must reach cut - base; rounded down, and a step more for the sum's own rounding
         const double base = sm.base[j];
-        const float least = sm.least[j];
+        float least = -INFINITY;
+        if (cut.v > -INFINITY) least = base > -INFINITY ? nextafterf(__double2float_rd(cut.v - base), -INFINITY) : INFINITY;
 #pragma unroll 4
         for (int e = tid; e < n; e += kThreads) {
             const float x = at(j, e);

@@ -47,10 +47,9 @@ constexpr int kGather = 2048;
 constexpr size_t kSmemMax = 227 * 1024;
 
 struct RowSmem {
-    Key lists[kWarps * 32];
+    Key lists[32];
     Key got[kGather];
     Key top[32];
-    Key cut;
     float wm[kWarps];
     double ws[kWarps];
     int count;
@@ -83,16 +82,10 @@ __global__ void __launch_bounds__(kThreads) k_ctc_rows(const CtcP p, const Step 
     }
     for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if (lane == 0) sm.wm[warp] = m;
-    const Key sorted = block_best32<kWarps>(best, sm.lists);
+    best_slots<kThreads>(best, tid, sm.lists);
     if (tid < 32) sm.top[tid] = 0;
-    if (tid == 0) sm.cut = 0;
     __syncthreads();
-    if (warp == 0) {
-        const Key cut = shfl(sorted, K - 1);
-        if (lane == 0) sm.cut = cut;
-    }
-    __syncthreads();
-    const Key cut = sm.cut;
+    const Key cut = kth_slot(sm.lists, K);
     m = sm.wm[0];
     for (int w = 1; w < kWarps; w++) m = fmaxf(m, sm.wm[w]);
     float s = 0.f;
@@ -438,10 +431,9 @@ template <typename T, int N, int E>
 __global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_rows_reg(const CtcP p, const Step out, int K, int64_t rows) {
     constexpr int WARPS = N / 32, PER = N == 32 ? 8 : 1, GOT = 512;
     __shared__ struct {
-        Key lists[N];
+        Key lists[32];
         Key got[GOT];
         Key top[32];
-        Key cut;
         float wm[WARPS], ws[WARPS];
         int count;
     } smem[PER];
@@ -483,14 +475,10 @@ __global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_row
     const Key best = bv > -INFINITY ? make_key(bv, bk * N + tid) : 0;
     for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if (lane == 0) sm.wm[warp] = m;
-    const Key sorted = block_best32<WARPS>(best, sm.lists);
-    if (warp == 0) {
-        const Key cut = shfl(sorted, K - 1);
-        if (lane == 0) sm.cut = cut;
-        sm.top[lane] = 0;
-    }
+    best_slots<N>(best, tid, sm.lists);
+    if (warp == 0) sm.top[lane] = 0;
     sync();
-    const Key cut = sm.cut;
+    const Key cut = kth_slot(sm.lists, K);
     const float least = cut ? key_value(cut) : -INFINITY;
     m = sm.wm[0];
 #pragma unroll

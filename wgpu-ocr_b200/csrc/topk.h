@@ -1,4 +1,4 @@
-// The best of many, in order: keys kept one per lane, sorted and merged by a warp.
+// The best of many, in order: keys that compare as (value, place), and a bound of the k best.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -40,46 +40,26 @@ __device__ __forceinline__ float key_value(Key k) {
 }
 __device__ __forceinline__ uint32_t key_place(Key k) { return 0xffffffffu - (uint32_t)k; }
 
-// A warp's 32 keys in descending order by lane (Batcher's bitonic network).
-template <typename K>
-__device__ __forceinline__ K sort32(K a) {
-    const int lane = threadIdx.x & 31;
+// The best key of each of 32 groups of N threads (N / 32 lanes each), into slots[32] of shared memory:
+// the k-th best of them (kth_slot, after a barrier) has k - 1 keys of other groups before it, so it
+// bounds the k best keys of all N threads' values from below, and few others pass it.
+template <int N, typename K>
+__device__ __forceinline__ void best_slots(K a, int tid, K *slots) {
 #pragma unroll
-    for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-        for (int d = size / 2; d; d /= 2) {
-            const K o = shfl_xor(a, d);
-            const bool first = ((lane & d) == 0) == ((lane & size) == 0 || size == 32);
-            if (better(o, a) == first) a = o;
-        }
-    return a;
-}
-// The best 32 of two descending lists, descending.
-template <typename K>
-__device__ __forceinline__ K merge32(K a, K b) {
-    const int lane = threadIdx.x & 31;
-    b = shfl(b, 31 - lane);
-    if (better(b, a)) a = b;
-#pragma unroll
-    for (int d = 16; d; d /= 2) {
+    for (int d = 1; d < N / 32; d *= 2) {
         const K o = shfl_xor(a, d);
-        if (better(o, a) == ((lane & d) == 0)) a = o;
+        if (better(o, a)) a = o;
     }
-    return a;
+    if (tid % (N / 32) == 0) slots[tid / (N / 32)] = a;
 }
-// The best 32 of a block's keys (one per thread, WARPS warps), descending in lanes of warp 0;
-// lists: WARPS * 32 keys of shared memory, free again after the block's next barrier.
-template <int WARPS, typename K>
-__device__ __forceinline__ K block_best32(K a, K *lists) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    a = sort32(a);
-#pragma unroll
-    for (int n = WARPS / 2; n; n /= 2) {
-        if (warp >= n && warp < 2 * n) lists[warp * 32 + lane] = a;
-        __syncthreads();
-        if (warp < n) a = merge32(a, lists[(warp + n) * 32 + lane]);
-    }
-    return a;
+template <typename K>
+__device__ __forceinline__ K kth_slot(const K *slots, int k) {  // by a whole warp
+    const K mine = slots[threadIdx.x & 31];
+    int before = 0;
+#pragma unroll 8
+    for (int o = 0; o < 32; o++) before += better(slots[o], mine);
+    const uint32_t at = __ballot_sync(0xffffffffu, before == k - 1);
+    return at ? shfl(mine, __ffs(at) - 1) : worst((K *)nullptr);  // fewer than k groups have a key
 }
 
 // Logits and scores that are no number never win; an infinite one counts as the largest number.
