@@ -426,7 +426,9 @@ int32_t wocr_last_transfer_bytes(void *handle, int32_t kind, int64_t *h2d, int64
  * context's stream; cudaStreamLegacy for the legacy default stream) and may be captured into a
  * graph.  The calling thread's current device is left as it was.  Element types are ONNX
  * TensorProto codes; sums, weights and masses are held in 32 bits or more whatever the type, and
- * results are rounded once. */
+ * results are rounded once (16-bit attention also rounds each weight to the values' type, as the
+ * matrix instructions take it).  A bounded wait inside a kernel that gives up is reported by the
+ * context's next synchronising call (WOCR_ERR_TIMEOUT). */
 enum { WOCR_F32 = 1, WOCR_F16 = 10, WOCR_BF16 = 16 };
 
 /* Softmax attention over [batch, heads, tokens, head_dim] tensors of one type.  Strides in

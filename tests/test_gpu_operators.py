@@ -156,6 +156,25 @@ def test_attention_leaves_what_is_masked_alone(gpu, type, TQ, TK, D):
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("TQ", [1, 40, 200])
+def test_attention_of_scores_that_are_no_number(gpu, type, TQ):
+    """Capped scores: an infinite product is the cap, a NaN in sight is a NaN in the result, one behind a mask is not."""
+    q, k, v = qkv(1, 2, 2, TQ, 300, 64, type, 95)
+    q = q.abs() + 0.1
+    k[0, 0, 150] = float("nan")
+    k[0, 1, 20] = float("inf")
+    docs = torch.zeros((1, 300), dtype=torch.int32, device="cuda")
+    docs[0, 150] = 1
+    same = torch.zeros((1, TQ), dtype=torch.int32, device="cuda")
+    out = attention_check(gpu, q, k, v, cap=5.0)
+    assert torch.isnan(out[0, 0]).all() and torch.isfinite(out[0, 1]).all()
+    out = attention_check(gpu, q, k, v, cap=5.0, q_docs=same, kv_docs=docs)
+    assert torch.isfinite(out).all()
+    attention_check(gpu, q, k, v, scale=-0.2)
+    attention_check(gpu, q, k[:, :, 21:150], v[:, :, 21:150], scale=0.0)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("value", [30.0, -30.0, 1000.0, -1000.0])
 def test_attention_of_large_scores(gpu, type, value):
     """Scores far from zero and far apart: the running maximum decides, nothing overflows."""
@@ -187,11 +206,13 @@ def test_attention_layouts(gpu, type, D):
 
 
 def test_attention_of_nothing(gpu):
-    q, k, v = qkv(2, 2, 2, 3, 0, 16, "f32")
-    out = torch.full(q.shape, 7.0, device="cuda")
-    gpu.attention(q, k, v, out, stream=0)
-    torch.cuda.synchronize()
-    assert (out == 0).all()
+    for type in ("f16", "f32"):
+        for TQ in (1, 3, 40, 200):
+            q, k, v = qkv(2, 2, 2, TQ, 0, 16, type)
+            out = torch.full(q.shape, 7.0, device="cuda", dtype=q.dtype)
+            gpu.attention(q, k, v, out, stream=0)
+            torch.cuda.synchronize()
+            assert (out == 0).all()
     gpu.attention(q[:0], k[:0], v[:0], out[:0])
     gpu.attention(q[:, :, :0], k, v, out[:, :, :0])
 

@@ -119,6 +119,8 @@ def test_beam_reorder_refuses():
         reorder(dst=(1 << 20) + 4096)
     with pytest.raises(wocr.WocrError, match="more than 32"):
         reorder(m=33, n=33)
+    lib, state = wocr.lib(), __import__("struct").pack("2Q4q", 1 << 20, 1 << 30, 1 << 62, 16, 1 << 40, 1 << 40)
+    assert lib.wocr_beam_reorder(None, 4096, 2, 3, 3, state, 1, None) == 1 and b"64 bits" in lib.wocr_last_error()
     for kw in (dict(axis=4), dict(axis=-1), dict(axis=2, live=9), dict(axis=2, live=-1)):
         with pytest.raises(ValueError):
             reorder(**kw)

@@ -48,8 +48,9 @@ static __device__ __noinline__ float capped32(float y, float cap) { return cap *
 template <typename T>
 __device__ __forceinline__ float capped2(float y, float cap) {
     if (sizeof(T) == 4) return capped32(y, cap);  // a call: inlined over a tile it fills the instruction caches
-    y /= cap;
-    return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + ex2(fminf(y * (2.f * kLog2e), 126.f))));
+    y *= 2.f * kLog2e / cap;
+    if (y > 126.f) y = 126.f;  // (a NaN passes)
+    return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + ex2(y)));
 }
 // Scores that are more than a product, or documents: kernels are built with and without them, since
 // the code of all of them together, unrolled over a tile, does not fit in the instruction caches.

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     int stage = 0;
-    if (async) copy(rank * BK, 0);
+    if (async && rank * BK < last) copy(rank * BK, 0);
     else if (AHEAD && rank * BK < last) {
         nk.fetch(kb, p.ks[2], rank * BK, sp.nk, p.dim, vec);
         nv.fetch(vb, p.vs[2], rank * BK, sp.nk, p.dim, vec);

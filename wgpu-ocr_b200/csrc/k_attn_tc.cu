@@ -296,159 +296,159 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
     bool got = false;
 
     if (warp >= kMmaWarp) {
-    // (a warpgroup changes its registers as one)
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-    if (warp == kTmaWarp) {
-        const uint32_t qbytes = 128 * DP * 2;
-        bool any = false;
-        int it = 0;
-        bool ok = true;
-        for (int j = next(3, ends, 0); j < ntiles && ok; j = next(3, ends, j + 1)) {
-            const int s = it & 1;
-            const uint32_t par = (it >> 1) & 1;
-            uint8_t *sk = sm + L::k + s * L::tile, *sv = sm + L::v + s * L::tile;
-            // values behind the last key must be finite: they are multiplied by weights of zero
-            const bool edge = sp.nk < (j + 1) * 128 && sp.nk < p.kv_len;
-            if (lane == 0) {
-                if (!any) {
-                    mbar_expect_tx(q_full, NT * qbytes);
-                    for (int t = 0; t < NT; t++)
-                        for (int x = 0; x < kPanels; x++)
-                            tma_load_4d(sm + L::q + t * L::tile + x * kPanel, &mq, q_full, x * 64, i_first + t * 128, h, b);
-                    any = true;
-                }
-                ok = mbar_wait_spin(&k_empty[s], par ^ 1, ta.status, stop, 41, ta.budget);
-                if (ok) {
-                    mbar_expect_tx(&k_full[s], qbytes);
-                    for (int x = 0; x < kPanels; x++) tma_load_4d(sk + x * kPanel, &mk, &k_full[s], x * 64, j * 128, hk, b);
-                    ok = mbar_wait_spin(&v_empty[s], par ^ 1, ta.status, stop, 42, ta.budget);
-                }
-                if (ok) {
-                    uint64_t *bar = edge ? tail : &v_full[s];
-                    mbar_expect_tx(bar, qbytes);
-                    for (int x = 0; x < kPanels; x++) tma_load_4d(sv + x * kPanel, &mv, bar, x * 64, j * 128, hk, b);
-                    if (edge) ok = mbar_wait_spin(tail, 0, ta.status, stop, 43, ta.budget);  // the last tile: once
-                }
-            }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            __syncwarp();
-            if (edge && ok) {
-                const int from = sp.nk - j * 128;  // a row is 128 bytes of each panel, wherever the swizzle puts its pieces
-                for (int u = lane; u < (128 - from) * 8 * kPanels; u += 32) {
-                    const int x = u / ((128 - from) * 8), v = u % ((128 - from) * 8);
-                    *(uint4 *)(sv + x * kPanel + (from + v / 8) * 128 + (v % 8) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&v_full[s]);
-            }
-            it++;
-        }
-        if (lane == 0) {
-            // copies land before the block may exit, however it ends (bounded)
-            const long long t0 = clock64();
-            if (it > 0)
-                while (!mbar_try(q_full, 0) && clock64() - t0 < ta.budget) {
-                }
-            for (int j = it > 2 ? it - 2 : 0; j < it; j++)
-                for (uint64_t *bar : {&k_full[j & 1], &v_full[j & 1]})
-                    while (!mbar_try(bar, (j >> 1) & 1) && clock64() - t0 < ta.budget && !*stop) {
+        // (a warpgroup changes its registers as one)
+        if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        if (warp == kTmaWarp) {
+            const uint32_t qbytes = 128 * DP * 2;
+            bool any = false;
+            int it = 0;
+            bool ok = true;
+            for (int j = next(3, ends, 0); j < ntiles && ok; j = next(3, ends, j + 1)) {
+                const int s = it & 1;
+                const uint32_t par = (it >> 1) & 1;
+                uint8_t *sk = sm + L::k + s * L::tile, *sv = sm + L::v + s * L::tile;
+                // values behind the last key must be finite: they are multiplied by weights of zero
+                const bool edge = sp.nk < (j + 1) * 128 && sp.nk < p.kv_len;
+                if (lane == 0) {
+                    if (!any) {
+                        mbar_expect_tx(q_full, NT * qbytes);
+                        for (int t = 0; t < NT; t++)
+                            for (int x = 0; x < kPanels; x++)
+                                tma_load_4d(sm + L::q + t * L::tile + x * kPanel, &mq, q_full, x * 64, i_first + t * 128, h, b);
+                        any = true;
                     }
-            if (*stop) {  // given up: some loads may never have been asked for, others are on their way
-                const long long t1 = clock64();
-                while (clock64() - t1 < 2000000) {
+                    ok = mbar_wait_spin(&k_empty[s], par ^ 1, ta.status, stop, 41, ta.budget);
+                    if (ok) {
+                        mbar_expect_tx(&k_full[s], qbytes);
+                        for (int x = 0; x < kPanels; x++) tma_load_4d(sk + x * kPanel, &mk, &k_full[s], x * 64, j * 128, hk, b);
+                        ok = mbar_wait_spin(&v_empty[s], par ^ 1, ta.status, stop, 42, ta.budget);
+                    }
+                    if (ok) {
+                        uint64_t *bar = edge ? tail : &v_full[s];
+                        mbar_expect_tx(bar, qbytes);
+                        for (int x = 0; x < kPanels; x++) tma_load_4d(sv + x * kPanel, &mv, bar, x * 64, j * 128, hk, b);
+                        if (edge) ok = mbar_wait_spin(tail, 0, ta.status, stop, 43, ta.budget);  // the last tile: once
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                __syncwarp();
+                if (edge && ok) {
+                    const int from = sp.nk - j * 128;  // a row is 128 bytes of each panel, wherever the swizzle puts its pieces
+                    for (int u = lane; u < (128 - from) * 8 * kPanels; u += 32) {
+                        const int x = u / ((128 - from) * 8), v = u % ((128 - from) * 8);
+                        *(uint4 *)(sv + x * kPanel + (from + v / 8) * 128 + (v % 8) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[s]);
+                }
+                it++;
+            }
+            if (lane == 0) {
+                // copies land before the block may exit, however it ends (bounded)
+                const long long t0 = clock64();
+                if (it > 0)
+                    while (!mbar_try(q_full, 0) && clock64() - t0 < ta.budget) {
+                    }
+                for (int j = it > 2 ? it - 2 : 0; j < it; j++)
+                    for (uint64_t *bar : {&k_full[j & 1], &v_full[j & 1]})
+                        while (!mbar_try(bar, (j >> 1) & 1) && clock64() - t0 < ta.budget && !*stop) {
+                        }
+                if (*stop) {  // given up: some loads may never have been asked for, others are on their way
+                    const long long t1 = clock64();
+                    while (clock64() - t1 < 2000000) {
+                    }
                 }
             }
-        }
-        __syncwarp();
-    } else if (warp == kMmaWarp) {
-        // The whole warp walks the loop, on values that are the same in every lane, and one lane
-        // issues: an instruction's descriptors are uniform registers, and from one lane's own ones
-        // they took 75 to 100 cycles an instruction to move there.
-        constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-        const int ksteps = (p.dim + 15) / 16;
-        const uint32_t id_s = idesc(bf, 128, false), id_o = idesc(bf, ksteps * 16, true), tm = same(tmem);
-        const uint64_t dq = smem_desc(same(smem_u32(sm + L::q))), dk = smem_desc(same(smem_u32(sm + L::k))),
-                       dv = desc_n_major(same(smem_u32(sm + L::v)), kPanel);
-        const int e0 = same(emax[0]), e1 = same(emax[1]), eb = max(e0, e1), nt = (eb + 127) / 128;
-        constexpr int kUnits = L::tile / 16;  // descriptors count 16 bytes
-        bool ok = true;
-        int pend[2] = {-1, -1};  // number of the key tile whose values a tile's weights wait for
-        int np[2] = {0, 0};      // weights consumed
-        int it = 0;
-        auto wait = [&](uint64_t *bar, int parity, int code) -> bool {
-            return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity & 1, ta.status, stop, code, ta.budget));
-        };
-        auto product = [&](int t) {  // O_t += P_t V
-            if (pend[t] < 0) return;
-            const int s = pend[t] & 1;
-            const uint64_t v = dv + s * kUnits;
-            const uint32_t weights = tm + kColS + t * 128, sums = tm + kColO + t * 128, more = np[t] > 0;
-            ok = ok && wait(&v_full[s], pend[t] >> 1, 45) && wait(&p_half[t], np[t], 44);
-            if (!ok) return;
-            tc_fence_after();
-            if (elect()) {
-                umma_ts(sums, weights, v, id_o, more);
-#pragma unroll
-                for (int x = 1; x < 4; x++) umma_ts(sums, weights + x * 8, v + x * (2048 / 16), id_o, 1);
-            }
             __syncwarp();
-            ok = wait(&p_full[t], np[t], 44);
-            if (!ok) return;
-            tc_fence_after();
-            if (elect()) {
+        } else if (warp == kMmaWarp) {
+            // The whole warp walks the loop, on values that are the same in every lane, and one lane
+            // issues: an instruction's descriptors are uniform registers, and from one lane's own ones
+            // they took 75 to 100 cycles an instruction to move there.
+            constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+            const int ksteps = (p.dim + 15) / 16;
+            const uint32_t id_s = idesc(bf, 128, false), id_o = idesc(bf, ksteps * 16, true), tm = same(tmem);
+            const uint64_t dq = smem_desc(same(smem_u32(sm + L::q))), dk = smem_desc(same(smem_u32(sm + L::k))),
+                           dv = desc_n_major(same(smem_u32(sm + L::v)), kPanel);
+            const int e0 = same(emax[0]), e1 = same(emax[1]), eb = max(e0, e1), nt = (eb + 127) / 128;
+            constexpr int kUnits = L::tile / 16;  // descriptors count 16 bytes
+            bool ok = true;
+            int pend[2] = {-1, -1};  // number of the key tile whose values a tile's weights wait for
+            int np[2] = {0, 0};      // weights consumed
+            int it = 0;
+            auto wait = [&](uint64_t *bar, int parity, int code) -> bool {
+                return __all_sync(0xffffffffu, mbar_wait_spin(bar, parity & 1, ta.status, stop, code, ta.budget));
+            };
+            auto product = [&](int t) {  // O_t += P_t V
+                if (pend[t] < 0) return;
+                const int s = pend[t] & 1;
+                const uint64_t v = dv + s * kUnits;
+                const uint32_t weights = tm + kColS + t * 128, sums = tm + kColO + t * 128, more = np[t] > 0;
+                ok = ok && wait(&v_full[s], pend[t] >> 1, 45) && wait(&p_half[t], np[t], 44);
+                if (!ok) return;
+                tc_fence_after();
+                if (elect()) {
+                    umma_ts(sums, weights, v, id_o, more);
 #pragma unroll
-                for (int x = 4; x < 8; x++) umma_ts(sums, weights + x * 8, v + x * (2048 / 16), id_o, 1);
+                    for (int x = 1; x < 4; x++) umma_ts(sums, weights + x * 8, v + x * (2048 / 16), id_o, 1);
+                }
+                __syncwarp();
+                ok = wait(&p_full[t], np[t], 44);
+                if (!ok) return;
+                tc_fence_after();
+                if (elect()) {
+#pragma unroll
+                    for (int x = 4; x < 8; x++) umma_ts(sums, weights + x * 8, v + x * (2048 / 16), id_o, 1);
+                }
+                __syncwarp();
+                pend[t] = -1;
+                np[t]++;
+            };
+            for (int j = same(next(3, eb, 0)); j < nt && ok; j = same(next(3, eb, j + 1)), it++) {
+                const bool v0 = same((int)visits(0, e0, j)), v1 = same((int)visits(1, e1, j));
+                const int s = it & 1;
+                if (it == 0) ok = wait(q_full, 0, 46);
+                ok = ok && wait(&k_full[s], it >> 1, 47);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    product(t);
+                    if (!ok) break;
+                    if (!(t ? v1 : v0)) continue;
+                    const uint64_t q = dq + t * kUnits, k = dk + s * kUnits;
+                    const uint32_t scores = tm + kColS + t * 128;
+                    if (elect()) {
+                        umma(scores, q, k, id_s, 0);
+#pragma unroll
+                        for (int x = 1; x < DP / 16; x++) {
+                            const int off = ((x >> 2) * kPanel + (x & 3) * 32) / 16;
+                            if (x < ksteps) umma(scores, q + off, k + off, id_s, 1);
+                        }
+                        umma_commit(&s_full[t]);
+                    }
+                    __syncwarp();
+                    pend[t] = it;
+                }
+                if (!ok) break;
+                if (elect()) {
+                    umma_commit(&k_empty[s]);
+                    if (it > 0) umma_commit(&v_empty[s ^ 1]);
+                }
+                __syncwarp();
             }
-            __syncwarp();
-            pend[t] = -1;
-            np[t]++;
-        };
-        for (int j = same(next(3, eb, 0)); j < nt && ok; j = same(next(3, eb, j + 1)), it++) {
-            const bool v0 = same((int)visits(0, e0, j)), v1 = same((int)visits(1, e1, j));
-            const int s = it & 1;
-            if (it == 0) ok = wait(q_full, 0, 46);
-            ok = ok && wait(&k_full[s], it >> 1, 47);
-            if (!ok) break;
-            tc_fence_after();
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 product(t);
-                if (!ok) break;
-                if (!(t ? v1 : v0)) continue;
-                const uint64_t q = dq + t * kUnits, k = dk + s * kUnits;
-                const uint32_t scores = tm + kColS + t * 128;
-                if (elect()) {
-                    umma(scores, q, k, id_s, 0);
-#pragma unroll
-                    for (int x = 1; x < DP / 16; x++) {
-                        const int off = ((x >> 2) * kPanel + (x & 3) * 32) / 16;
-                        if (x < ksteps) umma(scores, q + off, k + off, id_s, 1);
-                    }
-                    umma_commit(&s_full[t]);
-                }
+                if (elect()) umma_commit(&o_full[t]);
                 __syncwarp();
-                pend[t] = it;
             }
-            if (!ok) break;
-            if (elect()) {
-                umma_commit(&k_empty[s]);
-                if (it > 0) umma_commit(&v_empty[s ^ 1]);
-            }
+            const long long t0 = clock64();
+            for (int t = 0; t < NT; t++)
+                while (!mbar_try(&o_full[t], 0) && clock64() - t0 < ta.budget) {
+                }
             __syncwarp();
         }
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            product(t);
-            if (elect()) umma_commit(&o_full[t]);
-            __syncwarp();
-        }
-        const long long t0 = clock64();
-        for (int t = 0; t < NT; t++)
-            while (!mbar_try(&o_full[t], 0) && clock64() - t0 < ta.budget) {
-            }
-        __syncwarp();
-    }
     } else {
         if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 tensor-memory lanes

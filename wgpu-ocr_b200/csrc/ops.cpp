@@ -2,6 +2,8 @@
 // device of a call.
 #include "ops.h"
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "elem.h"
@@ -202,7 +204,7 @@ int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, 
         if (batch < 0 || beams < 1 || out_beams < 1 || n_states < 0) fail(WOCR_ERR_INVALID, "beam_reorder: negative or zero sizes");
         if (beams > k::kMaxBeams || out_beams > k::kMaxBeams)
             fail(WOCR_ERR_UNSUPPORTED, "beam_reorder: more than " + std::to_string(k::kMaxBeams) + " beams");
-        if (batch > 1 << 26) fail(WOCR_ERR_UNSUPPORTED, "beam_reorder: more than 2^26 batch elements");
+        if ((int64_t)batch * std::max(beams, out_beams) > INT32_MAX) fail(WOCR_ERR_UNSUPPORTED, "beam_reorder: more than 2^31 rows");
         if (n_states > 0 && !states) fail(WOCR_ERR_INVALID, "null states");
         if (batch == 0 || n_states == 0) {
             need_ctx(ctx);
@@ -214,6 +216,9 @@ int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, 
             const wocr_beam_state &s = states[i];
             if (s.pieces < 0 || s.piece_bytes < 0 || s.piece_stride < 0 || s.row_stride < 0)
                 fail(WOCR_ERR_INVALID, "beam_reorder: negative sizes");
+            const int64_t rows = (int64_t)batch * std::max(beams, out_beams), most = INT64_MAX / 4;
+            if ((s.pieces > 0 && s.piece_stride > most / s.pieces) || s.piece_bytes > most || s.row_stride > most / rows)
+                fail(WOCR_ERR_INVALID, "beam_reorder: sizes beyond 64 bits");
             const int64_t used = s.pieces > 0 && s.piece_bytes > 0 ? (s.pieces - 1) * s.piece_stride + s.piece_bytes : 0;
             if (used > 0) {
                 check_ptr(s.src, 1, "state");

@@ -71,7 +71,7 @@ def _dense(gpu, x, name: str, code: int, shape) -> int:
     """The address of a dense tensor of one type and shape."""
     if x is None:
         raise ValueError(f"{name} is missing")
-    if _code(x) != code or tuple(x.shape) != shape or not x.is_contiguous():
+    if _code(x) != code or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{name}: expected type {code}, contiguous, of shape {shape}, got {x.dtype} {tuple(x.shape)}")
     if x.get_device() != gpu.device:
         raise _elsewhere(gpu, name)
