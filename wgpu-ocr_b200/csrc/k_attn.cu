@@ -100,7 +100,8 @@ __device__ __forceinline__ void mma_parts(float (&c)[4], float (&low)[4], const 
 // Four warps.  FEW: all have the same 16 rows of the queries of all heads that share a key head (row
 // r: head r / q_len, query r % q_len), and each a quarter of a tile's keys; otherwise 64 queries of
 // one head, 16 to a warp.  A cluster's blocks share the keys out tile by tile; partial
-// results are joined in shared memory.
+// results are joined in shared memory.  Bound: matrix instructions (32 bits: six a product) and the
+// softmax's arithmetic (400 x 400, 512 heads of 15: 148 us in 32 bits, 72 us in 16).
 template <typename T, int DP, bool FEW, bool EXTRA>
 __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ AttnP p, int vec) {
     using S = TileSmem<T, DP>;

@@ -29,6 +29,7 @@ struct SelectSmem {
     float wm[kMaxBeams][kWarps], ws[kMaxBeams][kWarps];      // per warp: maximum, sum of exponentials
     float bm[kMaxBeams], bs[kMaxBeams];                      // per block, read by its cluster
     uint8_t fin[kMaxBeams];
+    Cand cut;
     int count;
 };
 
@@ -36,6 +37,8 @@ struct SelectSmem {
 // when `cached`, so that the logits are read from HBM once: maximum, then exponentials, then (with
 // the cluster's log-sum-exps) the best candidate of each thread.  The kout-th best of those is a
 // lower bound of the answer's last candidate, and few pass it: they are gathered and ranked.
+// Bound: the logits' bytes when there are many (256 rows of 18,709 in 16 bits: 9.6 MB in 41 us, cold,
+// of which most is the blocks' barriers and counts), else the chain of barriers.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int slice, int cached) {
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -123,7 +126,12 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int sli
     }
     best_slots<kThreads>(best, tid, sm.lists);
     __syncthreads();
-    const Cand cut = kth_slot(sm.lists, p.kout);
+    if (warp == 0) {
+        const Cand cut = kth_slot(sm.lists, p.kout);
+        if (lane == 0) sm.cut = cut;
+    }
+    __syncthreads();
+    const Cand cut = sm.cut;
     for (int j = 0; j < p.kin; j++) {
         // x must reach cut - base; rounded down, and a step more for the sum's own rounding
         const double base = sm.base[j];
@@ -203,7 +211,8 @@ struct ReorderArgs {
     int kin, kout;
 };
 
-// A block copies 8 x 256 words of V of one row of one state.
+// A block copies 8 x 256 words of V of one row of one state.  Bound: the bytes, once in and once out
+// (629 MB of caches in 70 us cold, 8.9 TB/s with what the L2 cache holds).
 template <typename V>
 __global__ void __launch_bounds__(256) k_beam_reorder(const __grid_constant__ ReorderArgs a) {
     const ReorderState &st = a.st[blockIdx.z];

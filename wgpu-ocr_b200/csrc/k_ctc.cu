@@ -226,7 +226,8 @@ struct SearchSmem {
 // in the order of their places: texts kept, then (beam, class); each one's rank is the number of
 // better ones, counted by four threads.  With all beams alive the least of the kept texts bounds the
 // candidates that are worth a count.
-// Bound: latency.  What a step reads is loaded a step ahead: its best classes, and its logits of every
+// Bound: latency, 1.4 us a step with 4 texts, 1.9 us with 16, of which a mass addition takes 0.17 us.
+// What a step reads is loaded a step ahead: its best classes, and its logits of every
 // class that a beam may then end in (the beams' last classes and the best classes of the step before),
 // which a prefetch into L2 has asked for a step earlier still.
 template <typename T>
@@ -425,8 +426,9 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
 }
 
 // The same with a row's logits in the registers of N threads, E each: rows of up to N E classes.
-// With N = 32 a block's eight warps have a row each.  Bound: the logits' bytes (18,709 classes of 32
-// bits: 17 instructions a logit are three quarters of the time that its bytes take).
+// With N = 32 a block's eight warps have a row each.  Bound: issue slots, 60 % of them taken by 30
+// instructions a logit (4,800 rows of 18,709 classes of 32 bits: 130 us, 2.7 TB/s; rounding only what is
+// taken out saved a third of the instructions and took 15 % longer).
 template <typename T, int N, int E>
 __global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_rows_reg(const CtcP p, const Step out, int K, int64_t rows) {
     constexpr int WARPS = N / 32, PER = N == 32 ? 8 : 1, GOT = 512;
@@ -434,6 +436,7 @@ __global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_row
         Key lists[32];
         Key got[GOT];
         Key top[32];
+        Key cut;
         float wm[WARPS], ws[WARPS];
         int count;
     } smem[PER];
@@ -476,9 +479,14 @@ __global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_row
     for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     if (lane == 0) sm.wm[warp] = m;
     best_slots<N>(best, tid, sm.lists);
-    if (warp == 0) sm.top[lane] = 0;
     sync();
-    const Key cut = kth_slot(sm.lists, K);
+    if (warp == 0) {  // one warp only: the count is as long as a pass over a thread's logits
+        const Key cut = kth_slot(sm.lists, K);
+        if (lane == 0) sm.cut = cut;
+        sm.top[lane] = 0;
+    }
+    sync();
+    const Key cut = sm.cut;
     const float least = cut ? key_value(cut) : -INFINITY;
     m = sm.wm[0];
 #pragma unroll

@@ -63,7 +63,7 @@ __device__ __forceinline__ K kth_slot(const K *slots, int k) {  // by a whole wa
 }
 
 // Logits and scores that are no number never win; an infinite one counts as the largest number.
-__device__ __forceinline__ float clean(float x) { return x <= FLT_MAX ? x : (x > FLT_MAX ? FLT_MAX : -INFINITY); }
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }  // (of a NaN and a number, the number)
 
 }  // namespace topk
 }  // namespace k
