@@ -422,9 +422,10 @@ int32_t wocr_last_transfer_bytes(void *handle, int32_t kind, int64_t *h2d, int64
 /* ---- Operators on device tensors -----------------------------------------------------------
  * No counterpart in the reference: what a recogniser with attention or a search over its classes
  * needs beside the graphs above.  Tensors are the caller's device memory; nothing is copied, and
- * nothing waits.  Work is queued on `stream` (a cudaStream_t of the context's device; NULL: the
- * context's stream; cudaStreamLegacy for the legacy default stream) and may be captured into a
- * graph.  The calling thread's current device is left as it was.  Element types are ONNX
+ * nothing waits: tensors and context must outlive the work.  Work is queued on `stream` (a
+ * cudaStream_t of the context's device; NULL: the context's stream; cudaStreamLegacy for the legacy
+ * default stream) and may be captured into a graph.  The calling thread's current device is left as
+ * it was.  Element types are ONNX
  * TensorProto codes; sums, weights and masses are held in 32 bits or more whatever the type, and
  * results are rounded once (16-bit attention also rounds each weight to the values' type, as the
  * matrix instructions take it).  A bounded wait inside a kernel that gives up is reported by the

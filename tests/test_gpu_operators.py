@@ -225,6 +225,15 @@ def test_attention_over_long_caches(gpu, type, TQ, TK, D):
     attention_check(gpu, q, k, v, causal=True, cap=20.0, slopes=torch.full((H,), 0.01, device="cuda"), kv_lens=i32([TQ, TK - 3]))
 
 
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [4, 8, 12, 40, 72, 80, 100, 128, 136])
+@pytest.mark.parametrize("H, HK, TQ", [(3, 3, 1), (2, 1, 1), (6, 2, 1), (8, 1, 1), (4, 1, 5), (20, 1, 3), (70, 1, 1)])
+def test_attention_of_few_rows(gpu, type, D, H, HK, TQ):
+    """Every count of rows that share a key head, every way that a head's dimension ends within a thread's words."""
+    q, k, v = qkv(2, H, HK, TQ, 330, D, type, 65 + D)
+    attention_check(gpu, q, k, v, causal=True, kv_lens=i32([330, 77]))
+
+
 @pytest.mark.parametrize("type, TQ, TK, D", [("f16", 20, 2500, 128), ("bf16", 150, 3300, 72), ("f16", 260, 1700, 64), ("bf16", 100, 900, 128)])
 @pytest.mark.parametrize("kind", ["", "prefix", "docs", "causal lens", "all"])
 def test_attention_with_keys_shared_out(gpu, kind, type, TQ, TK, D):
