@@ -698,3 +698,63 @@ def test_ndgraph_beam(gpu):
         assert e.value.code == code
     assert len(g.beam(x)) == 2  # and works on
     g.close()
+
+
+# ---- beam search: scores and logits far apart in size -----------------------------------------
+def select_far(gpu, logits, scores, kout, end=-1, finished=None):
+    """select_check, with every output filled beforehand: none may be left as it was."""
+    B = logits.shape[0]
+    o = [torch.full((B, kout), 111, dtype=t, device="cuda") for t in (torch.float32, torch.int32, torch.int32, torch.uint8)]
+    gpu.beam_select(logits, scores, o[0], o[1], o[2], end=end, finished=finished, out_finished=o[3], stream=0)
+    torch.cuda.synchronize()
+    got = [t.cpu().numpy() for t in o]
+    want = ref.beam_select(logits, scores, kout, end, finished.cpu().numpy() if finished is not None else None)
+    for g, w in zip(got[1:], want[1:]):
+        assert (g == w).all(), (g, w)
+    fin = np.isfinite(want[0])
+    assert (np.isneginf(got[0]) == ~fin).all()
+    assert (np.abs(got[0][fin] - want[0][fin]) <= 2.0 ** -24 * np.abs(want[0][fin]) + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("type, least", [("f32", -1e-20), ("f32", -2.0 ** -149), ("bf16", -2.0 ** -133), ("f16", -2.0 ** -24)])
+@pytest.mark.parametrize("V, M", [(97, 1), (5000, 1), (5000, 4), (30000, 8)])
+def test_beam_select_of_certain_log_probabilities(gpu, type, least, V, M):
+    """Log-probabilities next to zero beside scores that they do not change: candidates that tie in 64 bits go by their place."""
+    x = torch.full((2, 3, V), -50.0, device="cuda").to(TYPES[type])
+    x[:, :, V // 3] = least
+    x[1, 1, V // 2] = 0.0
+    for score in (-3.0, -200.0):
+        select_far(gpu, x[:, :1].contiguous(), torch.full((2, 1), score, device="cuda"), M)
+        select_far(gpu, x, torch.full((2, 3), score, device="cuda"), M)
+    # a tiny constant everywhere but for a few zeros
+    flat = torch.full((1, 2, V), least, device="cuda").to(TYPES[type])
+    flat[:, :, [V // 5, V - 2]] = 0.0
+    select_far(gpu, flat, torch.full((1, 2), -3.0, device="cuda"), M)
+
+
+@pytest.mark.parametrize("dead", [-1e9, -1e12, -1e30, float(np.finfo(np.float32).min)])
+@pytest.mark.parametrize("V, M", [(97, 4), (5000, 4), (30000, 12)])
+def test_beam_select_of_dead_beams(gpu, dead, V, M):
+    """Beams that a program scores far below all others: alone, beside ended ones, over logits and log-probabilities."""
+    for seed in range(6):
+        x = randn((3, 4, V), "f32", 200 + seed, 2.0)
+        for y in (x, torch.log_softmax(x, 2), torch.log_softmax(x, 2) - torch.log_softmax(x, 2).amax(2, keepdim=True)):
+            scores = torch.full((3, 4), dead, device="cuda")
+            select_far(gpu, y, scores, M)
+            scores[:, 0] = -1.5
+            fin = torch.zeros((3, 4), dtype=torch.uint8, device="cuda")
+            fin[:, 0] = 1  # an ended beam: one candidate, the others are of the dead ones
+            select_far(gpu, y, scores, M, end=2, finished=fin)
+            select_far(gpu, y, scores, M, end=2)
+
+
+def test_beam_select_of_infinite_logits(gpu):
+    """An infinite logit counts as the largest number: next to it all others of its beam tie."""
+    x = randn((2, 1, 5000), "f32", 41)
+    x[0, 0, 100] = math.inf
+    x[1, 0, [3, 4000]] = math.inf
+    select_far(gpu, x, torch.zeros((2, 1), device="cuda"), 4)
+    y = randn((1, 3, 400), "f32", 42)
+    y[0, 1, 5] = math.inf
+    select_far(gpu, y, torch.zeros((1, 3), device="cuda"), 6)
+    select_far(gpu, y, torch.full((1, 3), float(np.finfo(np.float32).max), device="cuda"), 6)

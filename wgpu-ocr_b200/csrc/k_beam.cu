@@ -134,10 +134,12 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int sli
     __syncthreads();
     const Cand cut = sm.cut;
     for (int j = 0; j < p.kin; j++) {
-        // x must reach cut - base; rounded down, and a step more for the sum's own rounding
+        // Where base + x rounds to cut or more, it is at least cut less half a step of 64 bits, below 2^-52 |cut|.
+        // The difference is rounded down: |base| may be so large that many x give the same sum.
         const double base = sm.base[j];
         float least = -INFINITY;
-        if (cut.v > -INFINITY) least = base > -INFINITY ? nextafterf(__double2float_rd(cut.v - base), -INFINITY) : INFINITY;
+        if (cut.v > -INFINITY)
+            least = base > -INFINITY ? __double2float_rd(__dsub_rd(__dsub_rd(cut.v, base), fabs(cut.v) * 0x1p-52)) : INFINITY;
 #pragma unroll 4
         for (int e = tid; e < n; e += kThreads) {
             const float x = at(j, e);
