@@ -758,3 +758,25 @@ def test_beam_select_of_infinite_logits(gpu):
     y[0, 1, 5] = math.inf
     select_far(gpu, y, torch.zeros((1, 3), device="cuda"), 6)
     select_far(gpu, y, torch.full((1, 3), float(np.finfo(np.float32).max), device="cuda"), 6)
+
+
+# ---- attention: what is seen with a weight of next to nothing ----------------------------------
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("TQ, TK, D", [(1, 200, 64), (3, 700, 128), (5, 60, 15), (40, 40, 15), (64, 100, 200), (150, 300, 64), (200, 900, 128)])
+@pytest.mark.parametrize("below", [20.0, 100.0, 600.0])
+def test_attention_sees_values_far_below_the_best(gpu, type, TQ, TK, D, below):
+    """A key in sight whose weight is e^-below: NaN and infinities among its values reach the result, as they do by the
+    definition, and the rows that do not see it stay finite."""
+    q, k, v = qkv(1, 4, 4, TQ, TK, D, type, 301)
+    q.fill_(1.0)
+    k.zero_()
+    at = TK - 1 - TQ // 2
+    k[:, :, at, 0] = -below
+    v[0, 0, at, 3], v[0, 1, at, 0], v[0, 2, at, D - 1] = float("nan"), math.inf, -math.inf
+    for kw in (dict(), dict(causal=True)):
+        out = attention_check(gpu, q, k, v, scale=1.0, **kw)
+        want, _, _ = ref.attention(q, k, v, 1.0, **kw)
+        got = out.cpu().double()
+        assert torch.equal(torch.isinf(got), torch.isinf(want))
+        assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+        assert torch.isinf(want[0, 1, -1, 0]) and torch.isnan(want[0, 0, -1, 3]) and torch.isfinite(want[0, 3]).all()

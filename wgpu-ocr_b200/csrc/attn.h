@@ -22,6 +22,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
+
 // What the masks leave of a batch element: rows below nq are its queries, keys below nk its keys;
 // query i stands at position off + i among the keys.
 struct Span {
@@ -80,9 +82,9 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
     const int end = key_end(p, sp, i);
     const float slope = p.slopes ? p.slopes[h] : 0.f;
     const int doc = p.q_docs ? p.q_docs[b * p.qds + i] : 0;
+    auto sees = [&](int j) -> bool { return j < end && !(p.q_docs && (doc < 0 || p.kv_docs[b * p.kds + j] != doc)); };
     auto score = [&](int j) -> float {
-        if (j >= end) return -INFINITY;
-        if (p.q_docs && (doc < 0 || p.kv_docs[b * p.kds + j] != doc)) return -INFINITY;
+        if (!sees(j)) return -INFINITY;
         const T *kr = kb + (int64_t)j * p.ks[2];
         float dot = 0.f;
         for (int d = 0; d < p.dim; d++) dot = fmaf(to_f(q[d]), to_f(kr[d]), dot);
@@ -109,14 +111,22 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
     for (int x = 0; x < 8; x++) acc[x] = 0.f;
     for (int j0 = 0; j0 < end; j0 += 32) {
         const float s = score(j0 + lane);
-        const float w = s == -INFINITY ? 0.f : ex2(s - base);  // NaN scores stay NaN
+        float w = s == -INFINITY ? 0.f : ex2(s - base);  // NaN scores stay NaN
+        // The exponential ends at 2^-126.  What is seen keeps a weight above zero, so that its infinities come
+        // through as they do by the definition; the mark stands for zero with finite values.
+        constexpr float mark = 0x1p-149f;
+        if (w == 0.f && s > -INFINITY) w = mark;
+        const uint32_t seen = __ballot_sync(0xffffffffu, sees(j0 + lane));
         for (int jj = 0; jj < 32; jj++) {
             const float wj = __shfl_sync(0xffffffffu, w, jj);
-            if (wj == 0.f) continue;  // unseen keys' values are not touched
+            if (!(seen >> jj & 1)) continue;  // unseen keys' values are not touched
             const T *vr = vb + (int64_t)(j0 + jj) * p.vs[2];
 #pragma unroll
             for (int x = 0; x < 8; x++)
-                if (lane + 32 * x < p.dim) acc[x] = fmaf(wj, to_f(vr[lane + 32 * x]), acc[x]);
+                if (lane + 32 * x < p.dim) {
+                    const float u = to_f(vr[lane + 32 * x]);
+                    acc[x] = fmaf(wj == mark && finite(u) ? 0.f : wj, u, acc[x]);
+                }
         }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zero
@@ -203,7 +213,6 @@ struct JoinSmem {
     float weight[512], l[512];  // per part and row of the cluster: maximum, then share; sum
     uint8_t odd[64];            // rows whose sums are not finite
 };
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234e38f; }
 
 // The parts of a cluster's blocks, joined and stored.  Four warps of a block wrote parts[warp]:
 // with PER = 4 the same 16 rows each, with PER = 1 rows 16 warp ..; row r is query query(r) of head
