@@ -780,3 +780,17 @@ def test_attention_sees_values_far_below_the_best(gpu, type, TQ, TK, D, below):
         assert torch.equal(torch.isinf(got), torch.isinf(want))
         assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
         assert torch.isinf(want[0, 1, -1, 0]) and torch.isnan(want[0, 0, -1, 3]) and torch.isfinite(want[0, 3]).all()
+
+
+@pytest.mark.parametrize("type, value", [("f32", 3e38), ("bf16", 3e38), ("f16", 6e4)])
+@pytest.mark.parametrize("TQ, TK, D", [(1, 200, 64), (3, 700, 128), (5, 60, 15), (40, 40, 15), (64, 100, 200), (150, 300, 64), (200, 900, 128)])
+def test_attention_of_values_near_the_largest(gpu, type, value, TQ, TK, D):
+    """A weighted mean of finite values is finite, although the sum before the division is not."""
+    q, k, v = qkv(1, 2, 2, TQ, TK, D, type, 302)
+    v.fill_(value)
+    v[:, 1, :, ::2] *= -1
+    v[:, :, TK // 2, 1] = 0.0
+    # below the largest number by more than the weights' rounding (a sum of rounded weights may exceed one by a 16-bit step)
+    v *= 0.99
+    out = attention_check(gpu, q, k, v, causal=True)
+    assert torch.isfinite(out).all()

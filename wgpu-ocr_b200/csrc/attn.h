@@ -106,12 +106,14 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
         m = mn;
     }
     const float base = m == -INFINITY ? 0.f : m;
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zero
     float acc[8];  // dimensions lane, lane + 32, ... of at most 256
 #pragma unroll
     for (int x = 0; x < 8; x++) acc[x] = 0.f;
     for (int j0 = 0; j0 < end; j0 += 32) {
         const float s = score(j0 + lane);
-        float w = s == -INFINITY ? 0.f : ex2(s - base);  // NaN scores stay NaN
+        // NaN scores stay NaN.  Divided here, so that the sum stays below the largest value.
+        float w = s == -INFINITY ? 0.f : ex2(s - base) * inv;
         // The exponential ends at 2^-126.  What is seen keeps a weight above zero, so that its infinities come
         // through as they do by the definition; the mark stands for zero with finite values.
         constexpr float mark = 0x1p-149f;
@@ -129,10 +131,9 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
                 }
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zero
 #pragma unroll
     for (int x = 0; x < 8; x++)
-        if (lane + 32 * x < p.dim) o[lane + 32 * x] = from_f<T>(acc[x] * inv);
+        if (lane + 32 * x < p.dim) o[lane + 32 * x] = from_f<T>(acc[x]);
 }
 
 // ---- warp matrix instructions (16 x 8 x 16, fp32 accumulators) -----------------------------
