@@ -794,3 +794,29 @@ def test_attention_of_values_near_the_largest(gpu, type, value, TQ, TK, D):
     v *= 0.99
     out = attention_check(gpu, q, k, v, causal=True)
     assert torch.isfinite(out).all()
+
+
+def infinities_compare(out, q, k, v, scale, **kw):
+    """Infinite outputs exactly, and no others: a tolerance cannot fail next to an infinite value."""
+    want, _, rows = ref.attention(q, k, v, scale, **kw)
+    got, want = out.cpu().double()[rows], want[rows]
+    assert torch.isinf(want).any()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("TQ, TK, D", [(1, 200, 64), (64, 200, 15), (200, 300, 64), (260, 400, 128), (4, 900, 128), (20, 2500, 128), (70, 90, 200)])
+def test_attention_of_infinities_in_sight(gpu, type, TQ, TK, D):
+    """Infinite values that some rows see and others do not, behind a causal mask and in documents: their sign and place."""
+    B, H = 2, 2
+    q, k, v = qkv(B, H, H, TQ, TK, D, type, 311)
+    at = TK - 1 - TQ // 2
+    v[0, 0, at, D - 1], v[1, 1, at, 0], v[1, 0, at, 1] = math.inf, -math.inf, math.inf
+    v[1, 0, at // 2, 1] = -math.inf  # both: no number, for the rows that see both
+    scale = D ** -0.5
+    docs = torch.zeros((B, TK), dtype=torch.int32, device="cuda")
+    docs[:, at // 2] = 1
+    same = torch.zeros((B, TQ), dtype=torch.int32, device="cuda")
+    for kw in (dict(), dict(causal=True), dict(q_docs=same, kv_docs=docs), dict(cap=9.0, causal=True)):
+        infinities_compare(attention_check(gpu, q, k, v, scale=scale, **kw), q, k, v, scale, **kw)
