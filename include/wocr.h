@@ -489,7 +489,9 @@ int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, 
  * alignments of the product of the steps' softmax probabilities; `width` (1 to 31) texts are kept
  * per step, compared in multiples of 2^-30 of the log mass (32-bit logits below 2^-6 are rounded
  * to such multiples), ties to texts kept before texts grown, in the order of their beams, then of
- * classes.  Outputs, the best `paths` texts of each line: tokens [lines][paths][steps], -1 past
+ * classes.  Masses are held in 64 bits, logits taken from their step's largest: what a step adds to
+ * all classes alike changes nothing, and among texts 2^22 or more below the best, whose differences
+ * 64 bits no longer hold to 2^-30, ties may go to the larger logit before the lower class.  Outputs, the best `paths` texts of each line: tokens [lines][paths][steps], -1 past
  * a text's end, lengths and scores (log mass) [lines][paths]; a path that does not exist has
  * length 0 and score -inf.  Logits are cleaned as in wocr_beam_select.  The call's workspace comes
  * from the device's stream-ordered pool, on `stream`. */

@@ -820,3 +820,39 @@ def test_attention_of_infinities_in_sight(gpu, type, TQ, TK, D):
     same = torch.zeros((B, TQ), dtype=torch.int32, device="cuda")
     for kw in (dict(), dict(causal=True), dict(q_docs=same, kv_docs=docs), dict(cap=9.0, causal=True)):
         infinities_compare(attention_check(gpu, q, k, v, scale=scale, **kw), q, k, v, scale, **kw)
+
+
+# ---- CTC: logits far from zero -------------------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("v, width", [(40, 5), (300, 16), (7000, 4)])
+def test_ctc_beam_of_steps_that_shift_every_class(gpu, type, v, width):
+    """A step whose classes are all alike says nothing, however low or high it stands: the texts and masses are those of the
+    step at zero."""
+    plain = peaky(3, 12, v, type, 400 + v)
+    plain[:, 4] = 0.0
+    plain[1, 0] = plain[2, 11] = plain[2, 7] = 0.0
+    x = plain.clone()
+    low = torch.finfo(x.dtype).min
+    x[:, 4] = low  # a padded step
+    x[1, 0], x[2, 11], x[2, 7] = math.inf, 1e30, -1e9
+    lens = i32([12, 12, 10])
+    search_compare(search(gpu, x, lens, width, 0, width), plain, lens, width, 0, width)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16"])
+@pytest.mark.parametrize("v", [60, 2500, 30000])
+def test_ctc_beam_of_certain_steps(gpu, type, v):
+    """An infinite logit, or all classes but one masked by a very low number: the step is that class, what comes before and
+    after decides the rest."""
+    plain = peaky(4, 9, v, type, 500 + v)
+    low = -5e4 if type == "f16" else -1e5
+    for t, c in ((2, 7), (3, 0), (5, v - 1)):
+        plain[:, t] = low
+        plain[:, t, c] = 0.0
+    x = plain.clone()
+    for t, c in ((2, 7), (3, 0), (5, v - 1)):
+        x[0, t] = plain[0, 6]  # any finite logits beside the infinite one
+        x[0, t, c] = math.inf
+        x[1, t, torch.arange(v, device="cuda") != c] = torch.finfo(x.dtype).min
+        x[2, t, torch.arange(v, device="cuda") != c] = -math.inf
+    search_compare(search(gpu, x, None, 4, 0, 2), plain, None, 4, 0, 2)

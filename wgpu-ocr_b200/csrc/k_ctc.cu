@@ -3,7 +3,8 @@
 //   class (pn).  A step with logits x keeps a text, pb' = log(e^pb + e^pn) + x_blank and
 //   pn' = pn + x_last, or appends a class c, pn' = log(e^pb + e^pn) + x_c (pb + x_c when c is its
 //   last class again); a text reached both ways adds the masses up.  The best `width` go on.
-// The steps' log-sum-exps shift every beam alike: they enter the scores only.
+// What a step adds to all classes alike shifts every beam alike: x is taken from the step's largest logit, so that
+// masses stay near zero and 64 bits hold their differences, and the log-sum-exp above it enters the scores only.
 #include <algorithm>
 #include <climits>
 
@@ -34,11 +35,12 @@ __device__ __forceinline__ float exp2_of(float x) {
 }
 
 // What a step's logits leave for the search: its best classes apart from the blank (value, class;
-// class -1 behind the last), the blank's logit and the log-sum-exp.
+// class -1 behind the last), the blank's logit, the largest logit (0 where all are -inf) and the
+// log-sum-exp above it.
 struct Step {
     float *val;
     int *cls;
-    float *blank;
+    float *blank, *max;
     double *lse;
 };
 
@@ -136,7 +138,8 @@ __global__ void __launch_bounds__(kThreads) k_ctc_rows(const CtcP p, const Step 
     if (tid == 0) {
         double sum = 0;
         for (int w = 0; w < kWarps; w++) sum += sm.ws[w];
-        out.lse[r] = m > -INFINITY ? m + log(sum) : -INFINITY;
+        out.max[r] = m > -INFINITY ? m : 0.f;
+        out.lse[r] = m > -INFINITY ? log(sum) : -INFINITY;
     }
 }
 
@@ -198,7 +201,7 @@ struct Beams {
     double pb[32], pn[32], tot[32];
     uint64_t hash[32], before[32];               // of the text, and of the text without its last class
     int last[32], len[32];
-    float xl[32];                                // the step's logit of the last class
+    double xl[32];                               // the step's logit of the last class, from its largest
     int live;
 };
 constexpr int64_t kNever = INT64_MIN;            // the key of what is no candidate
@@ -213,9 +216,9 @@ struct SearchSmem {
     uint8_t pi[kMaxCand], pk[kMaxCand];
     uint32_t kids[2][32];                        // beams that are a beam's text and a class more
     int parent[32];                              // and the beam that a text is one class more than, or -1
-    float val[2][32];
+    double val[2][32];                           // logits of a step, from its largest
     int cls[2][32];
-    float next[2][32];                           // the next step's logits of the beams' last classes, of the best classes
+    double next[2][32];                          // the next step's logits of the beams' last classes, of the best classes
     double blank[2], norm;
     uint32_t back[kTrace * 32];
 };
@@ -260,10 +263,10 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
         b.last[0] = -1;
         b.len[0] = 0;
         b.xl[0] = -INFINITY;
-        if (len > 0) sm.blank[0] = st.blank[r0];
+        if (len > 0) sm.blank[0] = (double)st.blank[r0] - st.max[r0];
     }
     if (tid < K && len > 0) {
-        sm.val[0][tid] = st.val[r0 * K + tid];
+        sm.val[0][tid] = (double)st.val[r0 * K + tid] - st.max[r0];
         sm.cls[0][tid] = st.cls[r0 * K + tid];
     }
     __syncthreads();
@@ -274,13 +277,14 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
         const int n = now.live;
         // loads for the next step, stored at the end of this one's first half
         T nx = from_f<T>(0.f);
-        float nv = 0.f, nb = 0.f;
+        float nv = 0.f, nb = 0.f, nm = 0.f;
         int nc = -1;
         const bool more = t + 1 < len;
         if (more && warp >= loader) {
             const int c = warp == loader ? (lane < n ? now.last[lane] : -1) : (lane < K ? sm.cls[cur][lane] : -1);
             const T *row = x0 + (t + 1) * p.lt;
             if (c >= 0) nx = row[c];
+            nm = st.max[r + 1];
             if (warp > loader && lane < K) {
                 nv = st.val[(r + 1) * K + lane];
                 nc = st.cls[(r + 1) * K + lane];
@@ -344,13 +348,13 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
         if (warp >= loader) {
             sm.kids[cur ^ 1][lane] = 0;
             if (more) {
-                sm.next[warp - loader][lane] = on_step(to_f(nx));
+                sm.next[warp - loader][lane] = (double)on_step(to_f(nx)) - nm;
                 if (warp > loader) {
                     if (lane < K) {
-                        sm.val[cur ^ 1][lane] = nv;
+                        sm.val[cur ^ 1][lane] = (double)nv - nm;
                         sm.cls[cur ^ 1][lane] = nc;
                     }
-                    if (lane == 0) sm.blank[cur ^ 1] = nb;
+                    if (lane == 0) sm.blank[cur ^ 1] = (double)nb - nm;
                 }
             }
         }
@@ -395,7 +399,7 @@ __global__ void __launch_bounds__(kMaxSearch) k_ctc_search(const CtcP p, const S
     }
     Beams &end = sm.beams[cur];
     const int n = end.live;
-    if (warp == 0) {  // the steps' log-sum-exps
+    if (warp == 0) {  // the steps' log-sum-exps above their largest logits
         double norm = 0;
         for (int t = lane; t < len; t += 32) norm += st.lse[r0 + t];
         for (int d = 16; d; d /= 2) norm += __shfl_xor_sync(0xffffffffu, norm, d);
@@ -542,7 +546,8 @@ __global__ void __launch_bounds__(N == 32 ? 256 : N, N == 512 ? 2 : 1) k_ctc_row
     if (tid == 0) {
         double sum = 0;
         for (int w = 0; w < WARPS; w++) sum += sm.ws[w];
-        out.lse[r] = m > -INFINITY ? m + log(sum) : -INFINITY;
+        out.max[r] = m > -INFINITY ? m : 0.f;
+        out.lse[r] = m > -INFINITY ? log(sum) : -INFINITY;
     }
 }
 
@@ -591,13 +596,14 @@ void ctc_beam(Ctx *c, const CtcP &p, cudaStream_t s) {
     auto up = [](size_t b) { return (b + 255) / 256 * 256; };
     const size_t a = up(rows * 8), b = up(rows * K * 4), d = up(rows * 4);
     uint8_t *w = nullptr;
-    WOCR_CUDA(cudaMallocFromPoolAsync((void **)&w, a + 2 * b + d + up(rows * p.width * 4), c->pool, s));
+    WOCR_CUDA(cudaMallocFromPoolAsync((void **)&w, a + 2 * b + 2 * d + up(rows * p.width * 4), c->pool, s));
     Step st;
     st.lse = (double *)w;
     st.val = (float *)(w + a);
     st.cls = (int *)(w + a + b);
     st.blank = (float *)(w + a + 2 * b);
-    uint32_t *back = (uint32_t *)(w + a + 2 * b + d);
+    st.max = (float *)(w + a + 2 * b + d);
+    uint32_t *back = (uint32_t *)(w + a + 2 * b + 2 * d);
     try {
         if (p.type == WOCR_F32) run<float>(c, p, st, back, s);
         else if (p.type == WOCR_F16) run<__half>(c, p, st, back, s);
