@@ -856,3 +856,18 @@ def test_ctc_beam_of_certain_steps(gpu, type, v):
         x[1, t, torch.arange(v, device="cuda") != c] = torch.finfo(x.dtype).min
         x[2, t, torch.arange(v, device="cuda") != c] = -math.inf
     search_compare(search(gpu, x, None, 4, 0, 2), plain, None, 4, 0, 2)
+
+
+def test_ndgraph_attention_in_a_chain(gpu):
+    """The product that ends one attention begins the next: the step is run once, in the first."""
+    from wocr import NdGraph
+    x = np.random.default_rng(3).normal(size=(2, 2, 5, 5)).astype(np.float32)
+    chain = [("Transpose", ["x"], "t", {"perm": [0, 1, 3, 2]}), ("MatMul", ["x", "t"], "s1", {}), ("Softmax", ["s1"], "p1", {"axis": -1}),
+             ("MatMul", ["p1", "x"], "s2", {}), ("Softmax", ["s2"], "p2", {"axis": -1}), ("MatMul", ["p2", "x"], "s3", {}),
+             ("Softmax", ["s3"], "p3", {"axis": -1}), ("MatMul", ["p3", "x"], "y", {})]
+    g = NdGraph(gpu, _graph(chain))
+    before = g.run(x)
+    assert g.fuse_attention() == 2  # the first and the last: the middle one shares a product with either
+    for _ in range(3):
+        assert np.abs(g.run(x) - before).max() < 1e-5
+    g.close()

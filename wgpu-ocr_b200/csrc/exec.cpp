@@ -976,6 +976,8 @@ void Executor::find_attention() {
     auto only = [&](int i) { return readers[steps[i].output] == 1 && steps[i].output != output ? reader[steps[i].output] : -1; };
     for (int i = 0; i < (int)steps.size(); i++) {
         if (!generic(i, "MatMul")) continue;
+        // the last product of one is not the first of the next: a step runs in one place
+        if (std::any_of(attn.begin(), attn.end(), [&](const Attn &x) { return x.out == i; })) continue;
         const int sm = only(i);
         if (sm < 0 || !generic(sm, "Softmax")) continue;
         const int64_t axis = model.nodes[steps[sm].node].int_("axis").value_or(-1);
