@@ -871,3 +871,16 @@ def test_ndgraph_attention_in_a_chain(gpu):
     for _ in range(3):
         assert np.abs(g.run(x) - before).max() < 1e-5
     g.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.float64, torch.int16, torch.float8_e4m3fn, torch.bool])
+def test_beam_reorder_of_any_type(gpu, dtype):
+    """States are bytes: a history of 64-bit tokens, a cache in 8 bits."""
+    par = i32([[2, 0, 0], [1, 1, 2]])
+    rows = (torch.arange(2, device="cuda")[:, None] * 3 + par).reshape(-1)
+    src = torch.randint(-9, 9, (6, 5, 7), device="cuda").to(dtype)
+    dst = torch.zeros((6, 5, 7), device="cuda").to(dtype)
+    gpu.beam_reorder(par, [(src, dst)], axis=2, live=3, stream=0)
+    torch.cuda.synchronize()
+    as_bytes = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+    assert torch.equal(as_bytes(dst[:, :, :3]), as_bytes(src[rows][:, :, :3])) and not as_bytes(dst[:, :, 3:]).any()

@@ -189,3 +189,18 @@ def test_reference_attention_is_softmax_attention():
     out, size, rows = ref.attention(q, k, v, 0.3)
     want = torch.softmax(q.double() @ k.double().transpose(2, 3) * 0.3, 3) @ v.double()
     assert rows.all() and (out - want).abs().max() < 1e-12 and (size >= out.abs()).all()
+
+
+def test_beam_reorder_takes_any_type():
+    """What is only copied may have any element type, alike in source and destination."""
+    par = arr((2, 3), "int32")
+    pair = lambda a, b: [(arr((6, 4), a), arr((6, 4), b, ptr=8 << 20))]  # noqa: E731
+    for t in ("int64", "float64", "int8", "bool", "float8_e4m3fn"):
+        with pytest.raises(wocr.WocrError, match="null ctx"):
+            _Bare().beam_reorder(par, pair(t, t))
+    for a, b in (("bool", "uint8"), ("int64", torch.int64)):
+        with pytest.raises(wocr.WocrError, match="null ctx"):
+            _Bare().beam_reorder(par, pair(a, b))
+    for a, b in (("int64", "float64"), ("float16", "bfloat16"), ("object", "object"), ("complex64", "complex64")):
+        with pytest.raises(ValueError):
+            _Bare().beam_reorder(par, pair(a, b))

@@ -15,8 +15,12 @@ from . import _lib as L
 
 F32, F16, BF16, I32, U8 = 1, 10, 16, 6, 2  # ONNX TensorProto codes
 _NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "int32": I32, "uint8": U8, "bool": U8}
-_SIZES = {F32: 4, F16: 2, BF16: 2, I32: 4, U8: 1}
 _codes = {}  # dtype object -> code
+# bytes of an element, for what is only copied
+_SIZES = {n: size for size, names in ((1, "uint8 int8 float8_e4m3fn float8_e4m3fnuz float8_e5m2 float8_e5m2fnuz float8_e8m0fnu"),
+                                      (2, "int16 uint16 float16 bfloat16"), (4, "int32 uint32 float32"),
+                                      (8, "int64 uint64 float64")) for n in names.split()}
+_kinds = {}  # dtype object -> (name, bytes of an element)
 _ARGS = struct.Struct("10Q14q8i2f")
 _STATE = struct.Struct("2Q4q")
 _LEGACY = 1  # cudaStreamLegacy
@@ -63,6 +67,17 @@ def _code(x) -> int:
     return code
 
 
+def _kind(x) -> Tuple[str, int]:
+    kind = _kinds.get(x.dtype)
+    if kind is None:
+        name = str(x.dtype).rsplit(".", 1)[-1]
+        name = "uint8" if name == "bool" else name
+        if name not in _SIZES:
+            raise ValueError(f"element type {x.dtype} is not supported")
+        kind = _kinds[x.dtype] = name, _SIZES[name]
+    return kind
+
+
 def _elsewhere(gpu, name: str):
     return ValueError(f"{name} is not on device {gpu.device}")
 
@@ -75,6 +90,15 @@ def _dense(gpu, x, name: str, code: int, shape) -> int:
         raise ValueError(f"{name}: expected type {code}, contiguous, of shape {shape}, got {x.dtype} {tuple(x.shape)}")
     if x.get_device() != gpu.device:
         raise _elsewhere(gpu, name)
+    return x.data_ptr()
+
+
+def _state(gpu, x, kind, shape) -> int:
+    """The address of a dense tensor of one type and shape that is only copied."""
+    if _kind(x) != kind or x.shape != shape or not x.is_contiguous():
+        raise ValueError(f"state: expected {kind[0]}, contiguous, of shape {shape}, got {x.dtype} {tuple(x.shape)}")
+    if x.get_device() != gpu.device:
+        raise _elsewhere(gpu, "state")
     return x.data_ptr()
 
 
@@ -163,8 +187,8 @@ class DeviceOps:
 
     def beam_reorder(self, parents, states, axis: int = 0, live: Optional[int] = None, stream: Optional[int] = None):
         """The states of the chosen beams in their new order (`wocr_beam_reorder`): `parents` int32 [batch, out_beams] as
-        beam_select gives them; `states` pairs of tensors (src [batch * beams, ...], dst [batch * out_beams, ...]), dense
-        and alike but for the first dimension.  With `axis` > 0 only the first `live` entries along it are copied (a
+        beam_select gives them; `states` pairs of tensors (src [batch * beams, ...], dst [batch * out_beams, ...]) of any
+        real type, dense and alike but for the first dimension.  With `axis` > 0 only the first `live` entries along it are copied (a
         cache's tokens); the rest of dst, and rows whose parent is not a beam, are left as they were."""
         if len(parents.shape) != 2:
             raise ValueError("parents [batch, beams] expected")
@@ -172,21 +196,21 @@ class DeviceOps:
         n, parts = None, []
         for src, dst in states:
             shape = tuple(src.shape)
-            code = _code(src)
+            kind = _kind(src)
             if not 0 <= axis < len(shape):
                 raise ValueError(f"axis {axis} of a state of shape {shape}")
             rows = shape[0] // b if b else 1
             if shape[0] != rows * b or (n is not None and rows != n):
                 raise ValueError(f"a state of shape {shape} for {b} x {m} parents and {n} beams")
             n = rows
-            full = _SIZES[code] * math.prod(shape[axis or 1:])  # bytes of a piece and of what of it is copied
+            full = kind[1] * math.prod(shape[axis or 1:])  # bytes of a piece and of what of it is copied
             part = full
             if axis and live is not None:
                 if not 0 <= live <= shape[axis]:
                     raise ValueError(f"live {live} of a state of shape {shape}")
                 part = full // max(shape[axis], 1) * live
             pieces = math.prod(shape[1:axis])
-            parts.append(_STATE.pack(_dense(self, src, "state", code, shape), _dense(self, dst, "state", code, (b * m,) + shape[1:]),
+            parts.append(_STATE.pack(_state(self, src, kind, shape), _state(self, dst, kind, (b * m,) + shape[1:]),
                                      pieces, part, full, pieces * full))
         st = L.lib().wocr_beam_reorder(self.h, _dense(self, parents, "parents", I32, (b, m)), b, n or 1, m, b"".join(parts),
                                        len(parts), _stream(stream))
