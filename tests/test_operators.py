@@ -204,3 +204,11 @@ def test_beam_reorder_takes_any_type():
     for a, b in (("int64", "float64"), ("float16", "bfloat16"), ("object", "object"), ("complex64", "complex64")):
         with pytest.raises(ValueError):
             _Bare().beam_reorder(par, pair(a, b))
+
+
+def test_beam_reorder_refuses_states_of_no_beams():
+    """A source without rows has no beam that a parent could name."""
+    with pytest.raises(ValueError, match="shape"):
+        _Bare().beam_reorder(arr((2, 3), "int32"), [(arr((0, 4)), arr((6, 4), ptr=8 << 20))])
+    with pytest.raises(wocr.WocrError, match="null ctx"):  # no batch elements: nothing to do
+        _Bare().beam_reorder(arr((0, 3), "int32"), [(arr((0, 4)), arr((0, 4), ptr=8 << 20))])

@@ -200,7 +200,7 @@ class DeviceOps:
             if not 0 <= axis < len(shape):
                 raise ValueError(f"axis {axis} of a state of shape {shape}")
             rows = shape[0] // b if b else 1
-            if shape[0] != rows * b or (n is not None and rows != n):
+            if rows < 1 or shape[0] != rows * b or (n is not None and rows != n):
                 raise ValueError(f"a state of shape {shape} for {b} x {m} parents and {n} beams")
             n = rows
             full = kind[1] * math.prod(shape[axis or 1:])  # bytes of a piece and of what of it is copied
