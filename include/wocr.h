@@ -475,7 +475,8 @@ int32_t wocr_beam_select(wocr_ctx *ctx, const void *logits, int32_t type, int32_
  * b * beams + parents[b][j] of src.  A row is `pieces` pieces of piece_bytes bytes, piece_stride
  * bytes apart (the live part of a cache, head by head); rows are row_stride bytes apart in src and
  * dst.  What lies between the pieces is left as it was, and so is a row whose parent is not a beam.
- * src and dst must not overlap. */
+ * The states of a call are copied in no order: what is written must be no other state's, source or
+ * destination (two that interleave need the same row_stride, within a row the same piece_stride). */
 typedef struct {
     const void *src;
     void *dst;

@@ -212,3 +212,31 @@ def test_beam_reorder_refuses_states_of_no_beams():
         _Bare().beam_reorder(arr((2, 3), "int32"), [(arr((0, 4)), arr((6, 4), ptr=8 << 20))])
     with pytest.raises(wocr.WocrError, match="null ctx"):  # no batch elements: nothing to do
         _Bare().beam_reorder(arr((0, 3), "int32"), [(arr((0, 4)), arr((0, 4), ptr=8 << 20))])
+
+
+def test_beam_reorder_refuses_states_that_share_memory():
+    """One launch copies all states, in no order: what one writes, no other may read or write."""
+    par = arr((2, 3), "int32")
+    t = lambda mb, shape=(6, 4, 8): arr(shape, ptr=mb << 20)  # noqa: E731
+    ok = pytest.raises(wocr.WocrError, match="null ctx")
+    bad = pytest.raises(wocr.WocrError, match="overlap")
+    with bad:  # a chain: the first's destination is the second's source
+        _Bare().beam_reorder(par, [(t(1), t(2)), (t(2), t(3))])
+    with bad:  # two with one destination
+        _Bare().beam_reorder(par, [(t(1), t(3)), (t(2), t(3))])
+    with bad:  # in part, several states apart
+        _Bare().beam_reorder(par, [(t(i), t(40 + i)) for i in range(1, 20)] + [(t(20), arr((6, 4, 8), ptr=(45 << 20) + 700))])
+    with ok:  # a source that two states read, any number of others
+        _Bare().beam_reorder(par, [(t(1), t(2)), (t(1), t(3))] + [(t(i), t(90 + i)) for i in range(10, 80)])
+    # keys and values interleaved in one allocation, row by row and head by head: the library's own call
+    lib, pack = wocr.lib(), __import__("struct").pack
+    call = lambda *st: (lib.wocr_beam_reorder(None, 4096, 2, 3, 3, b"".join(pack("2Q4q", *s) for s in st), len(st), None),  # noqa: E731
+                        lib.wocr_last_error())
+    a, b = 1 << 20, 1 << 24
+    assert b"null ctx" in call((a, b, 4, 64, 64, 1024), (a + 512, b + 512, 4, 64, 64, 1024))[1]   # halves of a row
+    assert b"null ctx" in call((a, b, 4, 64, 256, 1024), (a + 64, b + 64, 4, 64, 256, 1024))[1]   # quarters of a head
+    assert b"null ctx" in call((a, a + 512, 4, 64, 64, 1024))[1]                                  # both halves are one state's
+    assert b"overlap" in call((a, b, 4, 64, 256, 1024), (a + 64, b + 32, 4, 64, 256, 1024))[1]
+    assert b"overlap" in call((a, b, 4, 64, 128, 1024), (a + 512, b + 384, 4, 64, 128, 1024))[1]
+    assert b"overlap" in call((a, b, 1, 1024, 1024, 1024), (b + 5 * 1024, 1 << 26, 1, 1024, 1024, 1024))[1]  # a last row
+    assert b"null ctx" in call((a, b, 1, 1024, 1024, 1024), (b + 6 * 1024, 1 << 26, 1, 1024, 1024, 1024))[1]

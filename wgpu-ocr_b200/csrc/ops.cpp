@@ -60,6 +60,34 @@ void check_apart(const int64_t *dims, const int64_t *strides, int n, const char 
         reach = (d[i] - 1) * s[i] + reach;
     }
 }
+// What a call of beam_reorder reads or writes of a state: pieces in rows from `lo` on, all below `hi`.
+struct Reach {
+    uintptr_t lo, hi;
+    int64_t used, piece, step, row;  // bytes of a row from its first piece to its last, of a piece; from piece to piece, row to row
+    bool write;
+};
+bool shares(const Reach &a, const Reach &b) {  // a.lo <= b.lo
+    if (b.lo >= a.hi) return false;
+    // two that interleave: rows alike with each in its own part of a row, or of every piece's step
+    auto apart = [&](int64_t every, int64_t of_a, int64_t of_b) {
+        const int64_t at = (int64_t)((b.lo - a.lo) % every);
+        return at >= of_a && at + of_b <= every;
+    };
+    if (a.row != b.row) return true;
+    if (apart(a.row, a.used, b.used)) return false;
+    return !(a.step == b.step && a.step > 0 && a.row % a.step == 0 && apart(a.step, a.piece, b.piece));
+}
+// Nothing may be read or written twice of which one is a write: the states are copied in no order.
+void check_shares(std::vector<Reach> &all) {
+    std::sort(all.begin(), all.end(), [](const Reach &a, const Reach &b) { return a.lo < b.lo; });
+    std::vector<const Reach *> open;  // those that may reach to the next
+    for (const Reach &r : all) {
+        open.erase(std::remove_if(open.begin(), open.end(), [&](const Reach *o) { return o->hi <= r.lo; }), open.end());
+        for (const Reach *o : open)
+            if ((o->write || r.write) && shares(*o, r)) fail(WOCR_ERR_INVALID, "beam_reorder: what is written overlaps a source or another destination");
+        open.push_back(&r);
+    }
+}
 void check_strides(const int64_t *s, int n, const char *what) {
     for (int i = 0; i < n; i++)
         if (s[i] < 0) fail(WOCR_ERR_INVALID, std::string(what) + ": negative stride");
@@ -212,6 +240,8 @@ int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, 
         }
         check_ptr(parents, 4, "parents");
         std::vector<k::ReorderState> st((size_t)n_states);
+        std::vector<Reach> all;
+        all.reserve(2 * (size_t)n_states);
         for (int i = 0; i < n_states; i++) {
             const wocr_beam_state &s = states[i];
             if (s.pieces < 0 || s.piece_bytes < 0 || s.piece_stride < 0 || s.row_stride < 0)
@@ -225,13 +255,16 @@ int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, 
                 check_ptr(s.dst, 1, "state");
                 if (s.pieces > 1 && s.piece_stride < s.piece_bytes) fail(WOCR_ERR_INVALID, "beam_reorder: pieces overlap");
                 if (s.row_stride < used) fail(WOCR_ERR_INVALID, "beam_reorder: rows overlap");
-                const uintptr_t a = (uintptr_t)s.src, b = (uintptr_t)s.dst;
-                const uintptr_t an = a + ((int64_t)batch * beams - 1) * s.row_stride + used;
-                const uintptr_t bn = b + ((int64_t)batch * out_beams - 1) * s.row_stride + used;
-                if (a < bn && b < an) fail(WOCR_ERR_INVALID, "beam_reorder: source and destination overlap");
+                auto reach = [&](const void *p, int n, bool write) {
+                    const uintptr_t lo = (uintptr_t)p;
+                    all.push_back({lo, lo + ((int64_t)batch * n - 1) * s.row_stride + used, used, s.piece_bytes, s.piece_stride, s.row_stride, write});
+                };
+                reach(s.src, beams, false);
+                reach(s.dst, out_beams, true);
             }
             st[i] = {s.src, s.dst, s.pieces, s.piece_bytes, s.piece_stride, s.row_stride};
         }
+        check_shares(all);
         Ctx *c = need_ctx(ctx);
         OnDevice on(c->device);
         k::beam_reorder(c, parents, batch, beams, out_beams, st.data(), n_states, stream_of(c, stream));
