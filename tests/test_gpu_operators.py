@@ -884,3 +884,28 @@ def test_beam_reorder_of_any_type(gpu, dtype):
     torch.cuda.synchronize()
     as_bytes = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
     assert torch.equal(as_bytes(dst[:, :, :3]), as_bytes(src[rows][:, :, :3])) and not as_bytes(dst[:, :, 3:]).any()
+
+
+# ---- attention: caps far above the scores ------------------------------------------------------
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [300.0, 1e4, 1e8, 1e30])
+@pytest.mark.parametrize("TQ, TK, D", [(1, 300, 64), (3, 500, 128), (40, 60, 15), (200, 400, 64), (300, 300, 128)])
+def test_attention_of_wide_caps(gpu, type, cap, TQ, TK, D):
+    """A cap is as exact as its scores are, however wide it is: a score's tanh is off by 8 U of the score itself, where it was
+    off by 2^-22 of the cap."""
+    q, k, v = qkv(1, 4, 2, TQ, TK, D, type, 601)
+    for boost in (1.0, 60.0):  # the second: some scores beyond 0.6 of the least cap
+        qq = (q * boost).to(q.dtype)
+        scale = D ** -0.5
+        out = torch.zeros_like(q)
+        gpu.attention(qq, k, v, out, scale=scale, cap=cap, stream=0)
+        torch.cuda.synchronize()
+        want, size, _ = ref.attention(qq, k, v, scale, cap=cap)
+        mag = scale * float(torch.einsum("bhqd,bhkd->bhqk", qq.cpu().double().abs(), k.cpu().double().abs().repeat_interleave(2, 1)).max())
+        half = q.dtype != torch.float32
+        u = torch.finfo(q.dtype).eps / 2
+        es = (D + 8 + 8) * U * mag
+        tol = size * (2 * es + 2.0 ** -20 + TK * U + (u if half else 0)) + want.abs() * u
+        if type == "f16":
+            tol = tol + 2.0 ** -25 * (1 + TK * v.cpu().double().abs().max())
+        assert ((out.cpu().double() - want).abs() <= tol).all()

@@ -45,14 +45,19 @@ __device__ __forceinline__ int key_end(const AttnP &p, const Span &s, int i) {
 
 // cap tanh(y / cap) in units of log 2.  A score's error is a relative error of its weight: with
 // 32-bit values tanhf (within 2 ulp), with 16-bit values 1 - 2 / (1 + e^2y) from two approximate
-// instructions (within 2^-21).
+// instructions, within 2^-22 of the cap: up to a cap of 256 an eighth of a weight's rounding to fp16.
+// Wider caps, whose scores may all be near zero, take tanhf.
 static __device__ __noinline__ float capped32(float y, float cap) { return cap * tanhf(y / cap) * kLog2e; }
 template <typename T>
-__device__ __forceinline__ float capped2(float y, float cap) {
-    if (sizeof(T) == 4) return capped32(y, cap);  // a call: inlined over a tile it fills the instruction caches
+__host__ __device__ __forceinline__ bool by_tanh(float cap) { return sizeof(T) == 4 || cap > 256.f || cap < 0x1p-100f; }
+__device__ __forceinline__ float capped16(float y, float cap) {
     y *= 2.f * kLog2e / cap;
     if (y > 126.f) y = 126.f;  // (a NaN passes)
     return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + ex2(y)));
+}
+template <typename T>
+__device__ __forceinline__ float capped2(float y, float cap) {
+    return by_tanh<T>(cap) ? capped32(y, cap) : capped16(y, cap);  // a call: inlined over a tile it fills the instruction caches
 }
 // Scores that are more than a product, or documents: kernels are built with and without them, since
 // the code of all of them together, unrolled over a tile, does not fit in the instruction caches.
