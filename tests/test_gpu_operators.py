@@ -909,3 +909,14 @@ def test_attention_of_wide_caps(gpu, type, cap, TQ, TK, D):
         if type == "f16":
             tol = tol + 2.0 ** -25 * (1 + TK * v.cpu().double().abs().max())
         assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("TQ", [1, 3, 40, 200])
+def test_attention_of_documents_without_keys(gpu, type, TQ):
+    q, k, v = qkv(2, 2, 2, TQ, 0, 16, type)
+    out = torch.full(q.shape, 7.0, device="cuda", dtype=q.dtype)
+    docs = torch.zeros((2, TQ), dtype=torch.int32, device="cuda")
+    gpu.attention(q, k, v, out, q_docs=docs, kv_docs=docs[:, :0], stream=0)
+    torch.cuda.synchronize()
+    assert (out == 0).all()

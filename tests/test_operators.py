@@ -240,3 +240,12 @@ def test_beam_reorder_refuses_states_that_share_memory():
     assert b"overlap" in call((a, b, 4, 64, 128, 1024), (a + 512, b + 384, 4, 64, 128, 1024))[1]
     assert b"overlap" in call((a, b, 1, 1024, 1024, 1024), (b + 5 * 1024, 1 << 26, 1, 1024, 1024, 1024))[1]  # a last row
     assert b"null ctx" in call((a, b, 1, 1024, 1024, 1024), (b + 6 * 1024, 1 << 26, 1, 1024, 1024, 1024))[1]
+
+
+def test_attention_takes_empty_documents():
+    """No keys or no queries: their ids have no address, as any empty tensor's."""
+    docs = lambda n: arr((2, n), "int32", ptr=1 << 20 if n else 0)  # noqa: E731
+    for tq, tk in ((5, 0), (0, 7), (0, 0)):
+        with pytest.raises(wocr.WocrError, match="null ctx"):
+            attn(q=arr((2, 4, tq, 16)), out=arr((2, 4, tq, 16), ptr=4 << 20), k=arr((2, 2, tk, 16), ptr=2 << 20),
+                 v=arr((2, 2, tk, 16), ptr=3 << 20), q_docs=docs(tq), kv_docs=docs(tk))

@@ -110,7 +110,8 @@ int32_t wocr_attention(wocr_ctx *ctx, const wocr_attention_args *a, void *stream
             fail(WOCR_ERR_UNSUPPORTED, "attention: head dimension " + std::to_string(a->head_dim) + " (1 to 256 are supported)");
         if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0)
             fail(WOCR_ERR_INVALID, "attention: scale and cap must be finite, the cap not negative");
-        if ((a->q_docs == nullptr) != (a->kv_docs == nullptr))
+        // (no queries or no keys: their ids have no address)
+        if (a->q_len > 0 && a->kv_len > 0 && (a->q_docs == nullptr) != (a->kv_docs == nullptr))
             fail(WOCR_ERR_INVALID, "attention: documents need the queries' and the keys' ids");
         if (a->prefix && !a->causal) fail(WOCR_ERR_INVALID, "attention: a prefix without a causal mask");
         if ((int64_t)a->batch * a->heads > 0x7fffffff / 2 || a->q_len > 1 << 30 || a->kv_len > 1 << 30)
@@ -156,8 +157,8 @@ int32_t wocr_attention(wocr_ctx *ctx, const wocr_attention_args *a, void *stream
         p.prefix = a->prefix;
         p.q_lens = a->q_lens;
         p.kv_lens = a->kv_lens;
-        p.q_docs = a->q_docs;
-        p.kv_docs = a->kv_docs;
+        p.q_docs = a->kv_len > 0 ? a->q_docs : nullptr;  // without keys nothing is seen anyway
+        p.kv_docs = a->kv_len > 0 ? a->kv_docs : nullptr;
         p.qds = a->q_docs_stride;
         p.kds = a->kv_docs_stride;
         p.type = a->type;
