@@ -465,7 +465,8 @@ int32_t wocr_attention(wocr_ctx *ctx, const wocr_attention_args *args, void *str
  * out_finished: the parent was finished or the token is `end` (end < 0: none ends).  finished and
  * out_finished are nullable.  Logits that are no number are never chosen before others, infinite
  * ones count as the largest 32-bit number.  With as many beams out as in, scores and flags may be
- * updated in place.  Candidates are compared in 64 bits. */
+ * updated in place.  Candidates are compared in 64 bits; their log-sum-exps are 64-bit sums of 32-bit
+ * exponentials, so that candidates of different beams less than 2^-20 apart may change places. */
 int32_t wocr_beam_select(wocr_ctx *ctx, const void *logits, int32_t type, int32_t batch, int32_t beams, int32_t vocab,
                          int64_t batch_stride, int64_t beam_stride, const float *scores, const uint8_t *finished,
                          int32_t end, int32_t out_beams, float *out_scores, int32_t *out_parents, int32_t *out_tokens,

@@ -920,3 +920,16 @@ def test_attention_of_documents_without_keys(gpu, type, TQ):
     gpu.attention(q, k, v, out, q_docs=docs, kv_docs=docs[:, :0], stream=0)
     torch.cuda.synchronize()
     assert (out == 0).all()
+
+
+def test_beam_select_of_beams_that_are_all_but_certain(gpu):
+    """Beams of one score, each all but certain of its token: the one whose other tokens are least likely goes first,
+    although its log-sum-exp is the maximum in 32 bits."""
+    for type, V in (("f32", 5), ("f32", 700), ("f32", 30000), ("bf16", 700), ("f16", 30000)):
+        x = torch.full((2, 6, V), -60.0, device="cuda")
+        far = torch.tensor([-19.0, -24.0, -18.0, -32.0, -28.0, -21.0], device="cuda")  # e^-19 and less: below 2^-27
+        for j in range(6):
+            x[:, j, (3 * j) % V] = 0.0
+            x[:, j, (3 * j + 1) % V] = far[j]
+            x[1, j] += 8.0 * j  # (what a row adds to every logit says nothing)
+        select_far(gpu, x.to(TYPES[type]), torch.full((2, 6), -1.0, device="cuda"), 6)

@@ -26,8 +26,8 @@ struct SelectSmem {
     Cand got[kGather];
     Cand top[kMaxBeams];                                     // the block's best, read by its cluster
     double base[kMaxBeams];                                  // score - log-sum-exp
-    float wm[kMaxBeams][kWarps], ws[kMaxBeams][kWarps];      // per warp: maximum, sum of exponentials
-    float bm[kMaxBeams], bs[kMaxBeams];                      // per block, read by its cluster
+    double ws[kMaxBeams][kWarps], bs[kMaxBeams];             // sums of exponentials: per warp; per block, read by its cluster
+    float wm[kMaxBeams][kWarps], bm[kMaxBeams];              // maxima, the same
     uint8_t fin[kMaxBeams];
     Cand cut;
     int count;
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int sli
         if (sm.fin[j]) continue;
         float m = sm.wm[j][0];
         for (int w = 1; w < kWarps; w++) m = fmaxf(m, sm.wm[j][w]);
-        float s = 0.f;
+        double s = 0;  // (beside a certain token, what the others add decides between beams)
         if (m > -INFINITY)
 #pragma unroll 8
             for (int e = tid; e < n; e += kThreads) s += exp2f((at(j, e) - m) * 1.4426950408889634f);
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int sli
     }
     __syncthreads();
     if (tid < p.kin) {
-        float s = 0.f;
+        double s = 0;
         for (int w = 0; w < kWarps; w++) s += sm.ws[tid][w];
         sm.bs[tid] = s;
     }
