@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
                 for (int x = lane; x < 128; x += 32) dk[x] = j0 + x < sp.nk ? max(p.kv_docs[b * p.kds + j0 + x], -1) : -1;
                 __syncwarp();
             }
-            ok = mbar_wait_spin(&s_full[my], n & 1, ta.status, stop, 48, ta.budget);
+            // one outcome for the warp, whose lanes then load tensor memory together
+            ok = __all_sync(0xffffffffu, mbar_wait_spin(&s_full[my], n & 1, ta.status, stop, 48, ta.budget));
             if (!ok) break;
             tc_fence_after();
             float f[128], top = -INFINITY, mul = scale2;
