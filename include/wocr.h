@@ -440,7 +440,8 @@ enum { WOCR_F32 = 1, WOCR_F16 = 10, WOCR_BF16 = 16 };
  *   pos_i = kv_lens[b] - q_lens[b] + i              (lengths NULL: kv_len, q_len)
  * Query i sees key j when j < kv_lens[b], and (causal) j <= pos_i or j < prefix[b], and (documents)
  * q_docs[b][i] == kv_docs[b][j] >= 0.  Keys and values that a query does not see do not reach its
- * result, NaN and infinities among them.  A query that sees nothing gets zeros; rows of `out` from
+ * result, NaN and infinities among them.  A query that sees nothing gets zeros (one that sees scores
+ * of -inf alone no number); rows of `out` from
  * q_lens[b] on are left as they were.  Lengths outside the tensors are held to them.  slopes
  * [heads], prefix, q_lens, kv_lens [batch] and the document ids (a row per batch element, their
  * strides between rows) are device memory, each nullable (documents: both or neither; a prefix

@@ -933,3 +933,29 @@ def test_beam_select_of_beams_that_are_all_but_certain(gpu):
             x[:, j, (3 * j + 1) % V] = far[j]
             x[1, j] += 8.0 * j  # (what a row adds to every logit says nothing)
         select_far(gpu, x.to(TYPES[type]), torch.full((2, 6), -1.0, device="cuda"), 6)
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("TQ, TK, D", [(1, 200, 64), (3, 700, 128), (5, 60, 15), (40, 40, 15), (64, 100, 200), (150, 300, 64), (300, 2100, 64),
+                                       (200, 900, 128)])
+def test_attention_of_rows_whose_every_score_is_infinite(gpu, type, TQ, TK, D):
+    """Scores of -inf alone have no softmax: no number. A row that sees nothing is zero, in documents without keys too, and
+    whatever lies in the keys and values that it does not see."""
+    q, k, v = qkv(2, 2, 2, TQ, TK, D, type, 305)
+    q[:, 0, :: 2, 1] = -math.inf
+    k[:, :, :, 1] = k[:, :, :, 1].abs() + 0.5
+    odd = torch.zeros(TQ, dtype=torch.bool)
+    odd[::2] = True
+    ids = torch.zeros((2, TK), dtype=torch.int32, device="cuda")
+    ids[:, TK // 2:] = 4
+    seen = torch.zeros((2, TQ), dtype=torch.int32, device="cuda")
+    seen[1] = 4
+    seen[:, TQ // 3:] = 2  # a document that no key is in
+    seen[:, -1] = -1
+    bad = v.clone()
+    bad[1, :, TK // 4] = float("nan")
+    for values, kw in ((v, dict()), (v, dict(causal=True)), (v, dict(causal=True, kv_lens=i32([TK, max(TQ - 1, 1)]))),
+                       (bad, dict(q_docs=seen, kv_docs=ids)), (bad, dict(q_docs=seen, kv_docs=ids, causal=True))):
+        out = attention_check(gpu, q, k, values, **kw)
+        if not kw:
+            assert torch.isnan(out[:, 0, odd]).all() and torch.isfinite(out[:, 0, ~odd]).all() and torch.isfinite(out[:, 1]).all()

@@ -96,7 +96,9 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
         return score2<T>(p, dot, slope, sp.off + i - j);
     };
     float m = -INFINITY, l = 0.f;
+    bool any = false;
     for (int j0 = 0; j0 < end; j0 += 32) {
+        any |= sees(j0 + lane);
         const float s = score(j0 + lane);
         const float mn = fmaxf(m, s);
         const float base = mn == -INFINITY ? 0.f : mn;
@@ -111,10 +113,11 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
         m = mn;
     }
     const float base = m == -INFINITY ? 0.f : m;
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is zero
+    // a row that sees nothing is zero; one whose every score is -inf has no weights, 0 / 0
+    const float inv = l == 0.f ? 0.f : 1.f / l, start = __any_sync(0xffffffffu, any) && l == 0.f ? NAN : 0.f;
     float acc[8];  // dimensions lane, lane + 32, ... of at most 256
 #pragma unroll
-    for (int x = 0; x < 8; x++) acc[x] = 0.f;
+    for (int x = 0; x < 8; x++) acc[x] = start;
     for (int j0 = 0; j0 < end; j0 += 32) {
         const float s = score(j0 + lane);
         // NaN scores stay NaN.  Divided here, so that the sum stays below the largest value.
@@ -139,6 +142,43 @@ __device__ __noinline__ void row_by_warp(const AttnP &p, int b, int h, int i) {
 #pragma unroll
     for (int x = 0; x < 8; x++)
         if (lane + 32 * x < p.dim) o[lane + 32 * x] = from_f<T>(acc[x]);
+}
+
+// Whether row i may see a key, as far as its lengths and its own document tell.
+__device__ __forceinline__ bool may_see(const AttnP &p, const Span &s, int b, int i) {
+    return i >= 0 && key_end(p, s, i) > 0 && (!p.q_docs || p.q_docs[b * p.qds + i] >= 0);
+}
+// A document that is not among the first `end` keys.
+struct Absent {
+    int doc = -1, end = 0;
+};
+// row_by_warp for a row whose sums are not finite, or whose weights are all zero although it may see keys: where a
+// document has no keys (rows of padding, a run of one document) one look at the ids serves all of them, so the
+// rows of a block come last to first.
+template <typename T>
+__device__ __noinline__ Absent row_again(const AttnP &p, int b, int h, int i, Absent none) {
+    if (p.q_docs) {
+        const int lane = threadIdx.x & 31, doc = p.q_docs[b * p.qds + i], end = key_end(p, span_of(p, b), i);
+        const int *ids = p.kv_docs + b * p.kds;
+        bool in = false;
+        if (doc >= 0 && !(doc == none.doc && end <= none.end))
+            for (int j0 = lane; j0 - lane < end && !in; j0 += 256) {
+                int d[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++) d[x] = j0 + x * 32 < end ? ids[j0 + x * 32] : -1;
+#pragma unroll
+                for (int x = 0; x < 8; x++) in |= d[x] == doc;
+                in = __any_sync(0xffffffffu, in);
+            }
+        if (!in) {
+            if (doc >= 0 && !(doc == none.doc && end <= none.end)) none = {doc, end};
+            T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)i * p.os[2];
+            for (int d = lane; d < p.dim; d += 32) o[d] = from_f<T>(0.f);
+            return none;
+        }
+    }
+    row_by_warp<T>(p, b, h, i);
+    return none;
 }
 
 // ---- warp matrix instructions (16 x 8 x 16, fp32 accumulators) -----------------------------
@@ -217,7 +257,7 @@ struct PartSums {
 };
 struct JoinSmem {
     float weight[512], l[512];  // per part and row of the cluster: maximum, then share; sum
-    uint8_t odd[64];            // rows whose sums are not finite
+    uint8_t odd[64];            // rows to work out again
 };
 
 // The parts of a cluster's blocks, joined and stored.  Four warps of a block wrote parts[warp]:
@@ -250,6 +290,7 @@ __device__ __forceinline__ void join_parts(const AttnP &p, int b, PartSums<DP> *
             js.weight[x * ROWS + r] = f;
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (l == 0.f && rank == 0) js.odd[r] = may_see(p, span_of(p, b), b, query(r));
         for (int x = 0; x < n; x++) js.weight[x * ROWS + r] *= inv;
     }
     __syncthreads();
@@ -271,8 +312,9 @@ __device__ __forceinline__ void join_parts(const AttnP &p, int b, PartSums<DP> *
         ((T *)p.o)[b * p.os[0] + head(r) * p.os[1] + (int64_t)i * p.os[2] + d] = from_f<T>(v);
     }
     cl.sync();  // the parts are read until here; non-finite rows are written after the others
-    for (int r = threadIdx.x >> 5; r < ROWS; r += 4)
-        if (js.odd[r] && query(r) >= 0) row_by_warp<T>(p, b, head(r), query(r));
+    Absent none;
+    for (int r = ROWS - 1 - (threadIdx.x >> 5); r >= 0; r -= 4)
+        if (js.odd[r] && query(r) >= 0) none = row_again<T>(p, b, head(r), query(r), none);
 }
 
 // Blocks of `kernel` that an SM holds at a time, or four: more do not read faster.

@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
     T *ob = (T *)p.o + b * p.os[0];
     if (!FEW && cs == 1) {
         const float v0 = l0 == 0.f ? 0.f : 1.f / l0, v1 = l1 == 0.f ? 0.f : 1.f / l1;
-        bool bad0 = false, bad1 = false;
+        bool bad0 = l0 == 0.f && may_see(p, sp, b, i0), bad1 = l1 == 0.f && may_see(p, sp, b, i1);
 #pragma unroll
         for (int n = 0; n < DP / 8; n++)
 #pragma unroll
@@ -411,8 +411,9 @@ __global__ void __launch_bounds__(128) k_attn_tiles(const __grid_constant__ Attn
         if (bad0) js.odd[r0] = 1;
         if (bad1) js.odd[r1] = 1;
         __syncwarp();
-        for (int r = wr; r < wr + 16; r++)
-            if (js.odd[r] && row_query(r) >= 0) row_by_warp<T>(p, b, hq, row_query(r));
+        Absent none;
+        for (int r = wr + 15; r >= wr; r--)
+            if (js.odd[r] && row_query(r) >= 0) none = row_again<T>(p, b, hq, row_query(r), none);
         return;
     }
     __syncthreads();  // the tiles have been read: their place holds the parts now

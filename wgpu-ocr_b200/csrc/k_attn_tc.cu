@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
             tc_fence_after();
             if (!SPLIT) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                bool bad = !finite(l);
+                bool bad = !finite(l) || (l == 0.f && end > 0);
                 // rows through shared memory (the queries' tile is done with), 16-byte pieces XORed with the
                 // row against bank conflicts, so that a warp's stores cover whole rows
                 T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)(i - lane) * p.os[2];
@@ -618,11 +618,12 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
                 }
                 __syncwarp();
                 uint32_t rows = __ballot_sync(0xffffffffu, bad && row);
+                Absent none;
                 while (rows) {
-                    const int r = __ffs(rows) - 1;
-                    rows &= rows - 1;
+                    const int r = 31 - __clz(rows);
+                    rows ^= 1u << r;
                     __syncwarp();
-                    row_by_warp<T>(p, b, h, i - lane + r);
+                    none = row_again<T>(p, b, h, i - lane + r, none);
                 }
             }
         }
@@ -661,7 +662,8 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
         tc_fence_before();
         cl.sync();
         // a warp per row, the rows shared out
-        for (int r = rank * (kThreads / 32) + warp; r < 128 * NT; r += cs * (kThreads / 32)) {
+        Absent none;
+        for (int r = 128 * NT - 1 - rank * (kThreads / 32) - warp; r >= 0; r -= cs * (kThreads / 32)) {
             const int at = i_first + r;
             if (at >= sp.nq) continue;
             float top = -INFINITY, total = 0.f, share[8];
@@ -676,7 +678,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
                 total = fmaf(share[c], of[1], total);
             }
             const float inv = total == 0.f ? 0.f : 1.f / total;
-            bool bad = !finite(total);
+            bool bad = !finite(total) || (total == 0.f && may_see(p, sp, b, at));
             T *o = (T *)p.o + b * p.os[0] + h * p.os[1] + (int64_t)at * p.os[2];
             if (lane * 4 < p.dim) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__(threads_of(NT), 3 - NT)
                 for (int x = 0; x < 4; x++) o[lane * 4 + x] = from_f<T>(e[x]);
             }
             __syncwarp();
-            if (__any_sync(0xffffffffu, bad)) row_by_warp<T>(p, b, h, at);
+            if (__any_sync(0xffffffffu, bad)) none = row_again<T>(p, b, h, at, none);
         }
         cl.sync();  // the sums are read until here
     }
