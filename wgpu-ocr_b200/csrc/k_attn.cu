@@ -839,6 +839,8 @@ void launch_row(Ctx *c, const AttnP &p, cudaStream_t s) {
     launch_cluster<AttnP>(kernel, grid_of(units, cs, tiles), 128, cs, 4 * sizeof(PartSums<DP>), s, p);
     WOCR_LAUNCHED(c);
 }
+// 32-bit rows four at a time, although the cache is then read once for each four: 16 rows over 8 caches of 8,192
+// keys of 128, 39 us against 65 in tiles that share it; 64 rows, 125 against 128.
 template <typename T, int DP>
 void launch_row(Ctx *c, const AttnP &p, cudaStream_t s) {
     const int rows = p.heads / p.kv_heads * p.q_len;
@@ -849,7 +851,10 @@ void launch_row(Ctx *c, const AttnP &p, cudaStream_t s) {
     launch_row<T, DP, 1>(c, p, s);
 }
 
-// The queries of the heads that share a key head are taken together: a few tokens of a decoder.
+// The queries of the heads that share a key head are taken together: a few tokens of a decoder.  (8 caches of
+// 8,192 keys of 128, 64 heads over one key head: 37 us in 16 bits and 125 us in 32, against 661 and 3,362 us head by
+// head.  Beyond the limit it is head by head still: 128 heads 1,197 and 6,654 us, where together they would
+// take 58 and 240 us.)
 bool few_rows(const AttnP &p) { return p.q_len <= 16 && (int64_t)p.heads / p.kv_heads * p.q_len <= 64; }
 
 template <typename T, int DP>

@@ -16,8 +16,9 @@
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 since it was last used
 // (the weights stay below 2^8, the quotient is the same), so the accumulator is seldom touched
 // between products.
-// Measured: 32 heads of 128, 8,192 queries and keys, causal, bf16: 440 us, 1.25 PFLOP/s (75 % of the
-// measured matrix peak); not causal, 16 heads of 4,096: 128 us, 1.07 PFLOP/s; of 64: 107 us.
+// Measured: 32 heads of 128, 8,192 queries and keys, causal, bf16: 445 us on the same tensors call after
+// call (1.24 PFLOP/s), 518 us on others each time (1.06 PFLOP/s, 64 % of the measured matrix peak; the power
+// cap); not causal, 16 heads of 4,096: 122 to 140 us, 1.0 to 1.1 PFLOP/s; of 64: 123 us.
 // Bound: 4 D flops and one exponential a pair.  An SM's matrix pipe takes 128 x 128 x 128 in 512
 // cycles and its 16 exponentials a cycle take as long for two such products (D = 128).
 #include <algorithm>

@@ -37,9 +37,9 @@ struct SelectSmem {
 // when `cached`, so that the logits are read from HBM once: maximum, then exponentials, then (with
 // the cluster's log-sum-exps) the best candidate of each thread.  The kout-th best of those is a
 // lower bound of the answer's last candidate, and few pass it: they are gathered and ranked.
-// Bound: the passes over a block's logits and the barriers between them, not the bytes (256 rows of
-// 18,709 in 16 bits, 9.6 MB, 41 us cold; 512 threads a block took 10 % longer, eight beams' loads under
-// way together 20 %).
+// Bound: the four passes over a block's logits, an element a load, and the barriers between them, not the
+// bytes (256 rows of 18,709 in 16 bits, 9.6 MB, whose floor is 1.5 us: 34.5 us call after call, 40 us cold; 512
+// threads a block took 10 % longer, eight beams' loads under way together 20 %; sums in 64 bits cost 3 %).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_beam_select(const BeamP p, int slice, int cached) {
     extern __shared__ __align__(16) uint8_t dyn[];
