@@ -494,10 +494,11 @@ int32_t wocr_beam_reorder(wocr_ctx *ctx, const int32_t *parents, int32_t batch, 
  * to such multiples), ties to texts kept before texts grown, in the order of their beams, then of
  * classes.  Masses are held in 64 bits, logits taken from their step's largest: what a step adds to
  * all classes alike changes nothing, and among texts 2^22 or more below the best, whose differences
- * 64 bits no longer hold to 2^-30, ties may go to the larger logit before the lower class.  Outputs, the best `paths` texts of each line: tokens [lines][paths][steps], -1 past
- * a text's end, lengths and scores (log mass) [lines][paths]; a path that does not exist has
- * length 0 and score -inf.  Logits are cleaned as in wocr_beam_select.  The call's workspace comes
- * from the device's stream-ordered pool, on `stream`. */
+ * 64 bits no longer hold to 2^-30, ties may go to the larger logit before the lower class.
+ * Outputs, the best `paths` texts of each line: tokens [lines][paths][steps], -1 past a text's
+ * end, lengths and scores (log mass) [lines][paths]; a path that does not exist has length 0 and
+ * score -inf.  Logits are cleaned as in wocr_beam_select.  The call's workspace comes from the
+ * device's stream-ordered pool, on `stream`. */
 int32_t wocr_ctc_beam(wocr_ctx *ctx, const void *logits, int32_t type, int32_t lines, int32_t steps, int32_t classes,
                       int64_t line_stride, int64_t step_stride, const int32_t *lens, int32_t width, int32_t blank,
                       int32_t paths, int32_t *tokens, int32_t *lengths, float *scores, void *stream);
